@@ -451,6 +451,72 @@ int qr_oblivious_upload(qr_ctx *ctx, const uint32_t *feat, const float *thr,
 int qr_oblivious_score(qr_ctx *ctx, const float *rowmajor, size_t N, size_t F,
                        double *scores_out, float *kernel_ms);
 
+/* ---- dense operators ---------------------------------------------------------*/
+/* What a NEURAL document scorer needs beside the lambda pass: layer norm, dropout  */
+/* and the gated feed-forward unit, with their gradients (the reference has no such  */
+/* scorer; quickrank_amd/neural.py is the one built on these).                       */
+/*   - stateless: device, stream (a hipStream_t, NULL = HIP's default stream) and    */
+/*     workspace come with the call, which enqueues and returns; nothing is kept, so  */
+/*     several threads and captured graphs may call at once.  Two calls in flight at  */
+/*     the same time need two workspaces                                              */
+/*   - all matrices are row-major device memory on `device`, elements of `type`,       */
+/*     `ld` = elements from one row to the next (inputs: any, 0 broadcasts a row;       */
+/*     outputs: at least a row).  Sums, statistics and products are held in 32 bits,    */
+/*     every output is rounded once.  No alignment beyond the element's own is needed;  */
+/*     16 bytes (base and stride) is faster                                             */
+/*   - rows == 0 is no work (sums over rows are then written as zeros); no columns,     */
+/*     unknown codes, missing pointers, a short workspace: QR_ERR_ARG before any launch  */
+/*   - the message of a failed call: qr_last_error(NULL) on the calling thread           */
+/*   - results do not depend on timing: no atomics, joins in a fixed order               */
+#define QR_F32 0
+#define QR_BF16 1
+#define QR_F16 2
+#define QR_ACT_SILU 0      /* g / (1 + exp(-g))                                  */
+#define QR_ACT_GELU 1      /* g (1 + erf(g / sqrt 2)) / 2                        */
+#define QR_ACT_GELU_TANH 2 /* its tanh form, 0.044715                            */
+#define QR_ACT_RELU 3      /* max(g, 0), derivative 0 at 0                       */
+#define QR_ACT_SIGMOID 4   /* 1 / (1 + exp(-g))                                  */
+
+/* y = (x - mean) rstd weight + bias over rows of `cols`, rstd = 1 / sqrt(var + eps),  */
+/* the variance that of the row itself (divided by cols).  weight / bias: NULL = 1 / 0, */
+/* of param_type (`type` or QR_F32).  mean / rstd: f32 [rows] or NULL.  y may be x.     */
+int qr_layer_norm_async(int device, void *hip_stream, int type, int param_type, size_t rows, size_t cols,
+                        const void *x, size_t ldx, const void *weight, const void *bias, float eps,
+                        void *y, size_t ldy, float *mean, float *rstd);
+/* dx (NULL = skip; may be dy or x), dweight, dbias [cols] of param_type (NULL = skip)   */
+/* from the forward pass's mean and rstd.                                                */
+int qr_layer_norm_backward_workspace(size_t rows, size_t cols, size_t *bytes);
+int qr_layer_norm_backward_async(int device, void *hip_stream, int type, int param_type, size_t rows, size_t cols,
+                                 const void *dy, size_t lddy, const void *x, size_t ldx, const void *weight,
+                                 const float *mean, const float *rstd, void *dx, size_t lddx, void *dweight,
+                                 void *dbias, void *workspace, size_t workspace_bytes);
+
+/* y = residual + (kept ? x / (1 - p) : 0); residual NULL = 0.  Element i = row * cols +  */
+/* column is kept iff 16 bits of a 64-bit word of (seed, offset + i / 4) reach p: a pure   */
+/* function of its arguments, no mask is stored, and the gradient of x is the same call on  */
+/* dy (that of the residual is dy).  p is used as floor(65536 p + 0.5) / 65536, in the       */
+/* scale too; p = 1 drops everything.  A call uses ceil(rows * cols / 4) words from `offset`: */
+/* the next one of the same seed starts behind them.  counter: NULL, or a word in device      */
+/* memory that is added to `offset` when the kernel runs, so that a captured graph draws a new */
+/* mask at each replay.  y may be x or residual.                                               */
+int qr_dropout_async(int device, void *hip_stream, int type, size_t rows, size_t cols, const void *x, size_t ldx,
+                     const void *residual, size_t ldr, void *y, size_t ldy, double p, uint64_t seed,
+                     uint64_t offset, const uint64_t *counter);
+
+/* h [m][n] = act(x w_gate^T) * (x w_up^T); x [m][k], weights [n][k] of stride ldw.        */
+/* gate / up: NULL (serving), or [m][n] contiguous: the two products, rounded to `type`,    */
+/* for the backward pass.  Outputs must not overlap each other or an input.                 */
+int qr_gated_ffn_async(int device, void *hip_stream, int type, int act, size_t m, size_t k, size_t n,
+                       const void *x, size_t ldx, const void *w_gate, const void *w_up, size_t ldw, void *h,
+                       size_t ldh, void *gate, void *up);
+/* dx [m][k] (NULL = skip), dw_gate, dw_up [n][k] contiguous (both or neither).  The         */
+/* gradients of the two products pass through the workspace rounded to `type`.               */
+int qr_gated_ffn_backward_workspace(int type, size_t m, size_t k, size_t n, size_t *bytes);
+int qr_gated_ffn_backward_async(int device, void *hip_stream, int type, int act, size_t m, size_t k, size_t n,
+                                const void *dh, size_t lddh, const void *x, size_t ldx, const void *w_gate,
+                                const void *w_up, size_t ldw, const void *gate, const void *up, void *dx,
+                                size_t lddx, void *dw_gate, void *dw_up, void *workspace, size_t workspace_bytes);
+
 /* ---- instrumentation ---------------------------------------------------------*/
 /* HIP-event timing of the dominant kernel (root histogram build) accumulated    */
 /* since the last reset: launches, total ms, algorithmic bytes per launch.       */

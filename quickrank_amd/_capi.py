@@ -50,6 +50,8 @@ SYMBOLS = [
     "qr_ensemble_set_depth_order", "qr_bins_build_wide_with",
     "qr_bins_stats_wide", "qr_thresholds_from_stats_wide", "qr_tree_pending", "qr_debug_check",
     "qr_readback_retries",
+    "qr_layer_norm_async", "qr_layer_norm_backward_workspace", "qr_layer_norm_backward_async", "qr_dropout_async",
+    "qr_gated_ffn_async", "qr_gated_ffn_backward_workspace", "qr_gated_ffn_backward_async",
 ]
 
 _LIB = None
@@ -199,6 +201,15 @@ def lib():
     L.qr_tree_leaves_finish.argtypes = [vp, C.c_int, vp, C.POINTER(sz)]
     L.qr_doc_exchange_buffers.argtypes = [vp, C.POINTER(vp), C.POINTER(sz), C.POINTER(vp),
                                           C.POINTER(sz), C.POINTER(vp), C.POINTER(sz)]
+    i, psz = C.c_int, C.POINTER(sz)
+    L.qr_layer_norm_async.argtypes = [i, vp, i, i, sz, sz, vp, sz, vp, vp, C.c_float, vp, sz, vp, vp]
+    L.qr_layer_norm_backward_workspace.argtypes = [sz, sz, psz]
+    L.qr_layer_norm_backward_async.argtypes = [i, vp, i, i, sz, sz, vp, sz, vp, sz, vp, vp, vp, vp, sz, vp, vp, vp, sz]
+    L.qr_dropout_async.argtypes = [i, vp, i, sz, sz, vp, sz, vp, sz, vp, sz, C.c_double, u64, u64, vp]
+    L.qr_gated_ffn_async.argtypes = [i, vp, i, i, sz, sz, sz, vp, sz, vp, vp, sz, vp, sz, vp, vp]
+    L.qr_gated_ffn_backward_workspace.argtypes = [i, sz, sz, sz, psz]
+    L.qr_gated_ffn_backward_async.argtypes = [i, vp, i, i, sz, sz, sz, vp, sz, vp, sz, vp, vp, sz, vp, vp, vp, sz, vp, vp,
+                                              vp, sz]
     for s in SYMBOLS:
         fn = getattr(L, s)
         if s not in ("qr_ctx_destroy", "qr_last_error"):

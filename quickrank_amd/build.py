@@ -8,11 +8,12 @@ CSRC = os.path.join(HERE, "csrc")
 LIBDIR = os.path.join(HERE, "lib")
 LIB = os.environ.get("QR_HIP_LIB") or os.path.join(LIBDIR, "libqr_hip.so")
 SOURCES = ["qr_api.hip", "k_bins.hip", "k_lambda.hip", "k_tree.hip", "k_score.hip", "k_sample.hip",
-           "k_wide.hip", "k_exact.hip"]
+           "k_wide.hip", "k_exact.hip", "k_norm.hip", "k_drop.hip", "k_ffn.hip"]
 # a measurement aid, NOT part of the product library: the bare LDS atomic rate bench.py prices the
 # root histogram launch against (qr_prof_lds_atomic loads it from the product library's directory)
 UBENCH_SRC, UBENCH_LIB = "k_ubench.hip", os.path.join(LIBDIR, "libqr_ubench.so")
 HEADERS = [os.path.join(CSRC, "qr_internal.h"), os.path.join(CSRC, "qr_wave.h"), os.path.join(CSRC, "qr_dev.h"),
+           os.path.join(CSRC, "qr_dense.h"),
            os.path.join(HERE, "..", "include", "qr_hip.h")]
 # -ffp-contract=off: the reference's arithmetic is separate multiply/add
 # (SURVEY.md section 7 hard part 8); hipcc contracts by default.
@@ -36,7 +37,7 @@ def _stale():
 
 def build(force=False, verbose=False):
     """One object per .hip source (compiled side by side, only the stale ones), then the link:
-    a change to one kernel file costs that file's compile, not all eight."""
+    a change to one kernel file costs that file's compile, not all of them."""
     if not force and not _stale():
         build_ubench(verbose=verbose)
         return LIB

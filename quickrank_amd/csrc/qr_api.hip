@@ -11,9 +11,19 @@
 #include <atomic>
 #include <functional>
 
+#include "qr_dense.h"
 #include "qr_internal.h"
 
 static thread_local std::string g_create_err;
+
+// (the dense operators have no context: their messages are the calling thread's)
+int qr_dense_fail(int code, const char *what) noexcept {
+  try {
+    g_create_err = what;
+  } catch (...) {
+  }
+  return code;
+}
 
 // QR_POISON=1 (a debugging aid, tests/tools/abort_hunt.py --poison): every device allocation of the
 // library starts as 0xA5 bytes -- a read of something nobody wrote gives the same garbage in every

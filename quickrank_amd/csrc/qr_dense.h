@@ -1,0 +1,76 @@
+// qr_dense.h -- what the dense operators (k_norm.hip, k_drop.hip, k_ffn.hip) share: element types,
+// argument checks and the host side of a stateless launch.
+//
+// Unlike the calls that take a qr_ctx, these hold no state between calls: device, stream and
+// workspace come with each call, so calls of several threads and captured graphs have nothing in
+// common but what their caller shares.
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include <string>
+
+#include "../../include/qr_hip.h"
+
+// the calling thread's message, read with qr_last_error(NULL); never throws (qr_api.hip)
+int qr_dense_fail(int code, const char *what) noexcept;
+
+#define QR_DENSE_ARG(cond, msg) \
+  do {                          \
+    if (!(cond)) return qr_dense_fail(QR_ERR_ARG, msg); \
+  } while (0)
+
+// Makes the call's device current for as long as it lives and puts the caller's back.
+struct QrDeviceGuard {
+  int old = -1;
+  hipError_t err = hipSuccess;
+  explicit QrDeviceGuard(int device) {
+    int cur = -1;
+    err = hipGetDevice(&cur);
+    if (err == hipSuccess && cur != device) {
+      err = hipSetDevice(device);
+      if (err == hipSuccess) old = cur;
+    }
+  }
+  ~QrDeviceGuard() {
+    if (old >= 0) (void)hipSetDevice(old);
+  }
+};
+
+#define QR_DENSE_DEVICE(device)                                                              \
+  QrDeviceGuard _guard(device);                                                              \
+  if (_guard.err != hipSuccess) {                                                            \
+    (void)hipGetLastError();                                                                 \
+    return qr_dense_fail(_guard.err == hipErrorNoDevice ? QR_ERR_NO_DEVICE : QR_ERR_ARG,     \
+                         "the device cannot be made current (this library has no CPU fallback)"); \
+  }
+
+inline int qr_dense_launched(const char *what) noexcept {
+  const hipError_t e = hipGetLastError();
+  if (e == hipSuccess) return QR_OK;
+  return qr_dense_fail(QR_ERR_HIP, hipGetErrorString(e) ? hipGetErrorString(e) : what);
+}
+
+inline bool qr_dense_type_ok(int t) { return t == QR_F32 || t == QR_BF16 || t == QR_F16; }
+inline size_t qr_dense_size(int t) { return t == QR_F32 ? 4 : 2; }
+// bytes from the first to behind the last element of a [rows][cols] matrix of stride ld
+inline size_t qr_dense_span(size_t rows, size_t cols, size_t ld, size_t e) {
+  return rows && cols ? ((rows - 1) * ld + cols) * e : 0;
+}
+inline bool qr_dense_overlap(const void *p, size_t np, const void *q, size_t nq) {
+  const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
+  return p && q && np && nq && a < b + nq && b < a + np;
+}
+// rows * cols elements of stride ld stay far below 2^63 bytes
+inline bool qr_dense_fits(size_t rows, size_t cols, size_t ld) {
+  const size_t most = (size_t)1 << 58;
+  return cols < ((size_t)1 << 31) && (rows == 0 || (ld < most && cols < most && rows < most / ((ld > cols ? ld : cols) + 1)));
+}
+
+// `T` of a type code for a generic lambda: qr_dense_dispatch(type, [&](auto t) { using T = decltype(t); ... })
+template <class F>
+inline void qr_dense_dispatch(int type, F &&f) {
+  if (type == QR_F32) f(float{});
+  else if (type == QR_BF16) f(__bf16{});
+  else f(_Float16{});
+}

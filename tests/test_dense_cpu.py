@@ -1,0 +1,115 @@
+"""The dense operators' refusals: the C calls check their arguments before they touch a device, the Python
+calls refuse what is not on one."""
+import ctypes as C
+
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def L():
+    from quickrank_amd import build, _capi
+    build.build()
+    return _capi.lib()
+
+
+# (an address that is never followed: every call below is refused first)
+P, Q, R = 1 << 30, 1 << 31, 1 << 32
+ARG = 3
+
+
+def message(L):
+    return L.qr_last_error(None).decode()
+
+
+def norm(L, type=0, ptype=0, rows=4, cols=8, x=P, ldx=8, w=None, b=None, eps=1e-5, y=Q, ldy=8):
+    return L.qr_layer_norm_async(0, None, type, ptype, rows, cols, x, ldx, w, b, eps, y, ldy, None, None)
+
+
+@pytest.mark.parametrize("bad", [dict(type=3), dict(type=-1), dict(type=0, ptype=1), dict(type=1, ptype=2), dict(cols=0),
+                                 dict(cols=1 << 31, ldx=1 << 31, ldy=1 << 31), dict(rows=1 << 60), dict(ldx=1 << 60), dict(eps=-1.0),
+                                 dict(eps=float("nan")), dict(eps=float("inf")), dict(ldy=7), dict(x=None), dict(y=None)])
+def test_norm_refusals(L, bad):
+    assert norm(L, **bad) == ARG and message(L).startswith("layer norm")
+
+
+def norm_back(L, type=0, ptype=0, rows=4, cols=8, dy=P, lddy=8, x=Q, ldx=8, mean=P, rstd=P, dx=R, lddx=8, dw=P, ws=P, n=1 << 30):
+    return L.qr_layer_norm_backward_async(0, None, type, ptype, rows, cols, dy, lddy, x, ldx, None, mean, rstd, dx, lddx, dw, None,
+                                          ws, n)
+
+
+@pytest.mark.parametrize("bad", [dict(type=9), dict(type=2, ptype=1), dict(cols=0), dict(rows=1 << 60), dict(lddx=7), dict(dy=None),
+                                 dict(x=None), dict(mean=None), dict(rstd=None), dict(ws=None), dict(n=8)])
+def test_norm_backward_refusals(L, bad):
+    assert norm_back(L, **bad) == ARG and message(L).startswith("layer norm backward")
+
+
+def drop(L, type=0, rows=4, cols=8, x=P, ldx=8, r=None, ldr=0, y=Q, ldy=8, p=0.1):
+    return L.qr_dropout_async(0, None, type, rows, cols, x, ldx, r, ldr, y, ldy, p, 1, 0, None)
+
+
+@pytest.mark.parametrize("bad", [dict(type=7), dict(p=-1e-9), dict(p=1.0000001), dict(p=float("nan")), dict(rows=1 << 60),
+                                 dict(cols=1 << 31), dict(ldy=7), dict(x=None), dict(y=None), dict(r=P, ldr=1 << 60)])
+def test_dropout_refusals(L, bad):
+    assert drop(L, **bad) == ARG and message(L).startswith("dropout")
+
+
+def ffn(L, type=0, act=0, m=4, k=8, n=16, x=P, ldx=8, wg=Q, wu=R, ldw=8, h=R + Q, ldh=16, g=None, u=None):
+    return L.qr_gated_ffn_async(0, None, type, act, m, k, n, x, ldx, wg, wu, ldw, h, ldh, g, u)
+
+
+@pytest.mark.parametrize("bad", [dict(type=5), dict(act=5), dict(act=-1), dict(k=0), dict(n=0), dict(m=1 << 60), dict(ldh=15),
+                                 dict(g=P + Q), dict(u=P + Q), dict(x=None), dict(wg=None), dict(wu=None), dict(h=None), dict(h=P + 64),
+                                 dict(h=Q), dict(h=R + 128), dict(g=R + Q + 32, u=R + R), dict(g=R + R, u=R + R + 255),
+                                 dict(g=P, u=R + R)])
+def test_ffn_refusals(L, bad):
+    assert ffn(L, **bad) == ARG and message(L).startswith("gated ffn")
+
+
+def ffn_back(L, type=0, act=0, m=4, k=8, n=16, dh=P, lddh=16, x=Q, wg=R, wu=R + P, g=R + Q, u=2 * R, dx=2 * R + P, lddx=8,
+             dwg=2 * R + Q, dwu=3 * R, ws=3 * R + Q, nbytes=1 << 30):
+    return L.qr_gated_ffn_backward_async(0, None, type, act, m, k, n, dh, lddh, x, 8, wg, wu, 8, g, u, dx, lddx, dwg, dwu, ws, nbytes)
+
+
+@pytest.mark.parametrize("bad", [dict(type=5), dict(act=5), dict(k=0), dict(n=0), dict(m=1 << 60), dict(lddx=7), dict(dh=None),
+                                 dict(x=None), dict(wg=None), dict(wu=None), dict(g=None), dict(u=None), dict(dwg=None),
+                                 dict(dwu=None), dict(ws=None), dict(nbytes=64), dict(dx=Q), dict(dwg=R), dict(ws=2 * R),
+                                 dict(ws=3 * R - 64), dict(dwu=2 * R + Q + 64)])
+def test_ffn_backward_refusals(L, bad):
+    assert ffn_back(L, **bad) == ARG and message(L).startswith("gated ffn backward")
+
+
+def test_workspace_queries(L):
+    n = C.c_size_t(99)
+    assert L.qr_layer_norm_backward_workspace(0, 8, C.byref(n)) == 0 and n.value == 0
+    assert L.qr_layer_norm_backward_workspace(1000, 136, C.byref(n)) == 0 and n.value >= 2 * 136 * 4
+    assert L.qr_layer_norm_backward_workspace(4, 0, C.byref(n)) == ARG
+    assert L.qr_gated_ffn_backward_workspace(1, 100, 8, 16, C.byref(n)) == 0 and n.value >= 2 * 100 * 16 * 2
+    assert L.qr_gated_ffn_backward_workspace(1, 0, 8, 16, C.byref(n)) == 0
+    assert L.qr_gated_ffn_backward_workspace(4, 1, 8, 16, C.byref(n)) == ARG
+    assert L.qr_gated_ffn_backward_workspace(1, 1, 8, 16, None) == ARG
+    assert L.qr_layer_norm_backward_workspace(4, 8, None) == ARG
+
+
+def test_no_rows_is_no_work(L):
+    """Nothing is followed or launched: these hold where there is no device, too."""
+    assert norm(L, rows=0, x=None, y=None) == 0
+    assert drop(L, rows=0, x=None, y=None) == 0 and drop(L, cols=0) == 0
+    assert ffn(L, m=0, x=None, h=None) == 0
+
+
+def test_without_a_device(L):
+    if torch.cuda.is_available():
+        pytest.skip("a GPU is visible")
+    assert norm(L) in (1, ARG) and "device" in message(L)
+
+
+def test_python_refuses_host_tensors():
+    from quickrank_amd import QrError, dense
+    x, w = torch.zeros(4, 8), torch.zeros(6, 8)
+    for call in (lambda: dense.layer_norm(x), lambda: dense.dropout(x, 0.1, 1), lambda: dense.gated_ffn(x, w, w),
+                 lambda: dense.layer_norm_backward(x, x, None, x[:, 0], x[:, 0]),
+                 lambda: dense.gated_ffn_backward(x, x, w, w, x, x), lambda: dense.layer_norm([1.0]), lambda: dense.dropout(x.int(), 0.1, 1)):
+        with pytest.raises(QrError) as e:
+            call()
+        assert e.value.code == ARG
