@@ -505,10 +505,13 @@ int qr_dropout_async(int device, void *hip_stream, int type, size_t rows, size_t
 
 /* h [m][n] = act(x w_gate^T) * (x w_up^T); x [m][k], weights [n][k] of stride ldw.        */
 /* gate / up: NULL (serving), or [m][n] contiguous: the two products, rounded to `type`,    */
-/* for the backward pass.  Outputs must not overlap each other or an input.                 */
+/* for the backward pass.  Outputs must not overlap each other or an input.  The workspace   */
+/* is used (NULL, 0 will do otherwise) where a row of x or of a weight does not start at a    */
+/* 16-byte boundary: such matrices are copied to rows that do.                                */
+int qr_gated_ffn_workspace(int type, size_t m, size_t k, size_t n, size_t *bytes);
 int qr_gated_ffn_async(int device, void *hip_stream, int type, int act, size_t m, size_t k, size_t n,
                        const void *x, size_t ldx, const void *w_gate, const void *w_up, size_t ldw, void *h,
-                       size_t ldh, void *gate, void *up);
+                       size_t ldh, void *gate, void *up, void *workspace, size_t workspace_bytes);
 /* dx [m][k] (NULL = skip), dw_gate, dw_up [n][k] contiguous (both or neither).  The         */
 /* gradients of the two products pass through the workspace rounded to `type`.               */
 int qr_gated_ffn_backward_workspace(int type, size_t m, size_t k, size_t n, size_t *bytes);

@@ -51,7 +51,7 @@ SYMBOLS = [
     "qr_bins_stats_wide", "qr_thresholds_from_stats_wide", "qr_tree_pending", "qr_debug_check",
     "qr_readback_retries",
     "qr_layer_norm_async", "qr_layer_norm_backward_workspace", "qr_layer_norm_backward_async", "qr_dropout_async",
-    "qr_gated_ffn_async", "qr_gated_ffn_backward_workspace", "qr_gated_ffn_backward_async",
+    "qr_gated_ffn_workspace", "qr_gated_ffn_async", "qr_gated_ffn_backward_workspace", "qr_gated_ffn_backward_async",
 ]
 
 _LIB = None
@@ -206,7 +206,8 @@ def lib():
     L.qr_layer_norm_backward_workspace.argtypes = [sz, sz, psz]
     L.qr_layer_norm_backward_async.argtypes = [i, vp, i, i, sz, sz, vp, sz, vp, sz, vp, vp, vp, vp, sz, vp, vp, vp, sz]
     L.qr_dropout_async.argtypes = [i, vp, i, sz, sz, vp, sz, vp, sz, vp, sz, C.c_double, u64, u64, vp]
-    L.qr_gated_ffn_async.argtypes = [i, vp, i, i, sz, sz, sz, vp, sz, vp, vp, sz, vp, sz, vp, vp]
+    L.qr_gated_ffn_workspace.argtypes = [i, sz, sz, sz, psz]
+    L.qr_gated_ffn_async.argtypes = [i, vp, i, i, sz, sz, sz, vp, sz, vp, vp, sz, vp, sz, vp, vp, vp, sz]
     L.qr_gated_ffn_backward_workspace.argtypes = [i, sz, sz, sz, psz]
     L.qr_gated_ffn_backward_async.argtypes = [i, vp, i, i, sz, sz, sz, vp, sz, vp, sz, vp, vp, sz, vp, vp, vp, sz, vp, vp,
                                               vp, sz]

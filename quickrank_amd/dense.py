@@ -190,9 +190,14 @@ def gated_ffn(x, w_gate, w_up, act="silu", save=False):
     h = torch.empty(shape, dtype=x.dtype, device=x.device)
     g = torch.empty(shape, dtype=x.dtype, device=x.device) if save else None
     u = torch.empty(shape, dtype=x.dtype, device=x.device) if save else None
-    rc = lib().qr_gated_ffn_async(x.device.index, _stream(x), TYPES[x.dtype], a, m, k, n, x.data_ptr(), ldx, w_gate.data_ptr(),
-                                  w_up.data_ptr(), ldw, h.data_ptr(), n, g.data_ptr() if save else None,
-                                  u.data_ptr() if save else None)
+    px, pg, pu, e = x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), x.element_size()
+    ws, need, rc = None, C.c_size_t(), 0
+    if (px | pg | pu | ldx * e | ldw * e) & 15:  # rows that do not start at 16-byte boundaries
+        rc = lib().qr_gated_ffn_workspace(TYPES[x.dtype], m, k, n, C.byref(need))
+        ws = torch.empty(need.value, dtype=torch.uint8, device=x.device)
+    rc = rc or lib().qr_gated_ffn_async(x.device.index, _stream(x), TYPES[x.dtype], a, m, k, n, px, ldx, pg, pu, ldw, h.data_ptr(), n,
+                                        g.data_ptr() if save else None, u.data_ptr() if save else None,
+                                        ws.data_ptr() if ws is not None else None, need.value)
     if rc:
         _fail(rc)
     return (h, g, u) if save else h

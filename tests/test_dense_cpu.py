@@ -54,14 +54,16 @@ def test_dropout_refusals(L, bad):
     assert drop(L, **bad) == ARG and message(L).startswith("dropout")
 
 
-def ffn(L, type=0, act=0, m=4, k=8, n=16, x=P, ldx=8, wg=Q, wu=R, ldw=8, h=R + Q, ldh=16, g=None, u=None):
-    return L.qr_gated_ffn_async(0, None, type, act, m, k, n, x, ldx, wg, wu, ldw, h, ldh, g, u)
+def ffn(L, type=0, act=0, m=4, k=8, n=16, x=P, ldx=8, wg=Q, wu=R, ldw=8, h=R + Q, ldh=16, g=None, u=None, ws=None,
+        nbytes=0):
+    return L.qr_gated_ffn_async(0, None, type, act, m, k, n, x, ldx, wg, wu, ldw, h, ldh, g, u, ws, nbytes)
 
 
 @pytest.mark.parametrize("bad", [dict(type=5), dict(act=5), dict(act=-1), dict(k=0), dict(n=0), dict(m=1 << 60), dict(ldh=15),
                                  dict(g=P + Q), dict(u=P + Q), dict(x=None), dict(wg=None), dict(wu=None), dict(h=None), dict(h=P + 64),
                                  dict(h=Q), dict(h=R + 128), dict(g=R + Q + 32, u=R + R), dict(g=R + R, u=R + R + 255),
-                                 dict(g=P, u=R + R)])
+                                 dict(g=P, u=R + R), dict(x=P + 4), dict(ldx=9), dict(ldw=10), dict(wu=R + 8), dict(x=P + 4, ws=2 * R),
+                                 dict(x=P + 4, ws=2 * R, nbytes=256), dict(x=P + 4, ws=R, nbytes=1 << 20)])
 def test_ffn_refusals(L, bad):
     assert ffn(L, **bad) == ARG and message(L).startswith("gated ffn")
 
@@ -84,6 +86,8 @@ def test_workspace_queries(L):
     assert L.qr_layer_norm_backward_workspace(0, 8, C.byref(n)) == 0 and n.value == 0
     assert L.qr_layer_norm_backward_workspace(1000, 136, C.byref(n)) == 0 and n.value >= 2 * 136 * 4
     assert L.qr_layer_norm_backward_workspace(4, 0, C.byref(n)) == ARG
+    assert L.qr_gated_ffn_workspace(0, 100, 9, 16, C.byref(n)) == 0 and n.value >= (100 + 32) * 12 * 4
+    assert L.qr_gated_ffn_workspace(0, 100, 0, 16, C.byref(n)) == ARG
     assert L.qr_gated_ffn_backward_workspace(1, 100, 8, 16, C.byref(n)) == 0 and n.value >= 2 * 100 * 16 * 2
     assert L.qr_gated_ffn_backward_workspace(1, 0, 8, 16, C.byref(n)) == 0
     assert L.qr_gated_ffn_backward_workspace(4, 1, 8, 16, C.byref(n)) == ARG

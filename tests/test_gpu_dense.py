@@ -467,11 +467,13 @@ def test_outputs_of_longer_rows_leave_the_rest_alone(dense, dtype):
     assert L.qr_dropout_async(0, s, code, m, k, x.data_ptr(), k, None, 0, d.data_ptr(), k + 5, 0.25, 3, 4, None) == 0
     assert torch.equal(d, dense.dropout(x, 0.25, 3, 4)) and untouched(bd, m, k)
     bh, h = out(m, n, 2)
+    need = C.c_size_t()
+    assert L.qr_gated_ffn_workspace(code, m, k, n, C.byref(need)) == 0
+    ws = torch.empty(need.value, dtype=torch.uint8, device="cuda")
     assert L.qr_gated_ffn_async(0, s, code, 0, m, k, n, x.data_ptr(), k, wg.data_ptr(), wu.data_ptr(), k, h.data_ptr(), n + 2,
-                                None, None) == 0
+                                None, None, ws.data_ptr(), need.value) == 0
     hr, g, u = dense.gated_ffn(x, wg, wu, save=True)
     assert torch.equal(h, hr) and untouched(bh, m, n)
-    need = C.c_size_t()
     bx, dx = out(m, k, 7)
     assert L.qr_gated_ffn_backward_workspace(code, m, k, n, C.byref(need)) == 0
     ws = torch.empty(need.value, dtype=torch.uint8, device="cuda")
