@@ -18,21 +18,68 @@ __host__ __device__ __forceinline__ uint64_t mix64(uint64_t z) {
 }
 constexpr uint64_t WEYL = 0x9E3779B97F4A7C15ull;
 
-// one thread per word: four elements, which may lie in several rows
 template <class T>
-__global__ __launch_bounds__(256) void k_drop(const size_t rows, const size_t cols, const T *x, const size_t ldx, const T *res,
-                                              const size_t ldr, T *y, const size_t ldy, const uint32_t t, const float scale,
-                                              const uint64_t key, const uint64_t offset, const uint64_t *__restrict__ counter) {
+struct Raw {
+  T v[16 / sizeof(T)];
+};
+
+template <class T>
+__device__ __forceinline__ T dropped(const T x, const float r, const uint32_t bits, const uint32_t t, const float scale) {
+  return (T)((bits >= t ? (float)x * scale : 0.f) + r);
+}
+
+// rows without gaps: a thread takes pieces of 16 bytes of the whole, U of them under way at a time
+template <class T, bool RES, int U>
+__global__ __launch_bounds__(256) void k_drop_flat(const size_t n, const T *x, const T *res, T *y, const uint32_t t, const float scale,
+                                                   const uint64_t key, const uint64_t offset, const uint64_t *__restrict__ counter) {
+  constexpr int V = 16 / sizeof(T), W = V / 4;
+  const size_t pieces = (n + V - 1) / V, step = (size_t)gridDim.x * 256;
+  const uint64_t first = key + WEYL * (offset + (counter ? *counter : 0) + 1);
+  for (size_t p0 = (size_t)blockIdx.x * 256 + threadIdx.x; p0 < pieces; p0 += step * U) {
+    Raw<T> vx[U], vr[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const size_t at = (p0 + u * step) * V;
+      if (at + V <= n) {
+        __builtin_memcpy(&vx[u], x + at, 16);
+        if (RES) __builtin_memcpy(&vr[u], res + at, 16);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const size_t p = p0 + u * step, at = p * V;
+      if (at >= n) continue;
+      uint64_t bits[W];
+#pragma unroll
+      for (int w = 0; w < W; ++w) bits[w] = mix64(first + WEYL * (p * W + w));
+      if (at + V <= n) {
+        Raw<T> o;
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          o.v[e] = dropped(vx[u].v[e], RES ? (float)vr[u].v[e] : 0.f, (uint32_t)(bits[e / 4] >> (16 * (e % 4))) & 0xFFFF, t, scale);
+        __builtin_memcpy(y + at, &o, 16);
+      } else {
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (at + e < n)
+            y[at + e] = dropped(x[at + e], RES ? (float)res[at + e] : 0.f, (uint32_t)(bits[e / 4] >> (16 * (e % 4))) & 0xFFFF, t, scale);
+      }
+    }
+  }
+}
+
+// rows of a stride: one thread per word, four elements that may lie in several rows
+template <class T>
+__global__ __launch_bounds__(256) void k_drop_rows(const size_t rows, const size_t cols, const T *x, const size_t ldx, const T *res,
+                                                   const size_t ldr, T *y, const size_t ldy, const uint32_t t, const float scale,
+                                                   const uint64_t key, const uint64_t offset, const uint64_t *__restrict__ counter) {
   const size_t n = rows * cols, words = (n + 3) / 4;
   const uint64_t first = offset + (counter ? *counter : 0) + 1;
   for (size_t w = (size_t)blockIdx.x * 256 + threadIdx.x; w < words; w += (size_t)gridDim.x * 256) {
     const uint64_t bits = mix64(key + WEYL * (first + w));
     size_t r = w * 4 / cols, j = w * 4 - r * cols;
     for (int e = 0; e < 4 && w * 4 + e < n; ++e) {
-      const bool keep = (uint32_t)((bits >> (16 * e)) & 0xFFFF) >= t;
-      float v = keep ? (float)x[r * ldx + j] * scale : 0.f;
-      if (res) v += (float)res[r * ldr + j];
-      y[r * ldy + j] = (T)v;
+      y[r * ldy + j] = dropped(x[r * ldx + j], res ? (float)res[r * ldr + j] : 0.f, (uint32_t)(bits >> (16 * e)) & 0xFFFF, t, scale);
       if (++j == cols) j = 0, ++r;
     }
   }
@@ -53,12 +100,20 @@ extern "C" int qr_dropout_async(int device, void *stream, int type, size_t rows,
   QR_DENSE_DEVICE(device);
   const uint32_t t = (uint32_t)(p * 65536.0 + 0.5);
   const float scale = t < 65536 ? 65536.f / (float)(65536 - t) : 0.f;
-  const size_t words = (rows * cols + 3) / 4;
-  const unsigned grid = (unsigned)((words + 255) / 256 < 65536 ? (words + 255) / 256 : 65536);
+  const size_t n = rows * cols;
+  const bool flat = rows == 1 || (ldx == cols && ldy == cols && (!residual || ldr == cols));
+  const auto grid = [](size_t threads) { return (unsigned)((threads + 255) / 256 < 8192 ? (threads + 255) / 256 : 8192); };
   qr_dense_dispatch(type, [&](auto tt) {
     using T = decltype(tt);
-    k_drop<T><<<grid, 256, 0, (hipStream_t)stream>>>(rows, cols, (const T *)x, ldx, (const T *)residual, ldr, (T *)y, ldy, t, scale,
-                                                     mix64(seed), offset, counter);
+    const hipStream_t s = (hipStream_t)stream;
+    const unsigned pieces = grid((n + 16 / sizeof(T) - 1) / (16 / sizeof(T)));
+    if (flat && residual)
+      k_drop_flat<T, true, 2><<<pieces, 256, 0, s>>>(n, (const T *)x, (const T *)residual, (T *)y, t, scale, mix64(seed), offset, counter);
+    else if (flat)
+      k_drop_flat<T, false, 4><<<pieces, 256, 0, s>>>(n, (const T *)x, nullptr, (T *)y, t, scale, mix64(seed), offset, counter);
+    else
+      k_drop_rows<T><<<grid((n + 3) / 4), 256, 0, s>>>(rows, cols, (const T *)x, ldx, (const T *)residual, ldr, (T *)y, ldy, t, scale,
+                                                      mix64(seed), offset, counter);
   });
   return qr_dense_launched("dropout");
 }

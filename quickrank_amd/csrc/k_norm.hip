@@ -4,38 +4,305 @@
 //   xh_j = (x_j - mu) r,  g_j = dy_j w_j
 //   dx_j = r (g_j - mean(g) - xh_j mean(g xh)),  dw_j = sum_rows dy_j xh_j,  db_j = sum_rows dy_j
 //
-// Statistics and sums are held in 32 bits; outputs are rounded once.
+// Statistics and sums are held in 32 bits; outputs are rounded once.  Bound by memory: a row is read once, kept
+// in the registers of G lanes (16 for short rows, a wave, or a workgroup of four) as pieces of 16 bytes, and the
+// variance is taken from the mean, not from the squares.  The backward pass reads a row of dy and of x once for
+// dx and for the two column sums: a lane owns the same columns of every row its workgroup takes, adds them up in
+// registers, and the workgroups' sums are joined by a second launch in a fixed order.
+#include <type_traits>
+
 #include "qr_dense.h"
 
 namespace {
 
-__device__ __forceinline__ float wave_sum_f(float v) {
-  for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
-  return v;
+template <int CTRL>
+__device__ __forceinline__ float dpp(const float v) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float lane_of(const float v, const int l) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l));
+}
+// sums over groups of G lanes, in a fixed order: every lane gets its group's (G = 256: the workgroup's, through `lds`)
+template <int G, int K>
+__device__ __forceinline__ void group_sum(float (&v)[K], float *lds) {
+#pragma unroll
+  for (int i = 0; i < K; ++i) {
+    v[i] += dpp<0xB1>(v[i]);   // quad_perm [1,0,3,2]
+    v[i] += dpp<0x4E>(v[i]);   // quad_perm [2,3,0,1]
+    v[i] += dpp<0x141>(v[i]);  // row_half_mirror
+    v[i] += dpp<0x140>(v[i]);  // row_mirror
+    if constexpr (G >= 64) v[i] = (lane_of(v[i], 0) + lane_of(v[i], 16)) + (lane_of(v[i], 32) + lane_of(v[i], 48));
+  }
+  if constexpr (G == 256) {
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0)
+#pragma unroll
+      for (int i = 0; i < K; ++i) lds[i * 4 + (threadIdx.x >> 6)] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < K; ++i) v[i] = (lds[i * 4] + lds[i * 4 + 1]) + (lds[i * 4 + 2] + lds[i * 4 + 3]);
+  }
 }
 
-// one wave per row
+// The pieces of a row that lane l of G holds: l, l + G, ...; the last piece of a row is moved back to end with the
+// row, so that every load and store is a whole one, and its first `dup` elements belong to the piece before it.
+template <class T, int G>
+struct Pieces {
+  static constexpr int V = 16 / sizeof(T);
+  int cols, last;  // columns; the last piece
+  __device__ __forceinline__ Pieces(int c) : cols(c), last((c - 1) / V) {}
+  // the pieces l + G i of all lanes lie inside the row, none of them the last
+  __device__ __forceinline__ bool inner(int i) const { return G * (i + 1) <= last; }
+  __device__ __forceinline__ bool any(int i, int l) const { return l + G * i <= last; }
+  __device__ __forceinline__ int at(int i, int l) const { return l + G * i < last ? (l + G * i) * V : cols - V; }
+  __device__ __forceinline__ int dup(int i, int l) const { return (l + G * i) * V - at(i, l); }
+};
+
+template <class T>
+struct Raw {
+  T v[16 / sizeof(T)];
+};
+template <class T>
+__device__ __forceinline__ Raw<T> load(const T *p) {
+  Raw<T> r;
+  __builtin_memcpy(&r, p, 16);
+  return r;
+}
+template <class P, int V>
+__device__ __forceinline__ void load_params(const P *p, const int at, const float none, float (&v)[V]) {
+  if (p) {
+    P t[V];
+    __builtin_memcpy(t, p + at, sizeof t);
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = (float)t[e];
+  } else {
+#pragma unroll
+    for (int e = 0; e < V; ++e) v[e] = none;
+  }
+}
+
+template <class T, class P, int G, int N>
+__global__ __launch_bounds__(256) void k_norm(const size_t rows, const int cols, const T *x, const size_t ldx, const P *__restrict__ w,
+                                              const P *__restrict__ b, const float eps, T *y, const size_t ldy,
+                                              float *__restrict__ mean, float *__restrict__ rstd) {
+  constexpr int V = Pieces<T, G>::V;
+  __shared__ float lds[4];
+  const Pieces<T, G> S(cols);
+  const int l = threadIdx.x % G;
+  const size_t mine = (size_t)blockIdx.x * (256 / G) + threadIdx.x / G, r = mine < rows ? mine : rows - 1;
+  Raw<T> raw[N];
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+    if (S.inner(i) || S.any(i, l)) raw[i] = load(x + r * ldx + S.at(i, l));
+  float s[1] = {0.f};
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (S.inner(i)) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) s[0] += (float)raw[i].v[e];
+    } else if (S.any(i, l)) {
+      const int dup = S.dup(i, l);
+#pragma unroll
+      for (int e = 0; e < V; ++e) s[0] += e >= dup ? (float)raw[i].v[e] : 0.f;
+    }
+  }
+  group_sum<G>(s, lds);
+  const float mu = s[0] / (float)cols;
+  s[0] = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (S.inner(i)) {
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float d = (float)raw[i].v[e] - mu;
+        s[0] = fmaf(d, d, s[0]);
+      }
+    } else if (S.any(i, l)) {
+      const int dup = S.dup(i, l);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const float d = e >= dup ? (float)raw[i].v[e] - mu : 0.f;
+        s[0] = fmaf(d, d, s[0]);
+      }
+    }
+  }
+  group_sum<G>(s, lds);
+  const float rs = 1.f / sqrtf(s[0] / (float)cols + eps);
+  if (mine >= rows) return;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    if (S.inner(i) || S.any(i, l)) {
+      const int at = S.at(i, l);
+      float vw[V], vb[V];
+      load_params<P, V>(w, at, 1.f, vw);
+      load_params<P, V>(b, at, 0.f, vb);
+      Raw<T> o;
+#pragma unroll
+      for (int e = 0; e < V; ++e) o.v[e] = (T)fmaf(((float)raw[i].v[e] - mu) * rs, vw[e], vb[e]);
+      __builtin_memcpy(y + r * ldy + at, &o, 16);
+    }
+  }
+  if (l == 0) {
+    if (mean) mean[r] = mu;
+    if (rstd) rstd[r] = rs;
+  }
+}
+
+// part: [workgroup][2][cols] column sums of the rows a workgroup took, or NULL
+template <class T, class P, int G, int N>
+__global__ __launch_bounds__(256) void k_norm_grad(const size_t rows, const int cols, const T *dy, const size_t lddy, const T *x,
+                                                   const size_t ldx, const P *__restrict__ w, const float *__restrict__ mean,
+                                                   const float *__restrict__ rstd, T *dx, const size_t lddx, float *__restrict__ part) {
+  constexpr int V = Pieces<T, G>::V, RPB = 256 / G;
+  __shared__ float lds[8];
+  const Pieces<T, G> S(cols);
+  const int l = threadIdx.x % G, grp = threadIdx.x / G;
+  const float inv = 1.f / (float)cols;
+  float sw[N][V], sb[N][V];
+#pragma unroll
+  for (int i = 0; i < N; ++i)
+#pragma unroll
+    for (int e = 0; e < V; ++e) sw[i][e] = sb[i][e] = 0.f;
+
+  // a row's pieces are on their way while the row before is worked on
+  Raw<T> nx[N], nd[N];
+  float nm = 0.f, nr = 0.f;
+  auto fetch = [&](const size_t first) {
+    const size_t want = first + grp, r = want < rows ? want : rows - 1;
+#pragma unroll
+    for (int i = 0; i < N; ++i)
+      if (S.inner(i) || S.any(i, l)) {
+        nx[i] = load(x + r * ldx + S.at(i, l));
+        nd[i] = load(dy + r * lddy + S.at(i, l));
+      }
+    nm = mean[r];
+    nr = rstd[r];
+  };
+  size_t first = (size_t)blockIdx.x * RPB;
+  if (first < rows) fetch(first);
+  for (; first < rows; first += (size_t)gridDim.x * RPB) {
+    Raw<T> vx[N], vd[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) vx[i] = nx[i], vd[i] = nd[i];
+    const float mu = nm, rs = nr;
+    const size_t r = first + grp;
+    const bool live = r < rows;
+    if (first + (size_t)gridDim.x * RPB < rows) fetch(first + (size_t)gridDim.x * RPB);
+    float s[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      if (!S.inner(i) && !S.any(i, l)) continue;
+      const int dup = S.inner(i) ? 0 : S.dup(i, l);
+      float vw[V];
+      load_params<P, V>(w, S.at(i, l), 1.f, vw);
+#pragma unroll
+      for (int e = 0; e < V; ++e) {
+        const bool on = live && e >= dup;
+        const float d = on ? (float)vd[i].v[e] : 0.f, h = on ? ((float)vx[i].v[e] - mu) * rs : 0.f, g = d * vw[e];
+        s[0] += on ? g : 0.f;
+        s[1] = fmaf(on ? g : 0.f, h, s[1]);
+        sw[i][e] = fmaf(d, h, sw[i][e]);
+        sb[i][e] += d;
+      }
+    }
+    if (dx) {
+      group_sum<G>(s, lds);
+      const float a = s[0] * inv, c = s[1] * inv;
+      if (live) {
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          if (!S.inner(i) && !S.any(i, l)) continue;
+          const int at = S.at(i, l);
+          float vw[V];
+          load_params<P, V>(w, at, 1.f, vw);
+          Raw<T> o;
+#pragma unroll
+          for (int e = 0; e < V; ++e)
+            o.v[e] = (T)(rs * (fmaf((float)vd[i].v[e], vw[e], -a) - ((float)vx[i].v[e] - mu) * rs * c));
+          __builtin_memcpy(dx + r * lddx + at, &o, 16);
+        }
+      }
+    }
+  }
+  if (!part) return;
+  // the groups of the workgroup one after the other (each column has one owner in a group)
+  extern __shared__ float sum[];
+  for (int g = 0; g < RPB; ++g) {
+    if (grp == g) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        if (!S.inner(i) && !S.any(i, l)) continue;
+        const int at = S.at(i, l), dup = S.inner(i) ? 0 : S.dup(i, l);
+#pragma unroll
+        for (int e = 0; e < V; ++e)
+          if (e >= dup) {
+            if (RPB == 1) {
+              part[(size_t)blockIdx.x * 2 * cols + at + e] = sw[i][e];
+              part[((size_t)blockIdx.x * 2 + 1) * cols + at + e] = sb[i][e];
+            } else {
+              sum[at + e] = (g ? sum[at + e] : 0.f) + sw[i][e];
+              sum[cols + at + e] = (g ? sum[cols + at + e] : 0.f) + sb[i][e];
+            }
+          }
+      }
+    }
+    if (RPB > 1) __syncthreads();
+  }
+  if (RPB > 1)
+    for (int j = threadIdx.x; j < 2 * cols; j += 256) part[(size_t)blockIdx.x * 2 * cols + j] = sum[j];
+}
+
+// 32 columns by 32 shares of the partial sums
+template <class P>
+__global__ __launch_bounds__(1024) void k_norm_join(const int cols, const int parts, const float *__restrict__ part, P *__restrict__ dw,
+                                                    P *__restrict__ db) {
+  __shared__ float lds[32][33];
+  const int c = threadIdx.x & 31, q = threadIdx.x >> 5;
+  const size_t j = (size_t)blockIdx.x * 32 + c, n = 2 * (size_t)cols;
+  float s = 0.f;
+  if (j < n)
+    for (int p = q; p < parts; p += 32) s += part[p * n + j];
+  lds[q][c] = s;
+  __syncthreads();
+  if (q == 0 && j < n) {
+    s = 0.f;
+    for (int i = 0; i < 32; ++i) s += lds[i][c];
+    if (j < (size_t)cols) {
+      if (dw) dw[j] = (P)s;
+    } else if (db) {
+      db[j - cols] = (P)s;
+    }
+  }
+}
+
+// ---- rows that no workgroup's registers hold (and rows of less than 16 bytes): read again for every step ----------
+
+// the sum over a workgroup of 256, in every thread
+__device__ __forceinline__ float block_sum(float v) {
+  __shared__ float lds[8];
+  float a[1] = {v};
+  group_sum<256>(a, lds);
+  return a[0];
+}
+
 template <class T, class P>
-__global__ __launch_bounds__(256) void k_norm(const size_t rows, const int cols, const T *__restrict__ x, const size_t ldx,
-                                              const P *__restrict__ w, const P *__restrict__ b, const float eps, T *__restrict__ y,
-                                              const size_t ldy, float *__restrict__ mean, float *__restrict__ rstd) {
-  const int lane = threadIdx.x & 63;
-  for (size_t r = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += (size_t)gridDim.x * 4) {
+__global__ __launch_bounds__(256) void k_norm_any(const size_t rows, const int cols, const T *x, const size_t ldx,
+                                                  const P *__restrict__ w, const P *__restrict__ b, const float eps, T *y,
+                                                  const size_t ldy, float *__restrict__ mean, float *__restrict__ rstd) {
+  for (size_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const T *xr = x + r * ldx;
     float s = 0.f;
-    for (int j = lane; j < cols; j += 64) s += (float)xr[j];
-    const float mu = wave_sum_f(s) / (float)cols;
-    float q = 0.f;
-    for (int j = lane; j < cols; j += 64) {
+    for (int j = threadIdx.x; j < cols; j += 256) s += (float)xr[j];
+    const float mu = block_sum(s) / (float)cols;
+    s = 0.f;
+    for (int j = threadIdx.x; j < cols; j += 256) {
       const float d = (float)xr[j] - mu;
-      q = fmaf(d, d, q);
+      s = fmaf(d, d, s);
     }
-    const float rs = 1.f / sqrtf(wave_sum_f(q) / (float)cols + eps);
-    for (int j = lane; j < cols; j += 64) {
-      const float h = ((float)xr[j] - mu) * rs;
-      y[r * ldy + j] = (T)fmaf(h, w ? (float)w[j] : 1.f, b ? (float)b[j] : 0.f);
-    }
-    if (lane == 0) {
+    const float rs = 1.f / sqrtf(block_sum(s) / (float)cols + eps);
+    for (int j = threadIdx.x; j < cols; j += 256)
+      y[r * ldy + j] = (T)fmaf(((float)xr[j] - mu) * rs, w ? (float)w[j] : 1.f, b ? (float)b[j] : 0.f);
+    if (threadIdx.x == 0) {
       if (mean) mean[r] = mu;
       if (rstd) rstd[r] = rs;
     }
@@ -43,28 +310,25 @@ __global__ __launch_bounds__(256) void k_norm(const size_t rows, const int cols,
 }
 
 template <class T, class P>
-__global__ __launch_bounds__(256) void k_norm_dx(const size_t rows, const int cols, const T *dy, const size_t lddy, const T *x,
-                                                 const size_t ldx, const P *__restrict__ w, const float *__restrict__ mean,
-                                                 const float *__restrict__ rstd, T *dx, const size_t lddx) {
-  const int lane = threadIdx.x & 63;
-  for (size_t r = (size_t)blockIdx.x * 4 + (threadIdx.x >> 6); r < rows; r += (size_t)gridDim.x * 4) {
+__global__ __launch_bounds__(256) void k_norm_grad_any(const size_t rows, const int cols, const T *dy, const size_t lddy, const T *x,
+                                                       const size_t ldx, const P *__restrict__ w, const float *__restrict__ mean,
+                                                       const float *__restrict__ rstd, T *dx, const size_t lddx) {
+  for (size_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const float mu = mean[r], rs = rstd[r];
     float a = 0.f, c = 0.f;
-    for (int j = lane; j < cols; j += 64) {
+    for (int j = threadIdx.x; j < cols; j += 256) {
       const float g = (float)dy[r * lddy + j] * (w ? (float)w[j] : 1.f), h = ((float)x[r * ldx + j] - mu) * rs;
       a += g;
       c = fmaf(g, h, c);
     }
-    a = wave_sum_f(a) / (float)cols;
-    c = wave_sum_f(c) / (float)cols;
-    for (int j = lane; j < cols; j += 64) {
+    a = block_sum(a) / (float)cols;
+    c = block_sum(c) / (float)cols;
+    for (int j = threadIdx.x; j < cols; j += 256) {
       const float g = (float)dy[r * lddy + j] * (w ? (float)w[j] : 1.f), h = ((float)x[r * ldx + j] - mu) * rs;
       dx[r * lddx + j] = (T)(rs * (g - a - h * c));
     }
   }
 }
-
-constexpr int PARTS = 256;  // shares of the rows whose column sums are joined in a second launch
 
 template <class T>
 __global__ __launch_bounds__(256) void k_norm_cols(const size_t rows, const int cols, const T *__restrict__ dy, const size_t lddy,
@@ -72,7 +336,7 @@ __global__ __launch_bounds__(256) void k_norm_cols(const size_t rows, const int 
                                                    const float *__restrict__ rstd, float *__restrict__ part) {
   const int j = blockIdx.x * 256 + threadIdx.x;
   if (j >= cols) return;
-  const size_t r0 = rows * blockIdx.y / PARTS, r1 = rows * (blockIdx.y + 1) / PARTS;
+  const size_t r0 = rows * blockIdx.y / gridDim.y, r1 = rows * (blockIdx.y + 1) / gridDim.y;
   float sw = 0.f, sb = 0.f;
   for (size_t r = r0; r < r1; ++r) {
     const float d = (float)dy[r * lddy + j];
@@ -83,17 +347,30 @@ __global__ __launch_bounds__(256) void k_norm_cols(const size_t rows, const int 
   part[(size_t)blockIdx.y * 2 * cols + cols + j] = sb;
 }
 
-template <class P>
-__global__ __launch_bounds__(256) void k_norm_join(const int cols, const int parts, const float *__restrict__ part, P *__restrict__ dw, P *__restrict__ db) {
-  const int j = blockIdx.x * 256 + threadIdx.x;
-  if (j >= cols) return;
-  float sw = 0.f, sb = 0.f;
-  for (int p = 0; p < parts; ++p) {
-    sw += part[(size_t)p * 2 * cols + j];
-    sb += part[(size_t)p * 2 * cols + cols + j];
-  }
-  if (dw) dw[j] = (P)sw;
-  if (db) db[j] = (P)sb;
+// The lanes and pieces a row is kept in: the fewest lanes of 16, 64 and 256 that hold it in four (16, by rows of up
+// to 1 KB) or eight pieces each; f(G, N), or false where no workgroup's registers do
+template <class F>
+bool by_row(size_t cols, size_t e, F &&f) {
+  using std::integral_constant;
+  const size_t v = 16 / e, n = (cols + v - 1) / v;
+  if (cols < v || n > 2048) return false;
+  if (n <= 16) f(integral_constant<int, 16>{}, integral_constant<int, 1>{});
+  else if (n <= 32) f(integral_constant<int, 16>{}, integral_constant<int, 2>{});
+  else if (n <= 48) f(integral_constant<int, 16>{}, integral_constant<int, 3>{});
+  else if (n <= 64) f(integral_constant<int, 16>{}, integral_constant<int, 4>{});
+  else if (n <= 128) f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
+  else if (n <= 256) f(integral_constant<int, 64>{}, integral_constant<int, 4>{});
+  else if (n <= 512) f(integral_constant<int, 64>{}, integral_constant<int, 8>{});
+  else if (n <= 1024) f(integral_constant<int, 256>{}, integral_constant<int, 4>{});
+  else f(integral_constant<int, 256>{}, integral_constant<int, 8>{});
+  return true;
+}
+
+// workgroups of a backward pass, whose column sums are joined: as many as the chip holds at a time, fewer for long
+// rows, whose sums are long too
+size_t parts_of(size_t rows, size_t cols) {
+  const size_t most = cols > 2048 ? 512 : 1024;
+  return rows < most ? rows : most;
 }
 
 }  // namespace
@@ -110,13 +387,19 @@ extern "C" int qr_layer_norm_async(int device, void *stream, int type, int param
   if (!rows) return QR_OK;
   QR_DENSE_ARG(x && y, "layer norm: x or y is NULL");
   QR_DENSE_DEVICE(device);
-  const unsigned grid = (unsigned)((rows + 3) / 4 < 4096 ? (rows + 3) / 4 : 4096);
+  const hipStream_t s = (hipStream_t)stream;
   qr_dense_dispatch(type, [&](auto t) {
     using T = decltype(t);
     auto go = [&](auto p) {
       using P = decltype(p);
-      k_norm<T, P><<<grid, 256, 0, (hipStream_t)stream>>>(rows, (int)cols, (const T *)x, ldx, (const P *)weight, (const P *)bias, eps,
-                                                         (T *)y, ldy, mean, rstd);
+      const bool fits = by_row(cols, sizeof(T), [&](auto G, auto N) {
+        constexpr size_t RPB = 256 / G();
+        k_norm<T, P, G(), N()><<<(unsigned)((rows + RPB - 1) / RPB), 256, 0, s>>>(rows, (int)cols, (const T *)x, ldx, (const P *)weight,
+                                                                                 (const P *)bias, eps, (T *)y, ldy, mean, rstd);
+      });
+      if (!fits)
+        k_norm_any<T, P><<<(unsigned)(rows < 65536 ? rows : 65536), 256, 0, s>>>(rows, (int)cols, (const T *)x, ldx, (const P *)weight,
+                                                                                (const P *)bias, eps, (T *)y, ldy, mean, rstd);
     };
     if (param_type == QR_F32) go(float{});
     else go(T{});
@@ -126,7 +409,7 @@ extern "C" int qr_layer_norm_async(int device, void *stream, int type, int param
 
 extern "C" int qr_layer_norm_backward_workspace(size_t rows, size_t cols, size_t *bytes) {
   QR_DENSE_ARG(bytes && cols > 0 && cols < ((size_t)1 << 31), "layer norm backward: bad size");
-  *bytes = rows ? (size_t)PARTS * 2 * cols * 4 : 0;
+  *bytes = parts_of(rows, cols) * 2 * cols * 4;
   return QR_OK;
 }
 
@@ -145,23 +428,33 @@ extern "C" int qr_layer_norm_backward_async(int device, void *stream, int type, 
   size_t need = 0;
   (void)qr_layer_norm_backward_workspace(rows, cols, &need);
   QR_DENSE_ARG(!sums || !rows || (workspace && workspace_bytes >= need), "layer norm backward: the workspace is too small");
+  if (!rows && !sums) return QR_OK;
   QR_DENSE_DEVICE(device);
   const hipStream_t s = (hipStream_t)stream;
-  const unsigned grid = (unsigned)((rows + 3) / 4 < 4096 ? (rows + 3) / 4 : 4096), cb = (unsigned)((cols + 255) / 256);
+  const unsigned parts = (unsigned)parts_of(rows, cols);
   qr_dense_dispatch(type, [&](auto t) {
     using T = decltype(t);
     auto go = [&](auto p) {
       using P = decltype(p);
+      float *const part = sums ? (float *)workspace : nullptr;
+      const bool fits = !rows || by_row(cols, sizeof(T), [&](auto G, auto N) {
+        constexpr size_t RPB = 256 / G();
+        const size_t want = (rows + RPB - 1) / RPB;
+        const unsigned grid = (unsigned)(want < parts ? want : parts);
+        k_norm_grad<T, P, G(), N()><<<grid, 256, RPB > 1 && sums ? 2 * cols * 4 : 0, s>>>(
+            rows, (int)cols, (const T *)dy, lddy, (const T *)x, ldx, (const P *)weight, mean, rstd, (T *)dx, lddx, part);
+        if (sums) k_norm_join<P><<<(unsigned)((2 * cols + 31) / 32), 1024, 0, s>>>((int)cols, (int)grid, part, (P *)dweight, (P *)dbias);
+      });
+      if (fits && rows) return;
       // (the column sums first: dx may be written over dy or x)
-      if (sums) {
-        if (rows)
-          k_norm_cols<T><<<dim3(cb, PARTS), 256, 0, s>>>(rows, (int)cols, (const T *)dy, lddy, (const T *)x, ldx, mean, rstd,
-                                                        (float *)workspace);
-        k_norm_join<P><<<cb, 256, 0, s>>>((int)cols, rows ? PARTS : 0, (const float *)workspace, (P *)dweight, (P *)dbias);
-      }
-      if (dx && rows)
-        k_norm_dx<T, P><<<grid, 256, 0, s>>>(rows, (int)cols, (const T *)dy, lddy, (const T *)x, ldx, (const P *)weight, mean, rstd,
-                                            (T *)dx, lddx);
+      if (rows && sums)
+        k_norm_cols<T><<<dim3((unsigned)((cols + 255) / 256), parts), 256, 0, s>>>(rows, (int)cols, (const T *)dy, lddy, (const T *)x,
+                                                                                  ldx, mean, rstd, part);
+      if (sums)
+        k_norm_join<P><<<(unsigned)((2 * cols + 31) / 32), 1024, 0, s>>>((int)cols, (int)parts, part, (P *)dweight, (P *)dbias);
+      if (rows && dx)
+        k_norm_grad_any<T, P><<<(unsigned)(rows < 65536 ? rows : 65536), 256, 0, s>>>(
+            rows, (int)cols, (const T *)dy, lddy, (const T *)x, ldx, (const P *)weight, mean, rstd, (T *)dx, lddx);
     };
     if (param_type == QR_F32) go(float{});
     else go(T{});
