@@ -22,7 +22,7 @@ __device__ __forceinline__ float dpp(const float v) {
 __device__ __forceinline__ float lane_of(const float v, const int l) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l));
 }
-// sums over groups of G lanes, in a fixed order: every lane gets its group's (G = 256: the workgroup's, through `lds`)
+// sums over groups of G lanes, in a fixed order: every lane gets its group's (G > 64: the workgroup's, through `lds`)
 template <int G, int K>
 __device__ __forceinline__ void group_sum(float (&v)[K], float *lds) {
 #pragma unroll
@@ -33,14 +33,19 @@ __device__ __forceinline__ void group_sum(float (&v)[K], float *lds) {
     v[i] += dpp<0x140>(v[i]);  // row_mirror
     if constexpr (G >= 64) v[i] = (lane_of(v[i], 0) + lane_of(v[i], 16)) + (lane_of(v[i], 32) + lane_of(v[i], 48));
   }
-  if constexpr (G == 256) {
+  if constexpr (G > 64) {
+    constexpr int W = G / 64;
     __syncthreads();
     if ((threadIdx.x & 63) == 0)
 #pragma unroll
-      for (int i = 0; i < K; ++i) lds[i * 4 + (threadIdx.x >> 6)] = v[i];
+      for (int i = 0; i < K; ++i) lds[i * W + (threadIdx.x >> 6)] = v[i];
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < K; ++i) v[i] = (lds[i * 4] + lds[i * 4 + 1]) + (lds[i * 4 + 2] + lds[i * 4 + 3]);
+    for (int i = 0; i < K; ++i) {
+      v[i] = 0.f;
+#pragma unroll
+      for (int j = 0; j < W; ++j) v[i] += lds[i * W + j];
+    }
   }
 }
 
@@ -150,11 +155,11 @@ __global__ __launch_bounds__(256) void k_norm(const size_t rows, const int cols,
 
 // part: [workgroup][2][cols] column sums of the rows a workgroup took, or NULL
 template <class T, class P, int G, int N>
-__global__ __launch_bounds__(256) void k_norm_grad(const size_t rows, const int cols, const T *dy, const size_t lddy, const T *x,
+__global__ __launch_bounds__(G > 256 ? G : 256) void k_norm_grad(const size_t rows, const int cols, const T *dy, const size_t lddy, const T *x,
                                                    const size_t ldx, const P *__restrict__ w, const float *__restrict__ mean,
                                                    const float *__restrict__ rstd, T *dx, const size_t lddx, float *__restrict__ part) {
-  constexpr int V = Pieces<T, G>::V, RPB = 256 / G;
-  __shared__ float lds[8];
+  constexpr int V = Pieces<T, G>::V, RPB = G > 256 ? 1 : 256 / G;
+  __shared__ float lds[32];
   const Pieces<T, G> S(cols);
   const int l = threadIdx.x % G, grp = threadIdx.x / G;
   const float inv = 1.f / (float)cols;
@@ -164,64 +169,63 @@ __global__ __launch_bounds__(256) void k_norm_grad(const size_t rows, const int 
 #pragma unroll
     for (int e = 0; e < V; ++e) sw[i][e] = sb[i][e] = 0.f;
 
-  // a row's pieces are on their way while the row before is worked on
+  // a row's pieces are on their way while the row before is worked on; a group without a row works on zeros
   Raw<T> nx[N], nd[N];
   float nm = 0.f, nr = 0.f;
   auto fetch = [&](const size_t first) {
-    const size_t want = first + grp, r = want < rows ? want : rows - 1;
+    const size_t r = first + grp;
+    if (r < rows) {
 #pragma unroll
-    for (int i = 0; i < N; ++i)
-      if (S.inner(i) || S.any(i, l)) {
-        nx[i] = load(x + r * ldx + S.at(i, l));
-        nd[i] = load(dy + r * lddy + S.at(i, l));
-      }
-    nm = mean[r];
-    nr = rstd[r];
+      for (int i = 0; i < N; ++i)
+        if (S.inner(i) || S.any(i, l)) {
+          nx[i] = load(x + r * ldx + S.at(i, l));
+          nd[i] = load(dy + r * lddy + S.at(i, l));
+        }
+      nm = mean[r];
+      nr = rstd[r];
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) nx[i] = nd[i] = Raw<T>{};
+      nm = nr = 0.f;
+    }
   };
   size_t first = (size_t)blockIdx.x * RPB;
   if (first < rows) fetch(first);
   for (; first < rows; first += (size_t)gridDim.x * RPB) {
-    Raw<T> vx[N], vd[N];
-#pragma unroll
-    for (int i = 0; i < N; ++i) vx[i] = nx[i], vd[i] = nd[i];
+    float h[N][V], g[N][V], s[2] = {0.f, 0.f};
     const float mu = nm, rs = nr;
     const size_t r = first + grp;
-    const bool live = r < rows;
-    if (first + (size_t)gridDim.x * RPB < rows) fetch(first + (size_t)gridDim.x * RPB);
-    float s[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < N; ++i) {
       if (!S.inner(i) && !S.any(i, l)) continue;
-      const int dup = S.inner(i) ? 0 : S.dup(i, l);
+      const int dup = S.dup(i, l);
       float vw[V];
       load_params<P, V>(w, S.at(i, l), 1.f, vw);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const bool on = live && e >= dup;
-        const float d = on ? (float)vd[i].v[e] : 0.f, h = on ? ((float)vx[i].v[e] - mu) * rs : 0.f, g = d * vw[e];
-        s[0] += on ? g : 0.f;
-        s[1] = fmaf(on ? g : 0.f, h, s[1]);
-        sw[i][e] = fmaf(d, h, sw[i][e]);
+        const float d = (float)nd[i].v[e];
+        h[i][e] = ((float)nx[i].v[e] - mu) * rs;
+        g[i][e] = d * vw[e];
+        const float once = e >= dup ? g[i][e] : 0.f;
+        s[0] += once;
+        s[1] = fmaf(once, h[i][e], s[1]);
+        // (what a moved-back piece adds up in its first `dup` columns is not read)
+        sw[i][e] = fmaf(d, h[i][e], sw[i][e]);
         sb[i][e] += d;
       }
     }
-    if (dx) {
-      group_sum<G>(s, lds);
-      const float a = s[0] * inv, c = s[1] * inv;
-      if (live) {
+    if (first + (size_t)gridDim.x * RPB < rows) fetch(first + (size_t)gridDim.x * RPB);
+    if (!dx) continue;
+    group_sum<G>(s, lds);
+    const float a = -rs * (s[0] * inv), c = -rs * (s[1] * inv);
+    if (r >= rows) continue;
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          if (!S.inner(i) && !S.any(i, l)) continue;
-          const int at = S.at(i, l);
-          float vw[V];
-          load_params<P, V>(w, at, 1.f, vw);
-          Raw<T> o;
+    for (int i = 0; i < N; ++i) {
+      if (!S.inner(i) && !S.any(i, l)) continue;
+      Raw<T> o;
 #pragma unroll
-          for (int e = 0; e < V; ++e)
-            o.v[e] = (T)(rs * (fmaf((float)vd[i].v[e], vw[e], -a) - ((float)vx[i].v[e] - mu) * rs * c));
-          __builtin_memcpy(dx + r * lddx + at, &o, 16);
-        }
-      }
+      for (int e = 0; e < V; ++e) o.v[e] = (T)fmaf(h[i][e], c, fmaf(g[i][e], rs, a));
+      __builtin_memcpy(dx + r * lddx + S.at(i, l), &o, 16);
     }
   }
   if (!part) return;
@@ -347,9 +351,10 @@ __global__ __launch_bounds__(256) void k_norm_cols(const size_t rows, const int 
   part[(size_t)blockIdx.y * 2 * cols + cols + j] = sb;
 }
 
-// The lanes and pieces a row is kept in: the fewest lanes of 16, 64 and 256 that hold it in four (16, by rows of up
-// to 1 KB) or eight pieces each; f(G, N), or false where no workgroup's registers do
-template <class F>
+// The lanes and pieces a row is kept in: f(G, N), or false where no workgroup's registers hold a row.  Forward, the
+// fewest lanes of 16, 64 and 256 that hold it in four (16: rows of up to 1 KB) or eight pieces each.  Backward, where
+// a piece also has column sums, at most two pieces but for rows of 1 KB and less.
+template <bool BACK, class F>
 bool by_row(size_t cols, size_t e, F &&f) {
   using std::integral_constant;
   const size_t v = 16 / e, n = (cols + v - 1) / v;
@@ -357,19 +362,29 @@ bool by_row(size_t cols, size_t e, F &&f) {
   if (n <= 16) f(integral_constant<int, 16>{}, integral_constant<int, 1>{});
   else if (n <= 32) f(integral_constant<int, 16>{}, integral_constant<int, 2>{});
   else if (n <= 48) f(integral_constant<int, 16>{}, integral_constant<int, 3>{});
-  else if (n <= 64) f(integral_constant<int, 16>{}, integral_constant<int, 4>{});
-  else if (n <= 128) f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
-  else if (n <= 256) f(integral_constant<int, 64>{}, integral_constant<int, 4>{});
-  else if (n <= 512) f(integral_constant<int, 64>{}, integral_constant<int, 8>{});
-  else if (n <= 1024) f(integral_constant<int, 256>{}, integral_constant<int, 4>{});
-  else f(integral_constant<int, 256>{}, integral_constant<int, 8>{});
+  else if constexpr (BACK) {
+    if (n <= 64) f(integral_constant<int, 64>{}, integral_constant<int, 1>{});
+    else if (n <= 128) f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
+    else if (n <= 256) f(integral_constant<int, 256>{}, integral_constant<int, 1>{});
+    else if (n <= 512) f(integral_constant<int, 256>{}, integral_constant<int, 2>{});
+    else if (n <= 1024) f(integral_constant<int, 1024>{}, integral_constant<int, 1>{});
+    else f(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
+  } else {
+    if (n <= 64) f(integral_constant<int, 16>{}, integral_constant<int, 4>{});
+    else if (n <= 128) f(integral_constant<int, 64>{}, integral_constant<int, 2>{});
+    else if (n <= 256) f(integral_constant<int, 64>{}, integral_constant<int, 4>{});
+    else if (n <= 512) f(integral_constant<int, 64>{}, integral_constant<int, 8>{});
+    else if (n <= 1024) f(integral_constant<int, 256>{}, integral_constant<int, 4>{});
+    else f(integral_constant<int, 256>{}, integral_constant<int, 8>{});
+  }
   return true;
 }
 
-// workgroups of a backward pass, whose column sums are joined: as many as the chip holds at a time, fewer for long
-// rows, whose sums are long too
-size_t parts_of(size_t rows, size_t cols) {
-  const size_t most = cols > 2048 ? 512 : 1024;
+// Workgroups of a backward pass, whose column sums are joined: as many as the registers let the chip hold at a time
+// (six of 256 threads a compute unit with one piece a lane, four with more, two of 1024).  65536 x 2048 bf16 by 768 /
+// 1024 / 1536 / 2048 workgroups: 200 / 188 / 183 / 218 us; 71291 x 1001 f16 (two pieces): 114 / 111 / 127 / 123 us.
+size_t parts_of(size_t rows, int lanes, int pieces) {
+  const size_t most = lanes > 256 ? 512 : pieces > 1 ? 1024 : 1536;
   return rows < most ? rows : most;
 }
 
@@ -392,7 +407,7 @@ extern "C" int qr_layer_norm_async(int device, void *stream, int type, int param
     using T = decltype(t);
     auto go = [&](auto p) {
       using P = decltype(p);
-      const bool fits = by_row(cols, sizeof(T), [&](auto G, auto N) {
+      const bool fits = by_row<false>(cols, sizeof(T), [&](auto G, auto N) {
         constexpr size_t RPB = 256 / G();
         k_norm<T, P, G(), N()><<<(unsigned)((rows + RPB - 1) / RPB), 256, 0, s>>>(rows, (int)cols, (const T *)x, ldx, (const P *)weight,
                                                                                  (const P *)bias, eps, (T *)y, ldy, mean, rstd);
@@ -409,7 +424,7 @@ extern "C" int qr_layer_norm_async(int device, void *stream, int type, int param
 
 extern "C" int qr_layer_norm_backward_workspace(size_t rows, size_t cols, size_t *bytes) {
   QR_DENSE_ARG(bytes && cols > 0 && cols < ((size_t)1 << 31), "layer norm backward: bad size");
-  *bytes = parts_of(rows, cols) * 2 * cols * 4;
+  *bytes = parts_of(rows, 1, 1) * 2 * cols * 4;
   return QR_OK;
 }
 
@@ -431,27 +446,27 @@ extern "C" int qr_layer_norm_backward_async(int device, void *stream, int type, 
   if (!rows && !sums) return QR_OK;
   QR_DENSE_DEVICE(device);
   const hipStream_t s = (hipStream_t)stream;
-  const unsigned parts = (unsigned)parts_of(rows, cols);
+  const unsigned any = (unsigned)parts_of(rows, 1024, 1);
   qr_dense_dispatch(type, [&](auto t) {
     using T = decltype(t);
     auto go = [&](auto p) {
       using P = decltype(p);
       float *const part = sums ? (float *)workspace : nullptr;
-      const bool fits = !rows || by_row(cols, sizeof(T), [&](auto G, auto N) {
-        constexpr size_t RPB = 256 / G();
-        const size_t want = (rows + RPB - 1) / RPB;
+      const bool fits = !rows || by_row<true>(cols, sizeof(T), [&](auto G, auto N) {
+        constexpr size_t RPB = G() > 256 ? 1 : 256 / G();
+        const size_t want = (rows + RPB - 1) / RPB, parts = parts_of(rows, G(), N());
         const unsigned grid = (unsigned)(want < parts ? want : parts);
-        k_norm_grad<T, P, G(), N()><<<grid, 256, RPB > 1 && sums ? 2 * cols * 4 : 0, s>>>(
+        k_norm_grad<T, P, G(), N()><<<grid, G() > 256 ? G() : 256, RPB > 1 && sums ? 2 * cols * 4 : 0, s>>>(
             rows, (int)cols, (const T *)dy, lddy, (const T *)x, ldx, (const P *)weight, mean, rstd, (T *)dx, lddx, part);
         if (sums) k_norm_join<P><<<(unsigned)((2 * cols + 31) / 32), 1024, 0, s>>>((int)cols, (int)grid, part, (P *)dweight, (P *)dbias);
       });
       if (fits && rows) return;
       // (the column sums first: dx may be written over dy or x)
       if (rows && sums)
-        k_norm_cols<T><<<dim3((unsigned)((cols + 255) / 256), parts), 256, 0, s>>>(rows, (int)cols, (const T *)dy, lddy, (const T *)x,
+        k_norm_cols<T><<<dim3((unsigned)((cols + 255) / 256), any), 256, 0, s>>>(rows, (int)cols, (const T *)dy, lddy, (const T *)x,
                                                                                   ldx, mean, rstd, part);
       if (sums)
-        k_norm_join<P><<<(unsigned)((2 * cols + 31) / 32), 1024, 0, s>>>((int)cols, (int)parts, part, (P *)dweight, (P *)dbias);
+        k_norm_join<P><<<(unsigned)((2 * cols + 31) / 32), 1024, 0, s>>>((int)cols, (int)any, part, (P *)dweight, (P *)dbias);
       if (rows && dx)
         k_norm_grad_any<T, P><<<(unsigned)(rows < 65536 ? rows : 65536), 256, 0, s>>>(
             rows, (int)cols, (const T *)dy, lddy, (const T *)x, ldx, (const P *)weight, mean, rstd, (T *)dx, lddx);
