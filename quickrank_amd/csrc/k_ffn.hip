@@ -9,6 +9,8 @@
 // read itself).  The forward pass interleaves blocks of 16 rows of Wg and of Wu in its second operand's tile,
 // so that one lane ends with g and u of the same outputs and the activation, the product and the rounding
 // need no second kernel.
+#include <type_traits>
+
 #include "qr_dense.h"
 
 namespace {
@@ -22,15 +24,32 @@ __device__ __forceinline__ void act_of(const int act, const float g, float &a, f
     const float cdf = 0.5f * (1.f + erff(g * 0.70710678118654752f));
     a = g * cdf;
     d = fmaf(g * 0.39894228040143268f, expf(-0.5f * g * g), cdf);
-  } else if (act == QR_ACT_GELU_TANH) {
-    const float c = 0.79788456080286536f, t = tanhf(c * (g + 0.044715f * g * g * g));
-    a = 0.5f * g * (1.f + t);
-    d = 0.5f * (1.f + t) + 0.5f * g * (1.f - t * t) * c * (1.f + 3.f * 0.044715f * g * g);
   } else {
-    const float s = 1.f / (1.f + expf(-g));
+    // gelu_tanh is g sigmoid(2 c (g + 0.044715 g^3)), c = sqrt(2 / pi).  The hardware's exp2 and reciprocal are good to
+    // one step of f32, the product in exp2's argument to |g| steps
+    const float c2 = 1.5957691216057308f, z = act == QR_ACT_GELU_TANH ? c2 * fmaf(0.044715f * g * g, g, g) : g;
+    const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * z));
     a = act == QR_ACT_SIGMOID ? s : g * s;
-    d = act == QR_ACT_SIGMOID ? s * (1.f - s) : s * (1.f + g * (1.f - s));
+    d = act == QR_ACT_SIGMOID ? s * (1.f - s)
+                              : fmaf(g * (act == QR_ACT_GELU_TANH ? c2 * fmaf(3.f * 0.044715f * g, g, 1.f) : 1.f), s * (1.f - s), s);
   }
+}
+
+template <int ACT>
+__device__ __forceinline__ void gated8_of(const float (&g)[8], const float (&u)[8], float (&h)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    float a, d;
+    act_of(ACT, g[e], a, d);
+    h[e] = a * u[e];
+  }
+}
+__device__ __forceinline__ void gated8(const int act, const float (&g)[8], const float (&u)[8], float (&h)[8]) {
+  if (act == QR_ACT_SILU) gated8_of<QR_ACT_SILU>(g, u, h);
+  else if (act == QR_ACT_GELU) gated8_of<QR_ACT_GELU>(g, u, h);
+  else if (act == QR_ACT_GELU_TANH) gated8_of<QR_ACT_GELU_TANH>(g, u, h);
+  else if (act == QR_ACT_RELU) gated8_of<QR_ACT_RELU>(g, u, h);
+  else gated8_of<QR_ACT_SIGMOID>(g, u, h);
 }
 
 typedef float f4 __attribute__((ext_vector_type(4)));
@@ -58,20 +77,22 @@ __device__ __forceinline__ f4 mma(const i4 a, const i4 b, f4 c) {
 }
 
 // ---- LDS tiles -----------------------------------------------------------------------------------------
-// A tile holds R rows (outputs) of KT = 128 / sizeof(T) summed elements in 128 R bytes, moved in pieces of 16.
+// A stage holds R rows (outputs) of KT = 128 / sizeof(T) summed elements in 128 R bytes, moved in pieces of 16.  A row's
+// 128 bytes are a whole line of the L2, whose requests, not its bytes, were the bound with rows of 64 (1159 against 1344
+// TFLOP/s at 8192 x 8192 x 4096 bf16).
 //
-// Rows layout: row r at 128 r, its piece c at position c ^ (r & 7): the 16 lanes that read the same piece of 16
-// consecutive rows touch every bank once.
+// Rows layout: row r at 128 r, its piece c at position c ^ (r & 7).  A 16-byte read of a wave is served in four parts,
+// lanes 0-3 12-15 20-27, 4-11 16-19 28-31 and the same 32 higher; the lanes of each touch every bank once.
 // Columns layout: summed element k at k R sizeof(T), its pieces XORed with col_swz(k) so that the lanes of one
 // read, which lie in 8 (16-bit) or 4 (f32) such lines, touch every bank once.
 template <class T, int R>
 __device__ __forceinline__ int col_swz(const int k) {
-  if constexpr (sizeof(T) == 4) return ((k >> 2) & 3) << 2;              // segments of 16 floats
+  if constexpr (sizeof(T) == 4) return ((k >> 2) & 3) << 2;                    // segments of 16 floats
   else if constexpr (R >= 128) return ((k & 3) | (((k >> 3) & 1) << 2)) << 1;  // segments of 16 elements = 32 bytes
-  else return (((k >> 1) & 1) | (((k >> 3) & 1) << 1)) << 1;              // two lines of 128 bytes share the banks
+  else return (((k >> 1) & 1) | (((k >> 3) & 1) << 1)) << 1;                   // two lines of 128 bytes share the banks
 }
 
-// the piece q (of R * 8) of a tile in LDS order -> where it comes from
+// the piece q (of R * 8) of a stage in LDS order -> where it comes from
 template <class T, int R, bool KS>
 __device__ __forceinline__ void piece_of(const int q, int &r, int &k) {
   constexpr int E = 16 / sizeof(T);
@@ -85,27 +106,35 @@ __device__ __forceinline__ void piece_of(const int q, int &r, int &k) {
   }
 }
 
-// one operand fragment: 16 rows from row16 * 16 on, the step-th half of the tile's summed dimension
+// One operand fragment: 16 rows of one half (0, 1) of a stage, the c-th block of 16 behind the wave's first (a multiple of
+// the blocks a wave has).  `at` is the LDS address frag_base gave for block 0 of half 0; in the columns layout a block's
+// number is XORed in, in the rows layout the half's.
 template <class T, int R, bool KS>
-__device__ __forceinline__ i4 frag(const char *lds, const int row16, const int step) {
+__device__ __forceinline__ uint32_t frag_base(const uint32_t stage, const int block) {
   const int l = threadIdx.x & 63, g = l >> 4, i = l & 15;
   if constexpr (!KS) {
-    return *(const i4 *)(lds + (row16 * 16 + i) * 128 + (((step * 4 + g) ^ (i & 7)) << 4));
+    return stage + (block * 16 + i) * 128 + ((g ^ (i & 7)) << 4);
   } else if constexpr (sizeof(T) == 2) {
-    const int k = step * 32 + 8 * g + (i >> 2);
-    const char *p = lds + k * (R * 2) + (((row16 * 2) ^ col_swz<T, R>(k)) << 4) + (i & 3) * 8;
+    const int k = 8 * g + (i >> 2);
+    return stage + ((k * (R * 2) + (col_swz<T, R>(k) << 4) + (i & 3) * 8) ^ (block << 5));
+  } else {
+    return stage + ((4 * g * (R * 4) + (col_swz<T, R>(4 * g) << 4) + i * 4) ^ (block << 6));
+  }
+}
+template <class T, int R, bool KS>
+__device__ __forceinline__ i4 frag(const uint32_t at, const int c, const int half) {
+  if constexpr (!KS) {
+    return *(QR_LDS const i4 *)((at ^ (half << 6)) + c * 2048);
+  } else if constexpr (sizeof(T) == 2) {
+    const uint32_t p = (at ^ (c << 5)) + half * (32 * R * 2);
     const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((QR_LDS s4 *)p);
     const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((QR_LDS s4 *)(p + 4 * R * 2));
-    i4 v;
-    __builtin_memcpy(&v, &lo, 8);
-    __builtin_memcpy((char *)&v + 8, &hi, 8);
-    return v;
+    return __builtin_bit_cast(i4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   } else {
-    const int k = step * 16 + 4 * g;
-    const char *p = lds + k * (R * 4) + (((row16 * 4) ^ col_swz<T, R>(k)) << 4) + i * 4;
+    const uint32_t p = (at ^ (c << 6)) + half * (16 * R * 4);
     i4 v;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = *(const int *)(p + e * R * 4);
+    for (int e = 0; e < 4; ++e) v[e] = *(QR_LDS const int *)(p + e * R * 4);
     return v;
   }
 }
@@ -130,14 +159,17 @@ __device__ __forceinline__ i4 fetch16(const T *p, const size_t ld, const size_t 
   return v;
 }
 
-// eight results of one row, rounded; the row's base need not be aligned
-template <class T>
+// Eight results of one row, rounded; the row's base need not be aligned.  STREAM: past the caches, for outputs that are
+// far larger and would push the operands out of the L2 (32768 x 1024 x 4096 bf16 with both products kept: 716 -> 599 us).
+typedef int u4 __attribute__((ext_vector_type(4), aligned(4)));
+template <bool STREAM, class T>
 __device__ __forceinline__ void store8(T *p, const float (&v)[8], const size_t at, const size_t len) {
   if (at + 8 <= len) {
     T t[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) t[e] = (T)v[e];
-    __builtin_memcpy(p + at, t, sizeof t);
+    if constexpr (STREAM && sizeof(T) == 2) __builtin_nontemporal_store(__builtin_bit_cast(u4, t), (u4 *)(p + at));
+    else __builtin_memcpy(p + at, t, sizeof t);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
@@ -152,7 +184,7 @@ template <class T>
 struct GemmArgs {
   const T *a[2], *b[2];  // FWD: x | Wg, Wu.  DX: dg, du | Wg, Wu.  DW: dg, du | x.  Rows at 16-byte boundaries
   size_t lda, ldb;
-  size_t rows, cols, k;  // outputs (FWD: of h; DW: of one dW) and the length of one sum (DX: of each of its two)
+  size_t rows, cols, k;  // outputs (FWD: of h; DW: of one dW), length of one sum (DX: of each of its two, whole stages)
   T *o[3];               // FWD: h, g, u.  DX: dx.  DW: dWg, dWu
   float *part;           // DW: partial sums [split][2][rows][cols] where the sum is split
   size_t ldo;
@@ -160,16 +192,33 @@ struct GemmArgs {
   unsigned row_tiles, col_tiles, splits, steps;  // steps: k tiles of one split
 };
 
-// TM x TN sums (FWD: TM x TN / 2 of each product) by WM x WN waves.  Whole tiles go from memory to LDS without
-// passing registers; the last, partial one of a sum goes through them, zero-filled.
-template <class T, Kind KIND, int TM, int TN, int WM, int WN>
-__global__ __launch_bounds__(WM *WN * 64, 2) void k_gemm(const GemmArgs<T> P) {
+// Memory to LDS and its order.  The loads are written by hand so that the compiler does not wait for them in front of
+// LDS reads of other stages; every wait they need is wait_all, and all waves' parts are there behind the barrier after it.
+// 64 lanes bring 16 bytes each, from `base` + their `off`, to consecutive LDS addresses from `to` on.
+// (The wait states are those between a vector instruction's write of a scalar register and the load that reads it.)
+__device__ __forceinline__ void dma16(const char *base, const uint32_t off, const uint32_t to) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(__builtin_amdgcn_readfirstlane(to)), "v"(off),
+               "s"(base)
+               : "m0");
+}
+// none of this wave's loads and LDS operations is under way
+__device__ __forceinline__ void wait_all() { asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory"); }
+__device__ __forceinline__ void barrier() { asm volatile("s_barrier" ::: "memory"); }
+__device__ __forceinline__ uint32_t lds_offset(const char *p) { return (uint32_t)(uintptr_t)(QR_LDS const char *)p; }
+
+// TM x TN sums (FWD: TM x TN / 2 of each product) by 2 x 2 waves.  While the matrix cores work on one stage the next is
+// on its way: the first operand's to the other half of its LDS buffer without passing registers, the second's in
+// registers, from where it is written to its single buffer behind a barrier.  (Both double-buffered, two workgroups of the
+// largest tile would not fit a compute unit, 160 KB; they do, and one's matrix instructions run under the other's waits,
+// first loads and epilogue.)  The last, partial stage of a sum is zero-filled.
+template <class T, Kind KIND, int TM, int TN>
+__global__ __launch_bounds__(256, 2) void k_gemm(const GemmArgs<T> P) {
   constexpr bool AKS = KIND == DW, BKS = KIND != FWD;
-  constexpr int NT = WM * WN * 64, KT = 128 / sizeof(T), E = 16 / sizeof(T);
+  constexpr int WM = 2, WN = 2, NT = 256, KT = 128 / sizeof(T), E = 16 / sizeof(T);
   constexpr int MI = TM / WM / 16, NI = TN / WN / 16, PA = TM * 8 / NT, PB = TN * 8 / NT;
   constexpr int COLS = KIND == FWD ? TN / 2 : TN;
-  __shared__ __align__(128) char l0[(TM + TN) * 128];
-  __shared__ __align__(128) char l1[(TM + TN) * 128];
+  constexpr uint32_t ABUF = TM * 128, LDS_BYTES = 2 * ABUF + TN * 128;
+  __shared__ __align__(1024) char lds[LDS_BYTES];
 
   // consecutive workgroups go to the eight XCDs in turn: each XCD gets a run of tiles, and a run covers bands of
   // eight tile rows column by column, so that its L2 sees the same rows and columns again
@@ -196,15 +245,26 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void k_gemm(const GemmArgs<T> P) {
     up = KIND == FWD && ((r >> 4) & 1);
     row = KIND == FWD ? c0 + (r >> 5) * 16 + (r & 15) : c0 + r;
   };
-  // where this thread's pieces come from: bytes from the operand's first element of a tile.  Rows behind the
-  // matrix are replaced by its last piece of rows: their sums are not stored
-  int64_t offa[PA], offb[PB];
+  const unsigned kt_all = (unsigned)((P.k + KT - 1) / KT);  // stages of one sum
+  unsigned first = 0, last = KIND == DX ? 2 * kt_all : kt_all;
+  if constexpr (KIND == DW) {
+    first = split * P.steps;
+    last = first + P.steps < last ? first + P.steps : last;
+  }
+  // (DX: both sums are whole stages)
+  const unsigned whole = KIND != DX && P.k % KT && last == kt_all && last > first ? last - 1 : last;
+
+  // Where this thread's pieces of a stage come from: bytes from the operand's next stage of the tile (a wave's pieces of
+  // the forward pass's second operand are all of one weight; 256 rows stay below 2^31 bytes).  Rows behind the matrix are
+  // replaced by its last piece of rows: their sums are not stored
+  uint32_t offa[PA], offb[PB];
 #pragma unroll
   for (int j = 0; j < PA; ++j) {
     int r, k;
     piece_of<T, TM, AKS>(j * NT + tid, r, k);
-    const size_t most = AKS ? (P.rows - 1) / E * E : P.rows - 1, row = r0 + r < most ? r0 + r : most;
-    offa[j] = (int64_t)((AKS ? k * P.lda + row : row * P.lda + k) * sizeof(T));
+    const uint32_t most = (uint32_t)((AKS ? (P.rows - 1) / E * E : P.rows - 1) - r0 < TM - 1 ? (AKS ? (P.rows - 1) / E * E : P.rows - 1) - r0 : TM - 1);
+    const uint32_t row = (uint32_t)r < most ? r : most;
+    offa[j] = (AKS ? k * (uint32_t)P.lda + row : row * (uint32_t)P.lda + k) * sizeof(T);
   }
 #pragma unroll
   for (int j = 0; j < PB; ++j) {
@@ -214,52 +274,55 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void k_gemm(const GemmArgs<T> P) {
     piece_of<T, TN, BKS>(j * NT + tid, r, k);
     b_row(r, row, up);
     const size_t most = BKS ? (P.cols - 1) / E * E : P.cols - 1;
-    row = row < most ? row : most;
-    offb[j] = (int64_t)((BKS ? k * P.ldb + row : row * P.ldb + k) * sizeof(T)) +
-              (up ? (const char *)P.b[1] - (const char *)P.b[0] : 0);
+    const uint32_t rel = (uint32_t)((row < most ? row : most) - c0);
+    offb[j] = (BKS ? k * (uint32_t)P.ldb + rel : rel * (uint32_t)P.ldb + k) * sizeof(T);
   }
-
-  const unsigned kt_all = (unsigned)((P.k + KT - 1) / KT);  // tiles of one sum
-  unsigned first = 0, last = KIND == DX ? 2 * kt_all : kt_all;
-  if constexpr (KIND == DW) {
-    first = split * P.steps;
-    last = first + P.steps < last ? first + P.steps : last;
-  }
-  const unsigned odd = P.k % KT ? kt_all - 1 : kt_all;  // the partial tile of a sum
-
-  auto load = [&](unsigned t, char *to) {
-    const bool second = KIND == DX && t >= kt_all;
-    const unsigned kt = second ? t - kt_all : t;
-    if (kt != odd) {
-      const char *pa = (const char *)(second ? P.a[1] : a0) + (AKS ? (size_t)kt * KT * P.lda : (size_t)kt * KT) * sizeof(T);
-      const char *pb = (const char *)(second ? P.b[1] : P.b[0]) + (BKS ? (size_t)kt * KT * P.ldb : (size_t)kt * KT) * sizeof(T);
-#pragma unroll
-      for (int j = 0; j < PA; ++j)
-        __builtin_amdgcn_global_load_lds((const QR_GLB void *)(pa + offa[j]), (QR_LDS void *)(to + (j * NT + wave * 64) * 16), 16, 0, 0);
-#pragma unroll
-      for (int j = 0; j < PB; ++j)
-        __builtin_amdgcn_global_load_lds((const QR_GLB void *)(pb + offb[j]), (QR_LDS void *)(to + (TM * 8 + j * NT + wave * 64) * 16),
-                                         16, 0, 0);
-    } else {
-      const size_t kb = (size_t)kt * KT;
+  const char *sa = (const char *)(a0 + (AKS ? (size_t)first * KT * P.lda + r0 : r0 * P.lda + (size_t)first * KT));
+  const char *sb = (const char *)(P.b[KIND == FWD ? wave >> 1 : 0] + (BKS ? (size_t)first * KT * P.ldb + c0 : c0 * P.ldb + (size_t)first * KT));
+  // stages are loaded in order
+  auto next_a = [&](const unsigned t) {
+    sa += (AKS ? KT * P.lda : (size_t)KT) * sizeof(T);
+    if (KIND == DX && t + 1 == kt_all) sa = (const char *)(P.a[1] + r0 * P.lda);
+  };
+  auto next_b = [&](const unsigned t) {
+    sb += (BKS ? KT * P.ldb : (size_t)KT) * sizeof(T);
+    if (KIND == DX && t + 1 == kt_all) sb = (const char *)(P.b[1] + c0);
+  };
+  auto load_a = [&](const int d, const uint32_t to) { dma16(sa, offa[d], to + (d * NT + wave * 64) * 16); };
+  // the partial stage's
+  auto fill_a = [&](const unsigned t, char *to) {
 #pragma unroll 1
-      for (int q = tid; q < TM * 8; q += NT) {
-        int r, k;
-        piece_of<T, TM, AKS>(q, r, k);
-        const T *p = second ? P.a[1] : a0;
-        *(i4 *)(to + q * 16) = AKS ? fetch16(p, P.lda, kb + k, P.k, r0 + r, P.rows) : fetch16(p, P.lda, r0 + r, P.rows, kb + k, P.k);
+    for (int q = tid; q < TM * 8; q += NT) {
+      int r, k;
+      piece_of<T, TM, AKS>(q, r, k);
+      const size_t kk = (size_t)t * KT + k;
+      *(i4 *)(to + q * 16) = AKS ? fetch16(a0, P.lda, kk, P.k, r0 + r, P.rows) : fetch16(a0, P.lda, r0 + r, P.rows, kk, P.k);
+    }
+  };
+  i4 vb[PB];
+  auto load_b = [&](const unsigned t) {
+    if (KIND == DX || t < whole) {
+#pragma unroll
+      for (int d = 0; d < PB; ++d) {
+        vb[d] = *(const QR_GLB i4 *)((const QR_GLB char *)sb + offb[d]);
       }
-#pragma unroll 1
-      for (int q = tid; q < TN * 8; q += NT) {
+      next_b(t);
+    } else {
+#pragma unroll
+      for (int d = 0; d < PB; ++d) {
         int r, k;
         size_t row;
         bool up;
-        piece_of<T, TN, BKS>(q, r, k);
+        piece_of<T, TN, BKS>(d * NT + tid, r, k);
         b_row(r, row, up);
-        const T *p = second || up ? P.b[1] : P.b[0];
-        *(i4 *)(to + (TM * 8 + q) * 16) = BKS ? fetch16(p, P.ldb, kb + k, P.k, row, P.cols) : fetch16(p, P.ldb, row, P.cols, kb + k, P.k);
+        const size_t kk = (size_t)t * KT + k;
+        vb[d] = BKS ? fetch16(P.b[up ? 1 : 0], P.ldb, kk, P.k, row, P.cols) : fetch16(P.b[up ? 1 : 0], P.ldb, row, P.cols, kk, P.k);
       }
     }
+  };
+  auto keep_b = [&]() {
+#pragma unroll
+    for (int d = 0; d < PB; ++d) *(i4 *)(lds + 2 * ABUF + (d * NT + tid) * 16) = vb[d];
   };
 
   f4 acc[MI][NI];
@@ -267,44 +330,70 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void k_gemm(const GemmArgs<T> P) {
   for (int m = 0; m < MI; ++m)
 #pragma unroll
     for (int n = 0; n < NI; ++n) acc[m][n] = f4{0.f, 0.f, 0.f, 0.f};
-  auto compute = [&](const char *from) {
+  const uint32_t base_a = frag_base<T, TM, AKS>(lds_offset(lds), wm * MI);
+  const uint32_t base_b = frag_base<T, TN, BKS>(lds_offset(lds) + 2 * ABUF, wn * NI);
+  // a stage's 2 x MI rows of blocks: the first operand's fragments are read D ahead of their use
+  constexpr int D = MI > 3 ? 3 : MI - 1;
+  auto compute = [&](auto steady, const uint32_t ra, const uint32_t to) {
+    i4 fa[D + 1], fb[2][NI];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      i4 fa[MI], fb[NI];
+    for (int n = 0; n < NI; ++n) fb[0][n] = frag<T, TN, BKS>(base_b, n, 0);
 #pragma unroll
-      for (int n = 0; n < NI; ++n) fb[n] = frag<T, TN, BKS>(from + TM * 128, wn * NI + n, s);
+    for (int m = 0; m < D; ++m) fa[m] = frag<T, TM, AKS>(ra, m, 0);
 #pragma unroll
-      for (int m = 0; m < MI; ++m) fa[m] = frag<T, TM, AKS>(from, wm * MI + m, s);
+    for (int q = 0; q < 2 * MI; ++q) {
+      if (q + D < 2 * MI) fa[(q + D) % (D + 1)] = frag<T, TM, AKS>(ra, (q + D) % MI, (q + D) / MI);
+      if (q < MI)
 #pragma unroll
-      for (int m = 0; m < MI; ++m)
+        for (int n = q * NI / MI; n < (q + 1) * NI / MI; ++n) fb[1][n] = frag<T, TN, BKS>(base_b, n, 1);
+      if constexpr (decltype(steady)::value)
 #pragma unroll
-        for (int n = 0; n < NI; ++n) acc[m][n] = mma<T>(fb[n], fa[m], acc[m][n]);
+        for (int d = q * PA / MI / 2; d < (q + 1) * PA / MI / 2; ++d) load_a(d, to);
+#pragma unroll
+      for (int n = 0; n < NI; ++n) acc[q % MI][n] = mma<T>(fb[q / MI][n], fa[q % (D + 1)], acc[q % MI][n]);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
-
-  // tile t lies in one half of the LDS while t + 1 arrives in the other; one barrier a tile
   if (first < last) {
-    load(first, l0);
-    __syncthreads();
-    for (unsigned t = first; t < last; t += 2) {
-      if (t + 1 < last) load(t + 1, l1);
-      compute(l0);
-      __syncthreads();
+    if (KIND == DX || first < whole) {
+#pragma unroll
+      for (int d = 0; d < PA; ++d) load_a(d, lds_offset(lds));
+      next_a(first);
+    } else {
+      fill_a(first, lds);
+    }
+    load_b(first);
+    keep_b();
+    uint32_t cur = 0;
+    unsigned t = first;
+    for (; t + 1 < whole; ++t, cur ^= ABUF) {
+      wait_all();
+      barrier();  // stage t is there, and every wave is done with the first operand's stage t - 1
+      load_b(t + 1);
+      compute(std::true_type{}, base_a + cur, lds_offset(lds) + (cur ^ ABUF));
+      next_a(t + 1);
+      barrier();  // every wave is done with the second operand's stage t
+      keep_b();
+    }
+    for (; t < last; ++t, cur ^= ABUF) {
+      wait_all();
+      barrier();
       if (t + 1 < last) {
-        if (t + 2 < last) load(t + 2, l0);
-        compute(l1);
-        __syncthreads();
+        fill_a(t + 1, lds + (cur ^ ABUF));
+        load_b(t + 1);
       }
+      compute(std::false_type{}, base_a + cur, 0);
+      barrier();
+      if (t + 1 < last) keep_b();
     }
   }
 
   // Results pass through the wave's own share of the LDS, so that a lane ends with eight neighbours of a row: one
   // wide store, and one copy of the activation's code.  Pieces of four are XORed with the row against bank conflicts.
-  constexpr int WTN = NI * 16, PIECES = WTN / 4, SHARE = (TM + TN) * 256 / (WM * WN);
-  constexpr int MB = SHARE / (16 * WTN * 4) < MI ? SHARE / (16 * WTN * 4) : MI;  // blocks of 16 rows at a time
-  constexpr int HALF = WM * WN / 2;
-  static_assert(MI % MB == 0, "blocks fit the waves' shares");
-  char *const own = (wave < HALF ? l0 + wave * SHARE : l1 + (wave - HALF) * SHARE);
+  constexpr int WTN = NI * 16, PIECES = WTN / 4, SHARE = LDS_BYTES / 4 / (16 * WTN * 4) * (16 * WTN * 4);
+  constexpr int FIT = SHARE / (16 * WTN * 4), MB = FIT >= MI ? MI : FIT >= MI / 2 ? MI / 2 : MI / 4;  // blocks of 16 rows at a time
+  static_assert(MB > 0 && MB <= FIT && MI % MB == 0 && PA % MI == 0, "blocks fit the waves' shares");
+  char *const own = lds + wave * SHARE;
   const int l = tid & 63;
 #pragma unroll
   for (int m0 = 0; m0 < MI; m0 += MB) {
@@ -333,21 +422,16 @@ __global__ __launch_bounds__(WM *WN * 64, 2) void k_gemm(const GemmArgs<T> P) {
         float u[8], h[8];
         take((s >> 1) * 8 + (s & 1) * 2, v);
         take((s >> 1) * 8 + 4 + (s & 1) * 2, u);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          float a, d;
-          act_of(P.act, v[e], a, d);
-          h[e] = a * u[e];
-        }
-        store8(P.o[0] + row * P.ldo, h, col, P.cols);
+        gated8(P.act, v, u, h);
+        store8<(TM > 128)>(P.o[0] + row * P.ldo, h, col, P.cols);
         if (P.o[1]) {
-          store8(P.o[1] + row * P.cols, v, col, P.cols);
-          store8(P.o[2] + row * P.cols, u, col, P.cols);
+          store8<(TM > 128)>(P.o[1] + row * P.cols, v, col, P.cols);
+          store8<(TM > 128)>(P.o[2] + row * P.cols, u, col, P.cols);
         }
       } else {
         take(s * 2, v);
-        if (KIND == DW && P.part) store8(P.part + ((size_t)(split * 2 + z) * P.rows + row) * P.cols, v, col, P.cols);
-        else store8(P.o[KIND == DW ? z : 0] + row * P.ldo, v, col, P.cols);
+        if (KIND == DW && P.part) store8<(TM > 128)>(P.part + ((size_t)(split * 2 + z) * P.rows + row) * P.cols, v, col, P.cols);
+        else store8<(TM > 128)>(P.o[KIND == DW ? z : 0] + row * P.ldo, v, col, P.cols);
       }
     }
     __builtin_amdgcn_wave_barrier();
@@ -366,33 +450,60 @@ __global__ __launch_bounds__(256) void k_join(const float *__restrict__ part, co
   }
 }
 
-// dg, du in rows of stride ld, their padding zeroed
-template <class T>
-__global__ __launch_bounds__(256) void k_gate_grad(const size_t m, const size_t n, const int act, const T *__restrict__ dh,
-                                                   const size_t lddh, const T *__restrict__ g, const T *__restrict__ u,
-                                                   T *__restrict__ dg, T *__restrict__ du, const size_t ld) {
-  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < m * ld; i += (size_t)gridDim.x * 256) {
-    const size_t r = i / ld, c = i - r * ld;
-    float vg = 0.f, vu = 0.f;
-    if (c < n) {
-      float a, d;
-      act_of(act, (float)g[r * n + c], a, d);
-      const float v = (float)dh[r * lddh + c];
-      vg = v * (float)u[r * n + c] * d;
-      vu = v * a;
+// dg, du in rows of stride ld, their padding zeroed; eight elements a thread.  (The padding is at least as long as what
+// a row's last eight reach over.)
+template <class T, int ACT>
+__global__ __launch_bounds__(256) void k_gate_grad(const size_t m, const size_t n, const T *__restrict__ dh, const size_t lddh,
+                                                   const T *__restrict__ g, const T *__restrict__ u, T *__restrict__ dg,
+                                                   T *__restrict__ du, const size_t ld) {
+  const size_t per = ld / 8;
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < m * per; i += (size_t)gridDim.x * 256) {
+    const size_t r = i / per, c = (i - r * per) * 8;
+    T vh[8] = {}, vg[8] = {}, vu[8] = {}, og[8], ou[8];
+    if (c + 8 <= n) {
+      __builtin_memcpy(vh, dh + r * lddh + c, sizeof vh);
+      __builtin_memcpy(vg, g + r * n + c, sizeof vg);
+      __builtin_memcpy(vu, u + r * n + c, sizeof vu);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (c + e < n) vh[e] = dh[r * lddh + c + e], vg[e] = g[r * n + c + e], vu[e] = u[r * n + c + e];
     }
-    dg[i] = (T)vg;
-    du[i] = (T)vu;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      float a, d;
+      act_of(ACT, (float)vg[e], a, d);
+      const float v = (float)vh[e];
+      og[e] = (T)(v * (float)vu[e] * d);
+      ou[e] = (T)(v * a);
+    }
+    __builtin_memcpy(dg + r * ld + c, og, sizeof og);
+    __builtin_memcpy(du + r * ld + c, ou, sizeof ou);
   }
 }
+template <class T>
+void gate_grad(hipStream_t s, size_t m, size_t n, int act, const void *dh, size_t lddh, const void *g, const void *u, T *dg, T *du,
+               size_t ld) {
+  const size_t threads = m * (ld / 8);
+  const unsigned grid = (unsigned)((threads + 255) / 256 < 65536 ? (threads + 255) / 256 : 65536);
+  const auto go = [&](auto a) {
+    k_gate_grad<T, decltype(a)::value><<<grid, 256, 0, s>>>(m, n, (const T *)dh, lddh, (const T *)g, (const T *)u, dg, du, ld);
+  };
+  if (act == QR_ACT_SILU) go(std::integral_constant<int, QR_ACT_SILU>{});
+  else if (act == QR_ACT_GELU) go(std::integral_constant<int, QR_ACT_GELU>{});
+  else if (act == QR_ACT_GELU_TANH) go(std::integral_constant<int, QR_ACT_GELU_TANH>{});
+  else if (act == QR_ACT_RELU) go(std::integral_constant<int, QR_ACT_RELU>{});
+  else go(std::integral_constant<int, QR_ACT_SIGMOID>{});
+}
 
-// a matrix whose rows do not start at 16-byte boundaries, copied to one whose rows do; the padding zeroed
+// a matrix whose rows do not start at 16-byte boundaries, copied to one whose rows do; the padding, and rows
+// up to rows_to, zeroed
 template <class T>
 __global__ __launch_bounds__(256) void k_pack(const size_t rows, const size_t cols, const T *__restrict__ p, const size_t ld,
-                                              T *__restrict__ q, const size_t to) {
+                                              T *__restrict__ q, const size_t to, const size_t rows_to) {
   constexpr int E = 16 / sizeof(T);
   const size_t per = to / E;
-  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < rows * per; i += (size_t)gridDim.x * 256) {
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < rows_to * per; i += (size_t)gridDim.x * 256) {
     const size_t r = i / per, c = (i - r * per) * E;
     *(i4 *)(q + r * to + c) = fetch16(p, ld, r, rows, c, cols);
   }
@@ -403,36 +514,42 @@ unsigned tiles_of(size_t n, size_t t) { return (unsigned)((n + t - 1) / t); }
 
 size_t round256(size_t b) { return (b + 255) & ~(size_t)255; }
 size_t padded(size_t cols, size_t e) { return (cols + 16 / e - 1) / (16 / e) * (16 / e); }
+// the length of one of DX's two sums, in whole stages
+size_t stages_of(size_t n, size_t e) { return (n + 128 / e - 1) / (128 / e) * (128 / e); }
 size_t pack_bytes(size_t rows, size_t cols, size_t e) { return round256(rows * padded(cols, e) * e); }
 unsigned blocks(size_t n) { return (unsigned)((n + 255) / 256 < 65536 ? (n + 255) / 256 : 65536); }
+
+// longest row the product kernel takes: a tile's 256 rows lie within 2^31 bytes
+constexpr size_t ROW_BYTES = (size_t)1 << 22;
 
 // whether the product kernel can read a matrix where it lies: rows at 16-byte boundaries and, where the columns are
 // what it moves in pieces (the columns layout), none cut by the row's end
 bool in_place(const void *p, size_t ld, size_t cols, size_t e, bool columns) {
-  return ((uintptr_t)p & 15) == 0 && (ld * e) % 16 == 0 && (!columns || (cols * e) % 16 == 0);
+  return ((uintptr_t)p & 15) == 0 && (ld * e) % 16 == 0 && ld * e <= ROW_BYTES && (!columns || (cols * e) % 16 == 0);
 }
 
 template <class T>
-void pack(hipStream_t s, size_t rows, size_t cols, const T *&p, size_t ld, char *&ws) {
+void pack(hipStream_t s, size_t rows, size_t cols, const T *&p, size_t ld, char *&ws, size_t rows_to) {
   const size_t to = padded(cols, sizeof(T));
-  if (rows) k_pack<T><<<blocks(rows * to * sizeof(T) / 16), 256, 0, s>>>(rows, cols, p, ld, (T *)ws, to);
+  if (rows) k_pack<T><<<blocks(rows_to * to * sizeof(T) / 16), 256, 0, s>>>(rows, cols, p, ld, (T *)ws, to, rows_to);
   p = (const T *)ws;
-  ws += pack_bytes(rows, cols, sizeof(T));
+  ws += pack_bytes(rows_to, cols, sizeof(T));
 }
 
-template <class T, Kind KIND, int TM, int TN, int WM, int WN>
+template <class T, Kind KIND, int TM, int TN>
 void launch_gemm(hipStream_t s, GemmArgs<T> P) {
   P.row_tiles = tiles_of(P.rows, TM);
   P.col_tiles = tiles_of(P.cols, KIND == FWD ? TN / 2 : TN);
   const unsigned tiles = P.row_tiles * P.col_tiles * (KIND == DW ? 2 * P.splits : 1);
-  k_gemm<T, KIND, TM, TN, WM, WN><<<(tiles + 7) / 8 * 8, WM * WN * 64, 0, s>>>(P);
+  k_gemm<T, KIND, TM, TN><<<(tiles + 7) / 8 * 8, 256, 0, s>>>(P);
 }
 
 constexpr unsigned CUS = 256;
 
-// Outputs a workgroup takes: the largest square that still gives every compute unit a tile.
+// Outputs a workgroup takes: the largest of 256 x 128 (16-bit types), 128 x 128 and 64 x 64 that still gives every
+// compute unit a tile.
 int tile_of(size_t e, size_t rows, size_t cols, size_t times) {
-  if (e == 2 && (size_t)tiles_of(rows, 256) * tiles_of(cols, 256) * times >= CUS) return 256;
+  if (e == 2 && (size_t)tiles_of(rows, 256) * tiles_of(cols, 128) * times >= CUS) return 256;
   if ((size_t)tiles_of(rows, 128) * tiles_of(cols, 128) * times >= CUS) return 128;
   return 64;
 }
@@ -440,9 +557,9 @@ int tile_of(size_t e, size_t rows, size_t cols, size_t times) {
 template <class T, Kind KIND>
 void gemm(hipStream_t s, int tile, const GemmArgs<T> &P) {
   if constexpr (sizeof(T) == 2)
-    if (tile == 256) return launch_gemm<T, KIND, 256, 256, 2, 4>(s, P);
-  if (tile == 128) return launch_gemm<T, KIND, 128, 128, 2, 2>(s, P);
-  launch_gemm<T, KIND, 64, 64, 2, 2>(s, P);
+    if (tile == 256) return launch_gemm<T, KIND, 256, 128>(s, P);
+  if (tile == 128) return launch_gemm<T, KIND, 128, 128>(s, P);
+  launch_gemm<T, KIND, 64, 64>(s, P);
 }
 
 // The weights' gradients sum over all m rows: with few outputs the sum is split so that the launch fills the
@@ -451,7 +568,7 @@ void plan_dw(size_t e, size_t m, size_t k, size_t n, int &tile, unsigned &splits
   const size_t kt = 128 / e, tiles = (m + kt - 1) / kt;
   const size_t most = m / 512 ? m / 512 : 1;
   tile = tile_of(e, n, k, 2 * most);
-  const size_t out = 2 * (size_t)tiles_of(n, tile) * tiles_of(k, tile);
+  const size_t out = 2 * (size_t)tiles_of(n, tile) * tiles_of(k, tile < 128 ? tile : 128);
   size_t want = (2 * CUS + out - 1) / out;
   want = want < most ? want : most;
   if (!want) want = 1;
@@ -507,8 +624,8 @@ extern "C" int qr_gated_ffn_async(int device, void *stream, int type, int act, s
     P.a[0] = (const T *)x, P.b[0] = (const T *)w_gate, P.b[1] = (const T *)w_up;
     P.lda = ldx, P.ldb = ldw, P.rows = m, P.cols = n, P.k = k;
     P.o[0] = (T *)h, P.o[1] = (T *)gate, P.o[2] = (T *)up, P.ldo = ldh, P.act = act;
-    if (px) pack(s, m, k, P.a[0], ldx, ws), P.lda = padded(k, e);
-    if (pw) pack(s, n, k, P.b[0], ldw, ws), pack(s, n, k, P.b[1], ldw, ws), P.ldb = padded(k, e);
+    if (px) pack(s, m, k, P.a[0], ldx, ws, m), P.lda = padded(k, e);
+    if (pw) pack(s, n, k, P.b[0], ldw, ws, n), pack(s, n, k, P.b[1], ldw, ws, n), P.ldb = padded(k, e);
     gemm<T, FWD>(s, tile_of(e, m, 2 * n, 1), P);
   });
   return qr_dense_launched("gated ffn");
@@ -522,8 +639,8 @@ extern "C" int qr_gated_ffn_backward_workspace(int type, size_t m, size_t k, siz
   unsigned splits, steps;
   plan_dw(e, m, k, n, tile, splits, steps);
   // dg, du, the partial sums, copies of x and the weights where their rows are not aligned
-  *bytes = m ? 2 * pack_bytes(m, n, e) + round256(splits > 1 ? (size_t)splits * 2 * n * k * 4 : 0) + pack_bytes(m, k, e) +
-                   2 * pack_bytes(n, k, e) + 256
+  *bytes = m ? 2 * pack_bytes(m, stages_of(n, e), e) + round256(splits > 1 ? (size_t)splits * 2 * n * k * 4 : 0) + pack_bytes(m, k, e) +
+                   2 * pack_bytes(stages_of(n, e), k, e) + 256
              : 0;
   return QR_OK;
 }
@@ -557,17 +674,16 @@ extern "C" int qr_gated_ffn_backward_async(int device, void *stream, int type, i
   qr_dense_dispatch(type, [&](auto t) {
     using T = decltype(t);
     char *ws = (char *)(((uintptr_t)workspace + 255) & ~(uintptr_t)255);
-    const size_t ld = padded(n, e);
-    T *const dg = (T *)ws, *const du = (T *)(ws + pack_bytes(m, n, e));
-    ws += 2 * pack_bytes(m, n, e);
-    if (m)
-      k_gate_grad<T><<<blocks(m * ld), 256, 0, s>>>(m, n, act, (const T *)dh, lddh, (const T *)gate, (const T *)up, dg, du, ld);
+    const size_t ld = stages_of(n, e);
+    T *const dg = (T *)ws, *const du = (T *)(ws + pack_bytes(m, ld, e));
+    ws += 2 * pack_bytes(m, ld, e);
+    if (m) gate_grad<T>(s, m, n, act, dh, lddh, gate, up, dg, du, ld);
     if (dx && m) {
       GemmArgs<T> P{};
       P.a[0] = dg, P.a[1] = du, P.b[0] = (const T *)w_gate, P.b[1] = (const T *)w_up;
-      P.lda = ld, P.ldb = ldw, P.rows = m, P.cols = k, P.k = n, P.o[0] = (T *)dx, P.ldo = lddx;
-      if (!in_place(w_gate, ldw, k, e, true) || !in_place(w_up, ldw, k, e, true))
-        pack(s, n, k, P.b[0], ldw, ws), pack(s, n, k, P.b[1], ldw, ws), P.ldb = padded(k, e);
+      P.lda = ld, P.ldb = ldw, P.rows = m, P.cols = k, P.k = ld, P.o[0] = (T *)dx, P.ldo = lddx;
+      if (ld != n || !in_place(w_gate, ldw, k, e, true) || !in_place(w_up, ldw, k, e, true))
+        pack(s, n, k, P.b[0], ldw, ws, ld), pack(s, n, k, P.b[1], ldw, ws, ld), P.ldb = padded(k, e);
       gemm<T, DX>(s, tile_of(e, m, k, 1), P);
     }
     if (dw_gate) {
@@ -576,7 +692,7 @@ extern "C" int qr_gated_ffn_backward_async(int device, void *stream, int type, i
       plan_dw(e, m, k, n, tile, P.splits, P.steps);
       P.a[0] = dg, P.a[1] = du, P.b[0] = (const T *)x, P.lda = ld, P.ldb = ldx, P.rows = n, P.cols = k, P.k = m;
       P.o[0] = (T *)dw_gate, P.o[1] = (T *)dw_up, P.ldo = k;
-      if (m && !in_place(x, ldx, k, e, true)) pack(s, m, k, P.b[0], ldx, ws), P.ldb = padded(k, e);
+      if (m && !in_place(x, ldx, k, e, true)) pack(s, m, k, P.b[0], ldx, ws, m), P.ldb = padded(k, e);
       if (P.splits > 1) P.part = (float *)ws;
       gemm<T, DW>(s, tile, P);
       if (P.splits > 1)
