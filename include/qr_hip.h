@@ -503,6 +503,7 @@ int qr_dropout_async(int device, void *hip_stream, int type, size_t rows, size_t
                      const void *residual, size_t ldr, void *y, size_t ldy, double p, uint64_t seed,
                      uint64_t offset, const uint64_t *counter);
 
+/* (Rows of x, the weights and dh of up to 4 MB: QR_ERR_UNSUPPORTED beyond.)               */
 /* h [m][n] = act(x w_gate^T) * (x w_up^T); x [m][k], weights [n][k] of stride ldw.        */
 /* gate / up: NULL (serving), or [m][n] contiguous: the two products, rounded to `type`,    */
 /* for the backward pass.  Outputs must not overlap each other or an input.  The workspace   */

@@ -87,7 +87,7 @@ __device__ __forceinline__ f4 mma(const i4 a, const i4 b, f4 c) {
 // read, which lie in 8 (16-bit) or 4 (f32) such lines, touch every bank once.
 template <class T, int R>
 __device__ __forceinline__ int col_swz(const int k) {
-  if constexpr (sizeof(T) == 4) return ((k >> 2) & 3) << 2;                    // segments of 16 floats
+  if constexpr (sizeof(T) == 4) return ((k >> 2) & (R >= 64 ? 3 : 1)) << 2;    // segments of 16 floats
   else if constexpr (R >= 128) return ((k & 3) | (((k >> 3) & 1) << 2)) << 1;  // segments of 16 elements = 32 bytes
   else return (((k >> 1) & 1) | (((k >> 3) & 1) << 1)) << 1;                   // two lines of 128 bytes share the banks
 }
@@ -438,6 +438,84 @@ __global__ __launch_bounds__(256, 2) void k_gemm(const GemmArgs<T> P) {
   }
 }
 
+// The forward pass of few rows: bound by reading the weights once and by latency, so no tile is staged.  A workgroup
+// makes 16 columns of h for 16 MB rows; its eight waves share the sum over k in steps of 128 bytes, read straight into
+// fragments (any alignment: a lane takes 32 consecutive bytes of a row, in x and in the weights alike), and are joined in
+// LDS in a fixed order.
+template <class T, int MB>
+__global__ __launch_bounds__(512) void k_few(const GemmArgs<T> P) {
+  constexpr int W = 8, KT = 128 / sizeof(T), E = 16 / sizeof(T);
+  __shared__ f4 part[W][MB][2][64];
+  const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid >> 6), l = tid & 63, g = l >> 4, i = l & 15;
+  const size_t c0 = (size_t)blockIdx.x * 16, r0 = (size_t)blockIdx.y * (16 * MB);
+  const size_t col = c0 + i < P.cols ? c0 + i : P.cols - 1;
+  size_t row[MB];
+#pragma unroll
+  for (int b = 0; b < MB; ++b) row[b] = r0 + 16 * b + i < P.rows ? r0 + 16 * b + i : P.rows - 1;
+  f4 acc[MB][2];
+#pragma unroll
+  for (int b = 0; b < MB; ++b) acc[b][0] = acc[b][1] = f4{0.f, 0.f, 0.f, 0.f};
+  auto work = [&](const i4(&vw)[2][2], const i4(&vx)[MB][2]) {
+#pragma unroll
+    for (int b = 0; b < MB; ++b)
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) acc[b][p] = mma<T>(vw[p][h], vx[b][h], acc[b][p]);
+  };
+  size_t k = (size_t)w * KT;
+#pragma unroll 2
+  for (; k + KT <= P.k; k += W * KT) {
+    i4 vw[2][2], vx[MB][2];
+    const size_t at = k + 2 * g * E;
+#pragma unroll
+    for (int p = 0; p < 2; ++p) __builtin_memcpy(vw[p], P.b[p] + col * P.ldb + at, 32);
+#pragma unroll
+    for (int b = 0; b < MB; ++b) __builtin_memcpy(vx[b], P.a[0] + row[b] * P.lda + at, 32);
+    work(vw, vx);
+  }
+  if (k < P.k) {
+    i4 vw[2][2], vx[MB][2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const size_t at = k + (2 * g + h) * E;
+#pragma unroll
+      for (int p = 0; p < 2; ++p) vw[p][h] = fetch16(P.b[p], P.ldb, col, P.cols, at, P.k);
+#pragma unroll
+      for (int b = 0; b < MB; ++b) vx[b][h] = fetch16(P.a[0], P.lda, row[b], P.rows, at, P.k);
+    }
+    work(vw, vx);
+  }
+#pragma unroll
+  for (int b = 0; b < MB; ++b)
+#pragma unroll
+    for (int p = 0; p < 2; ++p) part[w][b][p][l] = acc[b][p];
+  __syncthreads();
+  if (tid >= MB * 64) return;
+  f4 sum[2];
+#pragma unroll
+  for (int p = 0; p < 2; ++p) {
+    sum[p] = part[0][w][p][l];
+#pragma unroll
+    for (int q = 1; q < W; ++q) sum[p] += part[q][w][p][l];
+  }
+  const size_t r = r0 + 16 * w + i, c = c0 + 4 * g;
+  if (r >= P.rows || c >= P.cols) return;
+  float a[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    float d;
+    act_of(P.act, sum[0][e], a[e], d);
+    a[e] *= sum[1][e];
+  }
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (c + e < P.cols) {
+      P.o[0][r * P.ldo + c + e] = (T)a[e];
+      if (P.o[1]) P.o[1][r * P.cols + c + e] = (T)sum[0][e], P.o[2][r * P.cols + c + e] = (T)sum[1][e];
+    }
+}
+
 // the partial sums of the weights' gradients, joined in the order of the splits
 template <class T>
 __global__ __launch_bounds__(256) void k_join(const float *__restrict__ part, const size_t n, const unsigned splits, T *__restrict__ o0,
@@ -544,37 +622,65 @@ void launch_gemm(hipStream_t s, GemmArgs<T> P) {
   k_gemm<T, KIND, TM, TN><<<(tiles + 7) / 8 * 8, 256, 0, s>>>(P);
 }
 
+
 constexpr unsigned CUS = 256;
 
-// Outputs a workgroup takes: the largest of 256 x 128 (16-bit types), 128 x 128 and 64 x 64 that still gives every
-// compute unit a tile.
-int tile_of(size_t e, size_t rows, size_t cols, size_t times) {
-  if (e == 2 && (size_t)tiles_of(rows, 256) * tiles_of(cols, 128) * times >= CUS) return 256;
-  if ((size_t)tiles_of(rows, 128) * tiles_of(cols, 128) * times >= CUS) return 128;
-  return 64;
+// Whether the forward pass takes the few-rows kernel: where tiles of 64 x 64 sums would leave half the compute units
+// without one, and up to one such tile of rows.  Few rows / tiles in us, back to back in a graph: k 1024, n 4096 bf16 1 row
+// 5.8 / 14.9, 64 9.8 / 14.6, 200 24 / 17; k 136, n 512 f32 100 rows 3.5 / 6.5, 512 5.8 / 6.7, 1000 8.3 / 7.0.
+bool few(size_t m, size_t n) { return m <= 64 || (size_t)tiles_of(m, 64) * tiles_of(2 * n, 64) <= CUS / 2; }
+
+template <class T>
+void launch_few(hipStream_t s, const GemmArgs<T> &P) {
+  const unsigned cols = tiles_of(P.cols, 16);
+  // the most rows a workgroup that still leave every compute unit one
+  if (P.rows > 32 && (size_t)cols * tiles_of(P.rows, 64) >= CUS) k_few<T, 4><<<dim3(cols, tiles_of(P.rows, 64)), 512, 0, s>>>(P);
+  else if (P.rows > 16 && (size_t)cols * tiles_of(P.rows, 32) >= CUS) k_few<T, 2><<<dim3(cols, tiles_of(P.rows, 32)), 512, 0, s>>>(P);
+  else k_few<T, 1><<<dim3(cols, tiles_of(P.rows, 16)), 512, 0, s>>>(P);
+}
+
+struct Tile {
+  int rows, cols;
+};
+
+// Sums a workgroup takes: 256 x 128 (16-bit types) or 128 x 128 where that gives every compute unit a tile, else 64 x 64.
+// Gradients may be narrow (features): a width of 64 or, in f32, whose matrix instructions hide the reads of narrow
+// tiles, 32 is taken where it pads the columns less.  (100000 x 136 x 512 f32, width 128 / 32: dx 436 / 273, dw 384 / 287 us.)
+Tile tile_of(size_t e, size_t rows, size_t cols, size_t times, bool narrow) {
+  int w = 128;
+  if (narrow)
+    for (int v = 64; v >= (e == 4 ? 32 : 64); v /= 2)
+      if ((size_t)tiles_of(cols, v) * v < (size_t)tiles_of(cols, w) * w) w = v;
+  if (e == 2 && w == 128 && (size_t)tiles_of(rows, 256) * tiles_of(cols, 128) * times >= CUS) return {256, 128};
+  if ((size_t)tiles_of(rows, 128) * tiles_of(cols, w) * times >= CUS) return {128, w};
+  return {64, 64};
 }
 
 template <class T, Kind KIND>
-void gemm(hipStream_t s, int tile, const GemmArgs<T> &P) {
+void gemm(hipStream_t s, const Tile t, const GemmArgs<T> &P) {
   if constexpr (sizeof(T) == 2)
-    if (tile == 256) return launch_gemm<T, KIND, 256, 128>(s, P);
-  if (tile == 128) return launch_gemm<T, KIND, 128, 128>(s, P);
+    if (t.rows == 256) return launch_gemm<T, KIND, 256, 128>(s, P);
+  if (t.rows == 128 && t.cols == 128) return launch_gemm<T, KIND, 128, 128>(s, P);
+  if constexpr (KIND != FWD) {
+    if (t.rows == 128 && t.cols == 64) return launch_gemm<T, KIND, 128, 64>(s, P);
+    if constexpr (sizeof(T) == 4)
+      if (t.rows == 128) return launch_gemm<T, KIND, 128, 32>(s, P);
+  }
   launch_gemm<T, KIND, 64, 64>(s, P);
 }
 
 // The weights' gradients sum over all m rows: with few outputs the sum is split so that the launch fills the
-// compute units, in shares of at least 512 rows.
-void plan_dw(size_t e, size_t m, size_t k, size_t n, int &tile, unsigned &splits, unsigned &steps) {
-  const size_t kt = 128 / e, tiles = (m + kt - 1) / kt;
+// compute units twice, in shares of at least 512 rows.
+void plan_dw(size_t e, size_t m, size_t k, size_t n, Tile &tile, unsigned &splits, unsigned &steps) {
+  const size_t kt = 128 / e, stages = (m + kt - 1) / kt;
   const size_t most = m / 512 ? m / 512 : 1;
-  tile = tile_of(e, n, k, 2 * most);
-  const size_t out = 2 * (size_t)tiles_of(n, tile) * tiles_of(k, tile < 128 ? tile : 128);
-  size_t want = (2 * CUS + out - 1) / out;
-  want = want < most ? want : most;
-  if (!want) want = 1;
-  steps = (unsigned)((tiles + want - 1) / want);
+  tile = tile_of(e, n, k, 2 * most, true);
+  const size_t out = 2 * (size_t)tiles_of(n, tile.rows) * tiles_of(k, tile.cols);
+  size_t want = 2 * CUS / out;  // (one workgroup more than that makes a compute unit work half as long again)
+  want = want < 1 ? 1 : want < most ? want : most;
+  steps = (unsigned)((stages + want - 1) / want);
   if (!steps) steps = 1;
-  splits = (unsigned)((tiles + steps - 1) / steps);
+  splits = (unsigned)((stages + steps - 1) / steps);
   if (!splits) splits = 1;
 }
 
@@ -600,12 +706,13 @@ extern "C" int qr_gated_ffn_async(int device, void *stream, int type, int act, s
   if (!m) return QR_OK;
   QR_DENSE_ARG(x && w_gate && w_up && h, "gated ffn: x, a weight or h is NULL");
   const size_t e = qr_dense_size(type);
-  const bool px = !in_place(x, ldx, k, e, false), pw = !in_place(w_gate, ldw, k, e, false) || !in_place(w_up, ldw, k, e, false);
+  const bool px = !few(m, n) && !in_place(x, ldx, k, e, false), pw = !few(m, n) && (!in_place(w_gate, ldw, k, e, false) || !in_place(w_up, ldw, k, e, false));
   size_t need = 0;
   if (px || pw)
     if (int rc = qr_gated_ffn_workspace(type, m, k, n, &need)) return rc;
   QR_DENSE_ARG(!need || (workspace && workspace_bytes >= need),
                "gated ffn: rows that do not start at 16-byte boundaries need the workspace");
+  if (!few(m, n) && k * e > ROW_BYTES) return qr_dense_fail(QR_ERR_UNSUPPORTED, "gated ffn: rows longer than 4 MB");
   const void *out[4] = {h, gate, up, workspace};
   const size_t bytes[4] = {qr_dense_span(m, n, ldh, e), m * n * e, m * n * e, need};
   for (int i = 0; i < 4; ++i) {
@@ -626,7 +733,8 @@ extern "C" int qr_gated_ffn_async(int device, void *stream, int type, int act, s
     P.o[0] = (T *)h, P.o[1] = (T *)gate, P.o[2] = (T *)up, P.ldo = ldh, P.act = act;
     if (px) pack(s, m, k, P.a[0], ldx, ws, m), P.lda = padded(k, e);
     if (pw) pack(s, n, k, P.b[0], ldw, ws, n), pack(s, n, k, P.b[1], ldw, ws, n), P.ldb = padded(k, e);
-    gemm<T, FWD>(s, tile_of(e, m, 2 * n, 1), P);
+    if (few(m, n)) launch_few(s, P);
+    else gemm<T, FWD>(s, tile_of(e, m, 2 * n, 1, false), P);
   });
   return qr_dense_launched("gated ffn");
 }
@@ -635,7 +743,7 @@ extern "C" int qr_gated_ffn_backward_workspace(int type, size_t m, size_t k, siz
   QR_DENSE_ARG(bytes && qr_dense_type_ok(type) && k > 0 && n > 0 && qr_dense_fits(m, n, n) && qr_dense_fits(m, k, k) && qr_dense_fits(n, k, k),
                "gated ffn backward: bad size");
   const size_t e = qr_dense_size(type);
-  int tile;
+  Tile tile;
   unsigned splits, steps;
   plan_dw(e, m, k, n, tile, splits, steps);
   // dg, du, the partial sums, copies of x and the weights where their rows are not aligned
@@ -661,6 +769,8 @@ extern "C" int qr_gated_ffn_backward_async(int device, void *stream, int type, i
   if (int rc = qr_gated_ffn_backward_workspace(type, m, k, n, &need)) return rc;
   QR_DENSE_ARG(!need || (workspace && workspace_bytes >= need), "gated ffn backward: the workspace is too small");
   const size_t e = qr_dense_size(type);
+  if (k * e > ROW_BYTES || stages_of(n, e) * e > ROW_BYTES)
+    return qr_dense_fail(QR_ERR_UNSUPPORTED, "gated ffn backward: rows longer than 4 MB");
   const void *out[4] = {dx, dw_gate, dw_up, workspace}, *in[6] = {dh, x, w_gate, w_up, gate, up};
   const size_t ob[4] = {qr_dense_span(m, k, lddx, e), n * k * e, n * k * e, need};
   const size_t ib[6] = {qr_dense_span(m, n, lddh, e), qr_dense_span(m, k, ldx, e), qr_dense_span(n, k, ldw, e),
@@ -684,11 +794,11 @@ extern "C" int qr_gated_ffn_backward_async(int device, void *stream, int type, i
       P.lda = ld, P.ldb = ldw, P.rows = m, P.cols = k, P.k = ld, P.o[0] = (T *)dx, P.ldo = lddx;
       if (ld != n || !in_place(w_gate, ldw, k, e, true) || !in_place(w_up, ldw, k, e, true))
         pack(s, n, k, P.b[0], ldw, ws, ld), pack(s, n, k, P.b[1], ldw, ws, ld), P.ldb = padded(k, e);
-      gemm<T, DX>(s, tile_of(e, m, k, 1), P);
+      gemm<T, DX>(s, tile_of(e, m, k, 1, true), P);
     }
     if (dw_gate) {
       GemmArgs<T> P{};
-      int tile;
+      Tile tile;
       plan_dw(e, m, k, n, tile, P.splits, P.steps);
       P.a[0] = dg, P.a[1] = du, P.b[0] = (const T *)x, P.lda = ld, P.ldb = ldx, P.rows = n, P.cols = k, P.k = m;
       P.o[0] = (T *)dw_gate, P.o[1] = (T *)dw_up, P.ldo = k;

@@ -23,30 +23,41 @@ __device__ __forceinline__ float lane_of(const float v, const int l) {
   return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), l));
 }
 // sums over groups of G lanes, in a fixed order: every lane gets its group's (G > 64: the workgroup's, through `lds`)
-template <int G, int K>
-__device__ __forceinline__ void group_sum(float (&v)[K], float *lds) {
-#pragma unroll
-  for (int i = 0; i < K; ++i) {
-    v[i] += dpp<0xB1>(v[i]);   // quad_perm [1,0,3,2]
-    v[i] += dpp<0x4E>(v[i]);   // quad_perm [2,3,0,1]
-    v[i] += dpp<0x141>(v[i]);  // row_half_mirror
-    v[i] += dpp<0x140>(v[i]);  // row_mirror
-    if constexpr (G >= 64) v[i] = (lane_of(v[i], 0) + lane_of(v[i], 16)) + (lane_of(v[i], 32) + lane_of(v[i], 48));
-  }
+template <int G>
+__device__ __forceinline__ float wave_part(float v) {
+  v += dpp<0xB1>(v);   // quad_perm [1,0,3,2]
+  v += dpp<0x4E>(v);   // quad_perm [2,3,0,1]
+  v += dpp<0x141>(v);  // row_half_mirror
+  v += dpp<0x140>(v);  // row_mirror
+  if constexpr (G >= 64) v = (lane_of(v, 0) + lane_of(v, 16)) + (lane_of(v, 32) + lane_of(v, 48));
+  return v;
+}
+template <int G>
+__device__ __forceinline__ void group_sum(float &a, float &b, float *lds) {
+  a = wave_part<G>(a);
+  b = wave_part<G>(b);
   if constexpr (G > 64) {
     constexpr int W = G / 64;
     __syncthreads();
-    if ((threadIdx.x & 63) == 0)
-#pragma unroll
-      for (int i = 0; i < K; ++i) lds[i * W + (threadIdx.x >> 6)] = v[i];
+    if ((threadIdx.x & 63) == 0) {
+      lds[threadIdx.x >> 6] = a;
+      lds[W + (threadIdx.x >> 6)] = b;
+    }
     __syncthreads();
+    a = lds[0], b = lds[W];
 #pragma unroll
-    for (int i = 0; i < K; ++i) {
-      v[i] = 0.f;
-#pragma unroll
-      for (int j = 0; j < W; ++j) v[i] += lds[i * W + j];
+    for (int j = 1; j < W; ++j) {
+      a += lds[j];
+      b += lds[W + j];
     }
   }
+}
+template <int G>
+__device__ __forceinline__ float group_sum(float a, float *lds) {
+  float none = 0.f;
+  if constexpr (G > 64) group_sum<G>(a, none, lds);
+  else a = wave_part<G>(a);
+  return a;
 }
 
 // The pieces of a row that lane l of G holds: l, l + G, ...; the last piece of a row is moved back to end with the
@@ -91,7 +102,7 @@ __global__ __launch_bounds__(256) void k_norm(const size_t rows, const int cols,
                                               const P *__restrict__ b, const float eps, T *y, const size_t ldy,
                                               float *__restrict__ mean, float *__restrict__ rstd) {
   constexpr int V = Pieces<T, G>::V;
-  __shared__ float lds[4];
+  __shared__ float lds[8];
   const Pieces<T, G> S(cols);
   const int l = threadIdx.x % G;
   const size_t mine = (size_t)blockIdx.x * (256 / G) + threadIdx.x / G, r = mine < rows ? mine : rows - 1;
@@ -99,40 +110,38 @@ __global__ __launch_bounds__(256) void k_norm(const size_t rows, const int cols,
 #pragma unroll
   for (int i = 0; i < N; ++i)
     if (S.inner(i) || S.any(i, l)) raw[i] = load(x + r * ldx + S.at(i, l));
-  float s[1] = {0.f};
+  float s = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     if (S.inner(i)) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) s[0] += (float)raw[i].v[e];
+      for (int e = 0; e < V; ++e) s += (float)raw[i].v[e];
     } else if (S.any(i, l)) {
       const int dup = S.dup(i, l);
 #pragma unroll
-      for (int e = 0; e < V; ++e) s[0] += e >= dup ? (float)raw[i].v[e] : 0.f;
+      for (int e = 0; e < V; ++e) s += e >= dup ? (float)raw[i].v[e] : 0.f;
     }
   }
-  group_sum<G>(s, lds);
-  const float mu = s[0] / (float)cols;
-  s[0] = 0.f;
+  const float mu = group_sum<G>(s, lds) / (float)cols;
+  s = 0.f;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     if (S.inner(i)) {
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         const float d = (float)raw[i].v[e] - mu;
-        s[0] = fmaf(d, d, s[0]);
+        s = fmaf(d, d, s);
       }
     } else if (S.any(i, l)) {
       const int dup = S.dup(i, l);
 #pragma unroll
       for (int e = 0; e < V; ++e) {
         const float d = e >= dup ? (float)raw[i].v[e] - mu : 0.f;
-        s[0] = fmaf(d, d, s[0]);
+        s = fmaf(d, d, s);
       }
     }
   }
-  group_sum<G>(s, lds);
-  const float rs = 1.f / sqrtf(s[0] / (float)cols + eps);
+  const float rs = 1.f / sqrtf(group_sum<G>(s, lds) / (float)cols + eps);
   if (mine >= rows) return;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
@@ -171,29 +180,25 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void k_norm_grad(const size_t ro
 
   // a row's pieces are on their way while the row before is worked on; a group without a row works on zeros
   Raw<T> nx[N], nd[N];
-  float nm = 0.f, nr = 0.f;
-  auto fetch = [&](const size_t first) {
+  auto fetch = [&](const size_t first) {  // -> the row's mean and rstd
     const size_t r = first + grp;
-    if (r < rows) {
+    const bool live = r < rows;
 #pragma unroll
-      for (int i = 0; i < N; ++i)
-        if (S.inner(i) || S.any(i, l)) {
-          nx[i] = load(x + r * ldx + S.at(i, l));
-          nd[i] = load(dy + r * lddy + S.at(i, l));
-        }
-      nm = mean[r];
-      nr = rstd[r];
-    } else {
-#pragma unroll
-      for (int i = 0; i < N; ++i) nx[i] = nd[i] = Raw<T>{};
-      nm = nr = 0.f;
+    for (int i = 0; i < N; ++i) {
+      nx[i] = nd[i] = Raw<T>{};
+      if (live && (S.inner(i) || S.any(i, l))) {
+        nx[i] = load(x + r * ldx + S.at(i, l));
+        nd[i] = load(dy + r * lddy + S.at(i, l));
+      }
     }
+    return live ? float2{mean[r], rstd[r]} : float2{0.f, 0.f};
   };
   size_t first = (size_t)blockIdx.x * RPB;
-  if (first < rows) fetch(first);
+  float2 stat = {0.f, 0.f};
+  if (first < rows) stat = fetch(first);
   for (; first < rows; first += (size_t)gridDim.x * RPB) {
-    float h[N][V], g[N][V], s[2] = {0.f, 0.f};
-    const float mu = nm, rs = nr;
+    float h[N][V], g[N][V], sg = 0.f, sh = 0.f;
+    const float mu = stat.x, rs = stat.y;
     const size_t r = first + grp;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -207,17 +212,17 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void k_norm_grad(const size_t ro
         h[i][e] = ((float)nx[i].v[e] - mu) * rs;
         g[i][e] = d * vw[e];
         const float once = e >= dup ? g[i][e] : 0.f;
-        s[0] += once;
-        s[1] = fmaf(once, h[i][e], s[1]);
+        sg += once;
+        sh = fmaf(once, h[i][e], sh);
         // (what a moved-back piece adds up in its first `dup` columns is not read)
         sw[i][e] = fmaf(d, h[i][e], sw[i][e]);
         sb[i][e] += d;
       }
     }
-    if (first + (size_t)gridDim.x * RPB < rows) fetch(first + (size_t)gridDim.x * RPB);
+    if (first + (size_t)gridDim.x * RPB < rows) stat = fetch(first + (size_t)gridDim.x * RPB);
     if (!dx) continue;
-    group_sum<G>(s, lds);
-    const float a = -rs * (s[0] * inv), c = -rs * (s[1] * inv);
+    group_sum<G>(sg, sh, lds);
+    const float a = -rs * (sg * inv), c = -rs * (sh * inv);
     if (r >= rows) continue;
 #pragma unroll
     for (int i = 0; i < N; ++i) {
@@ -256,21 +261,31 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void k_norm_grad(const size_t ro
     for (int j = threadIdx.x; j < 2 * cols; j += 256) part[(size_t)blockIdx.x * 2 * cols + j] = sum[j];
 }
 
-// 32 columns by 32 shares of the partial sums
+// 16 columns by 64 shares of the partial sums
 template <class P>
 __global__ __launch_bounds__(1024) void k_norm_join(const int cols, const int parts, const float *__restrict__ part, P *__restrict__ dw,
                                                     P *__restrict__ db) {
-  __shared__ float lds[32][33];
-  const int c = threadIdx.x & 31, q = threadIdx.x >> 5;
-  const size_t j = (size_t)blockIdx.x * 32 + c, n = 2 * (size_t)cols;
+  __shared__ float lds[64][17];
+  const int c = threadIdx.x & 15, q = threadIdx.x >> 4;
+  const size_t j = (size_t)blockIdx.x * 16 + c, n = 2 * (size_t)cols;
   float s = 0.f;
   if (j < n)
-    for (int p = q; p < parts; p += 32) s += part[p * n + j];
+#pragma unroll 4
+    for (int p = q; p < parts; p += 64) s += part[p * n + j];
   lds[q][c] = s;
   __syncthreads();
-  if (q == 0 && j < n) {
-    s = 0.f;
-    for (int i = 0; i < 32; ++i) s += lds[i][c];
+  if (threadIdx.x < 256) {
+    // four shares a thread, then the four quarters of a column's sixteen
+    const int h = threadIdx.x >> 4;
+    s = (lds[4 * h][c] + lds[4 * h + 1][c]) + (lds[4 * h + 2][c] + lds[4 * h + 3][c]);
+    s += __shfl_xor(s, 16);
+    s += __shfl_xor(s, 32);
+  }
+  __syncthreads();
+  if (threadIdx.x < 256 && (threadIdx.x & 63) < 16) lds[threadIdx.x >> 6][c] = s;
+  __syncthreads();
+  if (threadIdx.x < 16 && j < n) {
+    s = (lds[0][c] + lds[1][c]) + (lds[2][c] + lds[3][c]);
     if (j < (size_t)cols) {
       if (dw) dw[j] = (P)s;
     } else if (db) {
@@ -284,9 +299,7 @@ __global__ __launch_bounds__(1024) void k_norm_join(const int cols, const int pa
 // the sum over a workgroup of 256, in every thread
 __device__ __forceinline__ float block_sum(float v) {
   __shared__ float lds[8];
-  float a[1] = {v};
-  group_sum<256>(a, lds);
-  return a[0];
+  return group_sum<256>(v, lds);
 }
 
 template <class T, class P>
@@ -458,7 +471,7 @@ extern "C" int qr_layer_norm_backward_async(int device, void *stream, int type, 
         const unsigned grid = (unsigned)(want < parts ? want : parts);
         k_norm_grad<T, P, G(), N()><<<grid, G() > 256 ? G() : 256, RPB > 1 && sums ? 2 * cols * 4 : 0, s>>>(
             rows, (int)cols, (const T *)dy, lddy, (const T *)x, ldx, (const P *)weight, mean, rstd, (T *)dx, lddx, part);
-        if (sums) k_norm_join<P><<<(unsigned)((2 * cols + 31) / 32), 1024, 0, s>>>((int)cols, (int)grid, part, (P *)dweight, (P *)dbias);
+        if (sums) k_norm_join<P><<<(unsigned)((2 * cols + 15) / 16), 1024, 0, s>>>((int)cols, (int)grid, part, (P *)dweight, (P *)dbias);
       });
       if (fits && rows) return;
       // (the column sums first: dx may be written over dy or x)
@@ -466,7 +479,7 @@ extern "C" int qr_layer_norm_backward_async(int device, void *stream, int type, 
         k_norm_cols<T><<<dim3((unsigned)((cols + 255) / 256), any), 256, 0, s>>>(rows, (int)cols, (const T *)dy, lddy, (const T *)x,
                                                                                   ldx, mean, rstd, part);
       if (sums)
-        k_norm_join<P><<<(unsigned)((2 * cols + 31) / 32), 1024, 0, s>>>((int)cols, (int)any, part, (P *)dweight, (P *)dbias);
+        k_norm_join<P><<<(unsigned)((2 * cols + 15) / 16), 1024, 0, s>>>((int)cols, (int)any, part, (P *)dweight, (P *)dbias);
       if (rows && dx)
         k_norm_grad_any<T, P><<<(unsigned)(rows < 65536 ? rows : 65536), 256, 0, s>>>(
             rows, (int)cols, (const T *)dy, lddy, (const T *)x, ldx, (const P *)weight, mean, rstd, (T *)dx, lddx);

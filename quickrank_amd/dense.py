@@ -47,13 +47,14 @@ def _check(t, what, like=None):
 def _rows(t, what, like=None):
     """(rows, cols, stride) of a tensor read as a matrix of its last dimension."""
     _check(t, what, like)
-    if t.dim() == 0:
+    shape = t.shape
+    if not shape:
         _refuse(f"{what} has no dimension")
-    cols = t.shape[-1]
+    cols = shape[-1]
     if t.is_contiguous():
         return (t.numel() // cols if cols else 0), cols, cols
-    if t.dim() == 2 and (t.stride(1) == 1 or cols == 1):
-        return t.shape[0], cols, t.stride(0) if t.shape[0] > 1 else cols
+    if len(shape) == 2 and (t.stride(1) == 1 or cols == 1):
+        return shape[0], cols, t.stride(0) if shape[0] > 1 else cols
     _refuse(f"{what} is neither contiguous nor a matrix of contiguous rows")
 
 
@@ -92,13 +93,13 @@ def layer_norm(x, weight=None, bias=None, eps=1e-5):
     if weight is not None and bias is not None and weight.dtype != bias.dtype:
         _refuse("weight and bias have two types")
     p = weight if weight is not None else bias if bias is not None else x
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    stats = torch.empty((2, rows), dtype=torch.float32, device=x.device)
-    mean, rstd = stats[0], stats[1]
+    y, stats = x.new_empty(x.shape), x.new_empty((2, rows), dtype=torch.float32)
+    at = stats.data_ptr()
     rc = lib().qr_layer_norm_async(x.device.index, _stream(x), TYPES[x.dtype], TYPES[p.dtype], rows, cols, x.data_ptr(), ld,
-                                   w, b, eps, y.data_ptr(), cols, mean.data_ptr(), rstd.data_ptr())
+                                   w, b, eps, y.data_ptr(), cols, at, at + 4 * rows)
     if rc:
         _fail(rc)
+    mean, rstd = stats.unbind(0)
     return y, mean, rstd
 
 
@@ -114,17 +115,18 @@ def layer_norm_backward(dy, x, weight, mean, rstd, param_dtype=None):
     if pt != x.dtype and pt != torch.float32:
         _refuse("weight and bias have the rows' type or f32")
     m, r = _stat(mean, "mean", x, rows), _stat(rstd, "rstd", x, rows)
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    dp = torch.empty((2, cols), dtype=pt, device=x.device)
+    dx, dp = x.new_empty(x.shape), x.new_empty((2, cols), dtype=pt)
+    at = dp.data_ptr()
     need = C.c_size_t()
     rc = lib().qr_layer_norm_backward_workspace(rows, cols, C.byref(need))
-    ws = torch.empty(need.value, dtype=torch.uint8, device=x.device)
+    ws = x.new_empty(need.value, dtype=torch.uint8)
     rc = rc or lib().qr_layer_norm_backward_async(
         x.device.index, _stream(x), TYPES[x.dtype], TYPES[pt], rows, cols, dy.data_ptr(), lddy, x.data_ptr(), ldx, w, m, r,
-        dx.data_ptr(), cols, dp.data_ptr(), dp[1].data_ptr(), ws.data_ptr(), need.value)
+        dx.data_ptr(), cols, at, at + cols * dp.element_size(), ws.data_ptr(), need.value)
     if rc:
         _fail(rc)
-    return dx, dp[0], dp[1]
+    dweight, dbias = dp.unbind(0)
+    return dx, dweight, dbias
 
 
 def _dropout(x, p, seed, offset, residual, counter):
@@ -135,7 +137,7 @@ def _dropout(x, p, seed, offset, residual, counter):
         _refuse("counter is one int64 on the device of x")
     if not 0.0 <= p <= 1.0:
         _refuse("dropout: p is a number of 0 to 1")
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    y = x.new_empty(x.shape)
     rc = lib().qr_dropout_async(x.device.index, _stream(x), TYPES[x.dtype], rows, cols, x.data_ptr(), ld,
                                 residual.data_ptr() if residual is not None else None, ldr, y.data_ptr(), cols, p,
                                 seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF,
@@ -163,15 +165,16 @@ def dropout_words(x):
 
 
 def _weights(x, k, w_gate, w_up):
-    for w, what in ((w_gate, "w_gate"), (w_up, "w_up")):
-        _check(w, what, x)
-        if w.dim() != 2 or w.dtype != x.dtype or w.shape[1] != k or (w.stride(1) != 1 and k > 1):
-            _refuse(f"{what} is a matrix of contiguous rows, [n][columns of x], of the type of x")
-    if w_gate.shape != w_up.shape or (w_gate.stride(0) != w_up.stride(0) and w_gate.shape[0] > 1):
-        _refuse("w_gate and w_up differ in shape or stride")
-    if k == 0 or w_gate.shape[0] == 0:
+    _check(w_gate, "w_gate", x)
+    _check(w_up, "w_up", x)
+    shape, stride = w_gate.shape, w_gate.stride()
+    if len(shape) != 2 or shape[1] != k or w_gate.dtype != x.dtype or (stride[1] != 1 and k > 1):
+        _refuse("w_gate is a matrix of contiguous rows, [n][columns of x], of the type of x")
+    if w_up.shape != shape or w_up.dtype != x.dtype or (w_up.stride() != stride and shape[0] > 1 and k > 1):
+        _refuse("w_up differs from w_gate in shape, stride or type")
+    if k == 0 or shape[0] == 0:
         _refuse("gated ffn: no columns")
-    return w_gate.shape[0], w_gate.stride(0) if w_gate.shape[0] > 1 else k
+    return shape[0], stride[0] if shape[0] > 1 else k
 
 
 def _act(act):
@@ -187,14 +190,13 @@ def gated_ffn(x, w_gate, w_up, act="silu", save=False):
     n, ldw = _weights(x, k, w_gate, w_up)
     a = _act(act)
     shape = x.shape[:-1] + (n,)
-    h = torch.empty(shape, dtype=x.dtype, device=x.device)
-    g = torch.empty(shape, dtype=x.dtype, device=x.device) if save else None
-    u = torch.empty(shape, dtype=x.dtype, device=x.device) if save else None
+    h = x.new_empty(shape)
+    g, u = (x.new_empty(shape), x.new_empty(shape)) if save else (None, None)
     px, pg, pu, e = x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), x.element_size()
     ws, need, rc = None, C.c_size_t(), 0
     if (px | pg | pu | ldx * e | ldw * e) & 15:  # rows that do not start at 16-byte boundaries
         rc = lib().qr_gated_ffn_workspace(TYPES[x.dtype], m, k, n, C.byref(need))
-        ws = torch.empty(need.value, dtype=torch.uint8, device=x.device)
+        ws = x.new_empty(need.value, dtype=torch.uint8)
     rc = rc or lib().qr_gated_ffn_async(x.device.index, _stream(x), TYPES[x.dtype], a, m, k, n, px, ldx, pg, pu, ldw, h.data_ptr(), n,
                                         g.data_ptr() if save else None, u.data_ptr() if save else None,
                                         ws.data_ptr() if ws is not None else None, need.value)
@@ -215,15 +217,16 @@ def gated_ffn_backward(dh, x, w_gate, w_up, gate, up, act="silu"):
     if not gate.is_contiguous() or not up.is_contiguous():
         _refuse("gate and up are contiguous, as the forward call returns them")
     lddh = _rows(dh, "dh")[2]
-    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    dw = torch.empty((2, n, k), dtype=x.dtype, device=x.device)
+    dx, dw = x.new_empty(x.shape), x.new_empty((2, n, k))
+    at = dw.data_ptr()
     need = C.c_size_t()
     rc = lib().qr_gated_ffn_backward_workspace(TYPES[x.dtype], m, k, n, C.byref(need))
-    ws = torch.empty(need.value if not rc else 0, dtype=torch.uint8, device=x.device)
+    ws = x.new_empty(need.value, dtype=torch.uint8)
     rc = rc or lib().qr_gated_ffn_backward_async(
         x.device.index, _stream(x), TYPES[x.dtype], a, m, k, n, dh.data_ptr(), lddh, x.data_ptr(), ldx, w_gate.data_ptr(),
-        w_up.data_ptr(), ldw, gate.data_ptr(), up.data_ptr(), dx.data_ptr(), k, dw.data_ptr(), dw[1].data_ptr(), ws.data_ptr(),
+        w_up.data_ptr(), ldw, gate.data_ptr(), up.data_ptr(), dx.data_ptr(), k, at, at + n * k * dw.element_size(), ws.data_ptr(),
         need.value)
     if rc:
         _fail(rc)
-    return dx, dw[0], dw[1]
+    dw_gate, dw_up = dw.unbind(0)
+    return dx, dw_gate, dw_up

@@ -62,10 +62,24 @@ def ffn(L, type=0, act=0, m=4, k=8, n=16, x=P, ldx=8, wg=Q, wu=R, ldw=8, h=R + Q
 @pytest.mark.parametrize("bad", [dict(type=5), dict(act=5), dict(act=-1), dict(k=0), dict(n=0), dict(m=1 << 60), dict(ldh=15),
                                  dict(g=P + Q), dict(u=P + Q), dict(x=None), dict(wg=None), dict(wu=None), dict(h=None), dict(h=P + 64),
                                  dict(h=Q), dict(h=R + 128), dict(g=R + Q + 32, u=R + R), dict(g=R + R, u=R + R + 255),
-                                 dict(g=P, u=R + R), dict(x=P + 4), dict(ldx=9), dict(ldw=10), dict(wu=R + 8), dict(x=P + 4, ws=2 * R),
-                                 dict(x=P + 4, ws=2 * R, nbytes=256), dict(x=P + 4, ws=R, nbytes=1 << 20)])
+                                 dict(g=P, u=R + R)])
 def test_ffn_refusals(L, bad):
     assert ffn(L, **bad) == ARG and message(L).startswith("gated ffn")
+
+
+@pytest.mark.parametrize("bad", [dict(x=P + 4), dict(ldx=9), dict(ldw=10), dict(wu=R + 8), dict(x=P + 4, ws=2 * R),
+                                 dict(x=P + 4, ws=2 * R, nbytes=256), dict(x=P + 4, ws=R, nbytes=1 << 20)])
+def test_ffn_many_rows_off_boundaries_need_the_workspace(L, bad):
+    assert ffn(L, m=200, n=4096, ldh=4096, **bad) == ARG and message(L).startswith("gated ffn")
+
+
+def test_ffn_rows_beyond_4_mb_are_unsupported(L):
+    k = (1 << 20) + 1
+    assert ffn(L, m=200, n=4096, ldh=4096, k=k, ldx=k, ldw=k, wu=64 * R, h=128 * R, ws=256 * R, nbytes=1 << 50) == 5
+    assert ffn_back(L, m=200, k=k, x=2 * Q, wg=8 * R, wu=16 * R, g=32 * R, u=64 * R, dx=128 * R, lddx=k, dwg=256 * R, dwu=512 * R,
+                    ws=1024 * R, nbytes=1 << 50) == 5
+    assert ffn_back(L, m=200, n=k, dh=16 * R, lddh=k, x=2 * Q, wg=8 * R, wu=20 * R, g=32 * R, u=64 * R, dx=128 * R, dwg=256 * R,
+                    dwu=512 * R, ws=1024 * R, nbytes=1 << 50) == 5
 
 
 def ffn_back(L, type=0, act=0, m=4, k=8, n=16, dh=P, lddh=16, x=Q, wg=R, wu=R + P, g=R + Q, u=2 * R, dx=2 * R + P, lddx=8,
