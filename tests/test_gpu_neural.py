@@ -1,0 +1,88 @@
+"""The neural scorer (quickrank_amd/neural.py): the dense operators run together, under the lambda pass."""
+import numpy as np
+import pytest
+import torch
+
+from datagen import make_dataset
+
+pytestmark = pytest.mark.gpu
+
+
+def scorer(**kw):
+    from quickrank_amd.neural import NeuralScorer
+    return NeuralScorer(**{**dict(blocks=2, units=48, drop=0.2, steps=3, seed=5), **kw})
+
+
+def reference(s, x, offsets):
+    """Scores of the same parameters in 64 bits (leaves that autograd follows), masks from the operator itself."""
+    from quickrank_amd import dense
+    p = {k: v.double().requires_grad_(True) for k, v in s.params.items()}
+
+    def norm(z, name):
+        mean, var = z.mean(1, keepdim=True), z.var(1, keepdim=True, unbiased=False)
+        return (z - mean) / (var + 1e-5).sqrt() * p[f"norm_{name}.weight"] + p[f"norm_{name}.bias"]
+    z = norm(x.double(), "in")
+    for b in range(s.blocks):
+        y = norm(z, b)
+        g = y @ p[f"gate_{b}"].T
+        h = (g * torch.sigmoid(g) * (y @ p[f"up_{b}"].T)) @ p[f"down_{b}"].T
+        if offsets is not None:
+            # (in f32: the scale is that of the mask's 16 bits)
+            h = h * dense.dropout(torch.ones(h.shape, device=h.device), s.drop, s.seed, offsets[b]).double()
+        z = z + h
+    return norm(z, "out") @ p["score"], p
+
+
+def test_scores_and_gradients_against_64_bits():
+    """136 features, 48 units, 300 documents.  Every product and sum is f32 over at most 300 terms: 2^-24 a step, some
+    300 steps a layer, seven layers forward and seven back, relative to the largest value of a result."""
+    s = scorer()
+    x = torch.randn(300, 136, generator=torch.Generator().manual_seed(1)).cuda()
+    s.init(136)
+    tol = 2.0 ** -24 * 300 * 14
+    for train in (False, True):
+        s.drawn = 100
+        scores, kept = s.forward(x, train=train)
+        offsets = [k[7] for k in kept[1:-1]] if train else None
+        want, p = reference(s, x, offsets)
+        assert (scores.double() - want).abs().max() <= tol * want.abs().max()
+    ds = torch.randn(300, generator=torch.Generator().manual_seed(2)).cuda()
+    grads = s.backward(kept, ds)
+    (want * ds.double()).sum().backward()
+    assert set(grads) == set(s.params)
+    for name, leaf in p.items():
+        assert grads[name].shape == leaf.shape
+        assert (grads[name].double() - leaf.grad).abs().max() <= tol * leaf.grad.abs().max(), name
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_learns_from_the_lambda_pass(dtype):
+    """learn() runs on ragged queries; each step's gradient is that of the context's pseudo-responses for its scores."""
+    from quickrank_amd import Context
+    x, labels, qoff = make_dataset(nq=12, docs_per_query=25, F=40, seed=3)
+    s = scorer(dtype=dtype, units=24)
+    s.init(40)
+    before = {k: v.clone() for k, v in s.params.items()}
+    seen = []
+    inner = s.backward
+
+    def backward(kept, ds):
+        seen.append((s.ctx.get_scores(), ds.cpu().numpy()))
+        return inner(kept, ds)
+    s.backward = backward
+    s.learn(x, labels, qoff)
+    assert len(s.train_metric) == 3 and all(np.isfinite(s.train_metric)) and len(seen) == 3
+    assert all(torch.isfinite(v).all() and not torch.equal(v, before[k]) for k, v in s.params.items())
+    other = Context(0)
+    other.upload(x, labels, qoff)
+    for scores, ds in seen:
+        other.set_scores(scores)
+        other.compute_lambdas("NDCG", 10)
+        assert np.array_equal(ds, (-other.get_pseudo()[0]).astype(np.float32))
+    a, b = s.score_dataset(x), s.score_dataset(x)
+    assert a.shape == (len(x),) and np.array_equal(a, b) and np.isfinite(a).all()
+    # one document by itself: the same function of its row, by the few-rows kernels (roundings of the type apart)
+    one = s.score_dataset(x[7:8])
+    unit = 2.0 ** -24 if dtype == torch.float32 else 2.0 ** -8
+    assert abs(one[0] - a[7]) <= unit * 200 * max(1.0, np.abs(a).max())
+    other.close()
