@@ -76,6 +76,33 @@ __device__ __forceinline__ f4 mma(const i4 a, const i4 b, f4 c) {
   }
 }
 
+// f32 operands of the product kernel as three bf16 each: 24 bits of mantissa are 8 + 8 + 8, so high + mid + low IS the
+// number (down to 2^-110; an infinite one has NaN parts).  Of the nine products the six largest are taken, each exact in
+// f32; those left out are below 2^-21 of the whole, 2^-23.5 on average.  Six bf16 matrix instructions take 96 cycles for
+// 16 x 16 x 32 where the f32 ones take 256, for 5.5 vector instructions an element, which run under them.
+struct Split {
+  b8 part[3];
+};
+__device__ __forceinline__ Split three_parts(const i4 u, const i4 v) {
+  const f4 fu = __builtin_bit_cast(f4, u), fv = __builtin_bit_cast(f4, v);
+  float x[8];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) x[e] = fu[e], x[4 + e] = fv[e];
+  Split s;
+#pragma unroll
+  for (int p = 0; p < 3; ++p) {
+    i4 w;
+#pragma unroll
+    for (int e = 0; e < 4; ++e)  // the upper halves of two numbers
+      w[e] = (int)__builtin_amdgcn_perm(__builtin_bit_cast(uint32_t, x[2 * e + 1]), __builtin_bit_cast(uint32_t, x[2 * e]), 0x07060302u);
+    s.part[p] = __builtin_bit_cast(b8, w);
+    if (p < 2)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] -= __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, x[e]) & 0xFFFF0000u);
+  }
+  return s;
+}
+
 // ---- LDS tiles -----------------------------------------------------------------------------------------
 // A stage holds R rows (outputs) of KT = 128 / sizeof(T) summed elements in 128 R bytes, moved in pieces of 16.  A row's
 // 128 bytes are a whole line of the L2, whose requests, not its bytes, were the bound with rows of 64 (1159 against 1344
@@ -83,13 +110,21 @@ __device__ __forceinline__ f4 mma(const i4 a, const i4 b, f4 c) {
 //
 // Rows layout: row r at 128 r, its piece c at position c ^ (r & 7).  A 16-byte read of a wave is served in four parts,
 // lanes 0-3 12-15 20-27, 4-11 16-19 28-31 and the same 32 higher; the lanes of each touch every bank once.
-// Columns layout: summed element k at k R sizeof(T), its pieces XORed with col_swz(k) so that the lanes of one
-// read, which lie in 8 (16-bit) or 4 (f32) such lines, touch every bank once.
+// Columns layout: summed element k at k R sizeof(T), blocks of 16 elements permuted within the line (col_at) so that the
+// lanes of one read, which lie in 8 (16-bit) or 4 (f32) such lines, touch every bank once (but for widths of f32 that are
+// no power of two).
+// the position of block `b` of 16 elements in the line of summed element k
 template <class T, int R>
-__device__ __forceinline__ int col_swz(const int k) {
-  if constexpr (sizeof(T) == 4) return ((k >> 2) & (R >= 64 ? 3 : 1)) << 2;    // segments of 16 floats
-  else if constexpr (R >= 128) return ((k & 3) | (((k >> 3) & 1) << 2)) << 1;  // segments of 16 elements = 32 bytes
-  else return (((k >> 1) & 1) | (((k >> 3) & 1) << 1)) << 1;                   // two lines of 128 bytes share the banks
+__device__ __forceinline__ int col_at(const int b, const int k) {
+  if constexpr (sizeof(T) == 4) {
+    const int f = (k >> 2) & 3;
+    if constexpr ((R & (R - 1)) == 0) return b ^ f;
+    else return b + f >= R / 16 ? b + f - R / 16 : b + f;
+  } else if constexpr (R >= 128) {
+    return b ^ ((k & 3) | (((k >> 3) & 1) << 2));
+  } else {
+    return b ^ (((k >> 1) & 1) | (((k >> 3) & 1) << 1));  // two lines of 128 bytes share the banks
+  }
 }
 
 // the piece q (of R * 8) of a stage in LDS order -> where it comes from
@@ -100,15 +135,21 @@ __device__ __forceinline__ void piece_of(const int q, int &r, int &k) {
     r = q >> 3;
     k = ((q & 7) ^ (r & 7)) * E;
   } else {
-    constexpr int PER = R / E;
+    constexpr int PER = R / E, B = 16 / E;  // pieces of a line, of a block
     k = q / PER;
-    r = ((q % PER) ^ col_swz<T, R>(k)) * E;
+    const int at = (q % PER) / B;
+    int b = col_at<T, R>(at, k);  // (exclusive or undoes itself)
+    if constexpr ((R & (R - 1)) != 0) {
+      b = at - ((k >> 2) & 3);
+      b = b < 0 ? b + R / 16 : b;
+    }
+    r = b * 16 + (q % B) * E;
   }
 }
 
-// One operand fragment: 16 rows of one half (0, 1) of a stage, the c-th block of 16 behind the wave's first (a multiple of
-// the blocks a wave has).  `at` is the LDS address frag_base gave for block 0 of half 0; in the columns layout a block's
-// number is XORed in, in the rows layout the half's.
+// One operand fragment: 16 rows of one half (0, 1) of a stage, the c-th block of 16 behind the wave's first, `block` (a
+// multiple of the blocks a wave has).  `at` is the address frag_base gave; a block's number and the half are XORed in where
+// they can be.
 template <class T, int R, bool KS>
 __device__ __forceinline__ uint32_t frag_base(const uint32_t stage, const int block) {
   const int l = threadIdx.x & 63, g = l >> 4, i = l & 15;
@@ -116,13 +157,13 @@ __device__ __forceinline__ uint32_t frag_base(const uint32_t stage, const int bl
     return stage + (block * 16 + i) * 128 + ((g ^ (i & 7)) << 4);
   } else if constexpr (sizeof(T) == 2) {
     const int k = 8 * g + (i >> 2);
-    return stage + ((k * (R * 2) + (col_swz<T, R>(k) << 4) + (i & 3) * 8) ^ (block << 5));
+    return stage + k * (R * 2) + (col_at<T, R>(block, k) << 5) + (i & 3) * 8;
   } else {
-    return stage + ((4 * g * (R * 4) + (col_swz<T, R>(4 * g) << 4) + i * 4) ^ (block << 6));
+    return stage + 4 * g * (R * 4) + i * 4;
   }
 }
 template <class T, int R, bool KS>
-__device__ __forceinline__ i4 frag(const uint32_t at, const int c, const int half) {
+__device__ __forceinline__ i4 frag(const uint32_t at, const int block, const int c, const int half) {
   if constexpr (!KS) {
     return *(QR_LDS const i4 *)((at ^ (half << 6)) + c * 2048);
   } else if constexpr (sizeof(T) == 2) {
@@ -131,7 +172,7 @@ __device__ __forceinline__ i4 frag(const uint32_t at, const int c, const int hal
     const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((QR_LDS s4 *)(p + 4 * R * 2));
     return __builtin_bit_cast(i4, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
   } else {
-    const uint32_t p = (at ^ (c << 6)) + half * (16 * R * 4);
+    const uint32_t p = at + (col_at<T, R>(block + c, 4 * ((threadIdx.x & 63) >> 4)) << 6) + half * (16 * R * 4);
     i4 v;
 #pragma unroll
     for (int e = 0; e < 4; ++e) v[e] = *(QR_LDS const int *)(p + e * R * 4);
@@ -332,26 +373,53 @@ __global__ __launch_bounds__(256, 2) void k_gemm(const GemmArgs<T> P) {
     for (int n = 0; n < NI; ++n) acc[m][n] = f4{0.f, 0.f, 0.f, 0.f};
   const uint32_t base_a = frag_base<T, TM, AKS>(lds_offset(lds), wm * MI);
   const uint32_t base_b = frag_base<T, TN, BKS>(lds_offset(lds) + 2 * ABUF, wn * NI);
-  // a stage's 2 x MI rows of blocks: the first operand's fragments are read D ahead of their use
-  constexpr int D = MI > 3 ? 3 : MI - 1;
+  auto read_a = [&](const uint32_t ra, const int m, const int half) { return frag<T, TM, AKS>(ra, wm * MI, m, half); };
+  auto read_b = [&](const int n, const int half) { return frag<T, TN, BKS>(base_b, wn * NI, n, half); };
+  // 16-bit types: a stage's 2 x MI rows of blocks, the first operand's fragments read D ahead of their use.
+  // f32: its MI rows of blocks, split into three parts, one ahead.  In the steady state the next stage's loads are spread
+  // over the rows.
   auto compute = [&](auto steady, const uint32_t ra, const uint32_t to) {
-    i4 fa[D + 1], fb[2][NI];
+    constexpr bool STEADY = decltype(steady)::value;
+    if constexpr (sizeof(T) == 4) {
+      Split fb[NI];
+      i4 next[2] = {read_a(ra, 0, 0), read_a(ra, 0, 1)};
 #pragma unroll
-    for (int n = 0; n < NI; ++n) fb[0][n] = frag<T, TN, BKS>(base_b, n, 0);
+      for (int n = 0; n < NI; ++n) fb[n] = three_parts(read_b(n, 0), read_b(n, 1));
 #pragma unroll
-    for (int m = 0; m < D; ++m) fa[m] = frag<T, TM, AKS>(ra, m, 0);
+      for (int m = 0; m < MI; ++m) {
+        const Split fa = three_parts(next[0], next[1]);
+        if (m + 1 < MI) next[0] = read_a(ra, m + 1, 0), next[1] = read_a(ra, m + 1, 1);
+        if constexpr (STEADY)
 #pragma unroll
-    for (int q = 0; q < 2 * MI; ++q) {
-      if (q + D < 2 * MI) fa[(q + D) % (D + 1)] = frag<T, TM, AKS>(ra, (q + D) % MI, (q + D) / MI);
-      if (q < MI)
+          for (int d = m * PA / MI; d < (m + 1) * PA / MI; ++d) load_a(d, to);
+        constexpr int HI[6] = {1, 0, 2, 0, 1, 0}, LO[6] = {1, 2, 0, 1, 0, 0};  // the smallest first
 #pragma unroll
-        for (int n = q * NI / MI; n < (q + 1) * NI / MI; ++n) fb[1][n] = frag<T, TN, BKS>(base_b, n, 1);
-      if constexpr (decltype(steady)::value)
+        for (int p = 0; p < 6; ++p)
 #pragma unroll
-        for (int d = q * PA / MI / 2; d < (q + 1) * PA / MI / 2; ++d) load_a(d, to);
+          for (int n = 0; n < NI; ++n)
+            acc[m][n] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[n].part[HI[p]], fa.part[LO[p]], acc[m][n], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    } else {
+      constexpr int D = MI > 3 ? 3 : MI - 1;
+      i4 fa[D + 1], fb[2][NI];
 #pragma unroll
-      for (int n = 0; n < NI; ++n) acc[q % MI][n] = mma<T>(fb[q / MI][n], fa[q % (D + 1)], acc[q % MI][n]);
-      __builtin_amdgcn_sched_barrier(0);
+      for (int n = 0; n < NI; ++n) fb[0][n] = read_b(n, 0);
+#pragma unroll
+      for (int m = 0; m < D; ++m) fa[m] = read_a(ra, m, 0);
+#pragma unroll
+      for (int q = 0; q < 2 * MI; ++q) {
+        if (q + D < 2 * MI) fa[(q + D) % (D + 1)] = read_a(ra, (q + D) % MI, (q + D) / MI);
+        if (q < MI)
+#pragma unroll
+          for (int n = q * NI / MI; n < (q + 1) * NI / MI; ++n) fb[1][n] = read_b(n, 1);
+        if constexpr (STEADY)
+#pragma unroll
+          for (int d = q * PA / MI / 2; d < (q + 1) * PA / MI / 2; ++d) load_a(d, to);
+#pragma unroll
+        for (int n = 0; n < NI; ++n) acc[q % MI][n] = mma<T>(fb[q / MI][n], fa[q % (D + 1)], acc[q % MI][n]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
     }
   };
   if (first < last) {
@@ -389,11 +457,15 @@ __global__ __launch_bounds__(256, 2) void k_gemm(const GemmArgs<T> P) {
   }
 
   // Results pass through the wave's own share of the LDS, so that a lane ends with eight neighbours of a row: one
-  // wide store, and one copy of the activation's code.  Pieces of four are XORed with the row against bank conflicts.
+  // wide store, and one copy of the activation's code.  Pieces of four are moved by the row against bank conflicts.
   constexpr int WTN = NI * 16, PIECES = WTN / 4, SHARE = LDS_BYTES / 4 / (16 * WTN * 4) * (16 * WTN * 4);
   constexpr int FIT = SHARE / (16 * WTN * 4), MB = FIT >= MI ? MI : FIT >= MI / 2 ? MI / 2 : MI / 4;  // blocks of 16 rows at a time
   static_assert(MB > 0 && MB <= FIT && MI % MB == 0 && PA % MI == 0, "blocks fit the waves' shares");
   char *const own = lds + wave * SHARE;
+  auto at = [&](const int row, const int piece) -> f4 * {
+    const int r = row & 15, c = (PIECES & (PIECES - 1)) == 0 ? piece ^ (r & (PIECES - 1)) : (piece + r) % PIECES;
+    return (f4 *)(own + (row * PIECES + c) * 16);
+  };
   const int l = tid & 63;
 #pragma unroll
   for (int m0 = 0; m0 < MI; m0 += MB) {
@@ -401,7 +473,7 @@ __global__ __launch_bounds__(256, 2) void k_gemm(const GemmArgs<T> P) {
     for (int m = 0; m < MB; ++m)
 #pragma unroll
       for (int n = 0; n < NI; ++n)
-        *(f4 *)(own + ((m * 16 + (l & 15)) * PIECES + ((n * 4 + (l >> 4)) ^ (l & 15 & (PIECES - 1)))) * 16) = acc[m0 + m][n];
+        *at(m * 16 + (l & 15), n * 4 + (l >> 4)) = acc[m0 + m][n];
     __builtin_amdgcn_wave_barrier();
     constexpr int SEGS = (KIND == FWD ? WTN / 2 : WTN) / 8;  // eight outputs a lane
 #pragma unroll 1
@@ -411,7 +483,7 @@ __global__ __launch_bounds__(256, 2) void k_gemm(const GemmArgs<T> P) {
       auto take = [&](int piece, float (&v)[8]) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const f4 x = *(const f4 *)(own + (r * PIECES + ((piece + h) ^ (r & 15 & (PIECES - 1)))) * 16);
+          const f4 x = *at(r, piece + h);
 #pragma unroll
           for (int e = 0; e < 4; ++e) v[h * 4 + e] = x[e];
         }
@@ -644,15 +716,19 @@ struct Tile {
 };
 
 // Sums a workgroup takes: 256 x 128 (16-bit types) or 128 x 128 where that gives every compute unit a tile, else 64 x 64.
-// Gradients may be narrow (features): a width of 64 or, in f32, whose matrix instructions hide the reads of narrow
-// tiles, 32 is taken where it pads the columns less.  (100000 x 136 x 512 f32, width 128 / 32: dx 436 / 273, dw 384 / 287 us.)
+// Gradients may be narrow (features), and a width of 128 would pad 136 columns to 256: there the width is the one whose
+// tiles cost least.  16-bit types, 64 against 128: the columns.  f32, 64, 96, 128 or 160: by a wave's cycles per stage, of
+// its matrix instructions (4 rows of blocks of 6 x 16 each) or of the splitting of its 4 + width / 32 blocks (44 x 4 each).
 Tile tile_of(size_t e, size_t rows, size_t cols, size_t times, bool narrow) {
-  int w = 128;
-  if (narrow)
-    for (int v = 64; v >= (e == 4 ? 32 : 64); v /= 2)
-      if ((size_t)tiles_of(cols, v) * v < (size_t)tiles_of(cols, w) * w) w = v;
+  size_t w = 128, least = ~(size_t)0;
+  for (size_t v = 64; v <= 160 && narrow; v += 32) {
+    if (e == 2 && v % 64) continue;
+    const size_t b = v / 32, mat = 4 * b * 96, vec = (4 + b) * 176;
+    const size_t cost = tiles_of(cols, v) * (e == 2 ? v : mat > vec ? mat : vec);
+    if (cost <= least && v <= (e == 2 ? 128 : 160)) least = cost, w = v;
+  }
   if (e == 2 && w == 128 && (size_t)tiles_of(rows, 256) * tiles_of(cols, 128) * times >= CUS) return {256, 128};
-  if ((size_t)tiles_of(rows, 128) * tiles_of(cols, w) * times >= CUS) return {128, w};
+  if ((size_t)tiles_of(rows, 128) * tiles_of(cols, w) * times >= CUS) return {128, (int)w};
   return {64, 64};
 }
 
@@ -663,8 +739,10 @@ void gemm(hipStream_t s, const Tile t, const GemmArgs<T> &P) {
   if (t.rows == 128 && t.cols == 128) return launch_gemm<T, KIND, 128, 128>(s, P);
   if constexpr (KIND != FWD) {
     if (t.rows == 128 && t.cols == 64) return launch_gemm<T, KIND, 128, 64>(s, P);
-    if constexpr (sizeof(T) == 4)
-      if (t.rows == 128) return launch_gemm<T, KIND, 128, 32>(s, P);
+    if constexpr (sizeof(T) == 4) {
+      if (t.rows == 128 && t.cols == 96) return launch_gemm<T, KIND, 128, 96>(s, P);
+      if (t.rows == 128 && t.cols == 160) return launch_gemm<T, KIND, 128, 160>(s, P);
+    }
   }
   launch_gemm<T, KIND, 64, 64>(s, P);
 }
