@@ -480,6 +480,7 @@ int qr_oblivious_score(qr_ctx *ctx, const float *rowmajor, size_t N, size_t F,
 /* y = (x - mean) rstd weight + bias over rows of `cols`, rstd = 1 / sqrt(var + eps),  */
 /* the variance that of the row itself (divided by cols).  weight / bias: NULL = 1 / 0, */
 /* of param_type (`type` or QR_F32).  mean / rstd: f32 [rows] or NULL.  y may be x.     */
+/* (cols up to 2^24: QR_ERR_UNSUPPORTED beyond.)                                        */
 int qr_layer_norm_async(int device, void *hip_stream, int type, int param_type, size_t rows, size_t cols,
                         const void *x, size_t ldx, const void *weight, const void *bias, float eps,
                         void *y, size_t ldy, float *mean, float *rstd);
@@ -503,12 +504,14 @@ int qr_dropout_async(int device, void *hip_stream, int type, size_t rows, size_t
                      const void *residual, size_t ldr, void *y, size_t ldy, double p, uint64_t seed,
                      uint64_t offset, const uint64_t *counter);
 
-/* (Rows of x, the weights and dh of up to 4 MB: QR_ERR_UNSUPPORTED beyond.)               */
+/* (Rows of x and the weights, and backward of h, up to 4 MB: QR_ERR_UNSUPPORTED beyond.)   */
+/* f32 products: as exact as f32 sums are; an infinite factor gives NaN, numbers below        */
+/* 2^-110 lose bits.                                                                          */
 /* h [m][n] = act(x w_gate^T) * (x w_up^T); x [m][k], weights [n][k] of stride ldw.        */
 /* gate / up: NULL (serving), or [m][n] contiguous: the two products, rounded to `type`,    */
 /* for the backward pass.  Outputs must not overlap each other or an input.  The workspace   */
 /* is used (NULL, 0 will do otherwise) where a row of x or of a weight does not start at a    */
-/* 16-byte boundary: such matrices are copied to rows that do.                                */
+/* 16-byte boundary or lies more than 4 MB behind the one before: such matrices are copied.    */
 int qr_gated_ffn_workspace(int type, size_t m, size_t k, size_t n, size_t *bytes);
 int qr_gated_ffn_async(int device, void *hip_stream, int type, int act, size_t m, size_t k, size_t n,
                        const void *x, size_t ldx, const void *w_gate, const void *w_up, size_t ldw, void *h,

@@ -92,7 +92,7 @@ extern "C" int qr_dropout_async(int device, void *stream, int type, size_t rows,
                                 const uint64_t *counter) {
   QR_DENSE_ARG(qr_dense_type_ok(type), "dropout: unknown element type");
   QR_DENSE_ARG(p >= 0.0 && p <= 1.0, "dropout: p is a number of 0 to 1");
-  QR_DENSE_ARG(qr_dense_fits(rows, cols, ldx) && qr_dense_fits(rows, cols, ldy) && qr_dense_fits(rows, cols, residual ? ldr : 0),
+  QR_DENSE_ARG(qr_dense_spans(rows, cols, ldx) && qr_dense_spans(rows, cols, ldy) && qr_dense_spans(rows, cols, residual ? ldr : 0),
                "dropout: sizes out of range");
   QR_DENSE_ARG(rows < 2 || ldy >= cols, "dropout: the stride of y is shorter than a row");
   if (!rows || !cols) return QR_OK;

@@ -9,6 +9,7 @@
 // read itself).  The forward pass interleaves blocks of 16 rows of Wg and of Wu in its second operand's tile,
 // so that one lane ends with g and u of the same outputs and the activation, the product and the rounding
 // need no second kernel.
+#include <algorithm>
 #include <type_traits>
 
 #include "qr_dense.h"
@@ -227,7 +228,7 @@ struct GemmArgs {
   size_t lda, ldb;
   size_t rows, cols, k;  // outputs (FWD: of h; DW: of one dW), length of one sum (DX: of each of its two, whole stages)
   T *o[3];               // FWD: h, g, u.  DX: dx.  DW: dWg, dWu
-  float *part;           // DW: partial sums [split][2][rows][cols] where the sum is split
+  float *part;           // partial sums, DX [split][rows][cols], DW [split][2][rows][cols], where the sums are split
   size_t ldo;
   int act;
   unsigned row_tiles, col_tiles, splits, steps;  // steps: k tiles of one split
@@ -263,23 +264,18 @@ __global__ __launch_bounds__(256, 2) void k_gemm(const GemmArgs<T> P) {
 
   // consecutive workgroups go to the eight XCDs in turn: each XCD gets a run of tiles, and a run covers bands of
   // eight tile rows column by column, so that its L2 sees the same rows and columns again
-  const unsigned tiles = P.row_tiles * P.col_tiles * (KIND == DW ? 2 * P.splits : 1);
+  constexpr unsigned OUTS = KIND == DW ? 2 : 1;
+  const unsigned one = P.row_tiles * P.col_tiles, tiles = one * OUTS * (KIND == FWD ? 1 : P.splits);
   const unsigned per = (tiles + 7) / 8, id = (blockIdx.x % 8) * per + blockIdx.x / 8;
   if (id >= tiles) return;
-  unsigned t2 = id, z = 0, split = 0;
-  if constexpr (KIND == DW) {
-    split = id / (P.row_tiles * P.col_tiles * 2);
-    t2 = id % (P.row_tiles * P.col_tiles * 2);
-    z = t2 / (P.row_tiles * P.col_tiles);
-    t2 %= P.row_tiles * P.col_tiles;
-  }
+  const unsigned split = KIND == FWD ? 0 : id / (one * OUTS), z = KIND == DW ? id / one % 2 : 0, t2 = KIND == FWD ? id : id % one;
   const unsigned band = t2 / (8 * P.col_tiles), in = t2 % (8 * P.col_tiles);
   const unsigned high = P.row_tiles - band * 8 < 8 ? P.row_tiles - band * 8 : 8;
   const size_t r0 = (size_t)(band * 8 + in % high) * TM, c0 = (size_t)(in / high) * COLS;
 
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
-  const T *const a0 = KIND == DW ? P.a[z] : P.a[0];
+  const T *const a0 = P.a[z];
 
   // a row of the second operand's tile: the output column it makes, and (FWD) of which product
   auto b_row = [&](int r, size_t &row, bool &up) {
@@ -288,12 +284,13 @@ __global__ __launch_bounds__(256, 2) void k_gemm(const GemmArgs<T> P) {
   };
   const unsigned kt_all = (unsigned)((P.k + KT - 1) / KT);  // stages of one sum
   unsigned first = 0, last = KIND == DX ? 2 * kt_all : kt_all;
-  if constexpr (KIND == DW) {
+  const bool odd = KIND != DX && P.k % KT;  // (DX: both sums are whole stages)
+  unsigned whole = odd ? last - 1 : last;   // stages that are whole
+  if constexpr (KIND != FWD) {
     first = split * P.steps;
     last = first + P.steps < last ? first + P.steps : last;
+    whole = whole < last ? whole : last;
   }
-  // (DX: both sums are whole stages)
-  const unsigned whole = KIND != DX && P.k % KT && last == kt_all && last > first ? last - 1 : last;
 
   // Where this thread's pieces of a stage come from: bytes from the operand's next stage of the tile (a wave's pieces of
   // the forward pass's second operand are all of one weight; 256 rows stay below 2^31 bytes).  Rows behind the matrix are
@@ -318,8 +315,10 @@ __global__ __launch_bounds__(256, 2) void k_gemm(const GemmArgs<T> P) {
     const uint32_t rel = (uint32_t)((row < most ? row : most) - c0);
     offb[j] = (BKS ? k * (uint32_t)P.ldb + rel : rel * (uint32_t)P.ldb + k) * sizeof(T);
   }
-  const char *sa = (const char *)(a0 + (AKS ? (size_t)first * KT * P.lda + r0 : r0 * P.lda + (size_t)first * KT));
-  const char *sb = (const char *)(P.b[KIND == FWD ? wave >> 1 : 0] + (BKS ? (size_t)first * KT * P.ldb + c0 : c0 * P.ldb + (size_t)first * KT));
+  const unsigned second = KIND == DX && first >= kt_all ? 1 : 0;
+  const size_t k0 = (size_t)(first - (second ? kt_all : 0)) * KT;
+  const char *sa = (const char *)(P.a[KIND == DW ? z : second] + (AKS ? k0 * P.lda + r0 : r0 * P.lda + k0));
+  const char *sb = (const char *)(P.b[KIND == FWD ? wave >> 1 : second] + (BKS ? k0 * P.ldb + c0 : c0 * P.ldb + k0));
   // stages are loaded in order
   auto next_a = [&](const unsigned t) {
     sa += (AKS ? KT * P.lda : (size_t)KT) * sizeof(T);
@@ -502,8 +501,8 @@ __global__ __launch_bounds__(256, 2) void k_gemm(const GemmArgs<T> P) {
         }
       } else {
         take(s * 2, v);
-        if (KIND == DW && P.part) store8<(TM > 128)>(P.part + ((size_t)(split * 2 + z) * P.rows + row) * P.cols, v, col, P.cols);
-        else store8<(TM > 128)>(P.o[KIND == DW ? z : 0] + row * P.ldo, v, col, P.cols);
+        if (P.part) store8<(TM > 128)>(P.part + ((size_t)(split * OUTS + z) * P.rows + row) * P.cols, v, col, P.cols);
+        else store8<(TM > 128)>(P.o[z] + row * P.ldo, v, col, P.cols);
       }
     }
     __builtin_amdgcn_wave_barrier();
@@ -588,16 +587,33 @@ __global__ __launch_bounds__(512) void k_few(const GemmArgs<T> P) {
     }
 }
 
-// the partial sums of the weights' gradients, joined in the order of the splits
-template <class T>
-__global__ __launch_bounds__(256) void k_join(const float *__restrict__ part, const size_t n, const unsigned splits, T *__restrict__ o0,
-                                              T *__restrict__ o1) {
-  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < 2 * n; i += (size_t)gridDim.x * 256) {
-    float s = 0.f;
-    for (unsigned p = 0; p < splits; ++p) s += part[p * 2 * n + i];
-    if (i < n) o0[i] = (T)s;
-    else o1[i - n] = (T)s;
+// Partial sums joined in the order of the splits: `outs` matrices of [rows][cols], rows of stride ldo.  V = 4: four
+// neighbours of a row a thread (cols a multiple of four)
+template <class T, int V>
+__global__ __launch_bounds__(256) void k_join(const float *__restrict__ part, const size_t rows, const size_t cols, const unsigned outs,
+                                              const unsigned splits, T *__restrict__ o0, T *__restrict__ o1, const size_t ldo) {
+  const size_t n = rows * cols;
+  for (size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * V; i < outs * n; i += (size_t)gridDim.x * 256 * V) {
+    float s[V] = {}, v[V];
+#pragma unroll 4
+    for (unsigned p = 0; p < splits; ++p) {
+      __builtin_memcpy(v, part + p * outs * n + i, sizeof v);
+#pragma unroll
+      for (int e = 0; e < V; ++e) s[e] += v[e];
+    }
+    const size_t j = i < n ? i : i - n, r = n <= 0xFFFFFFFFu ? (uint32_t)j / (uint32_t)cols : j / cols;
+    T t[V];
+#pragma unroll
+    for (int e = 0; e < V; ++e) t[e] = (T)s[e];
+    __builtin_memcpy((i < n ? o0 : o1) + r * ldo + (j - r * cols), t, sizeof t);
   }
+}
+template <class T>
+void join(hipStream_t s, const float *part, size_t rows, size_t cols, unsigned outs, unsigned splits, T *o0, T *o1, size_t ldo) {
+  const size_t n = outs * rows * cols;
+  const auto grid = [](size_t t) { return (unsigned)std::min<size_t>((t + 255) / 256, 65536); };
+  if (cols % 4 == 0) k_join<T, 4><<<grid(n / 4), 256, 0, s>>>(part, rows, cols, outs, splits, o0, o1, ldo);
+  else k_join<T, 1><<<grid(n), 256, 0, s>>>(part, rows, cols, outs, splits, o0, o1, ldo);
 }
 
 // dg, du in rows of stride ld, their padding zeroed; eight elements a thread.  (The padding is at least as long as what
@@ -646,16 +662,25 @@ void gate_grad(hipStream_t s, size_t m, size_t n, int act, const void *dh, size_
   else go(std::integral_constant<int, QR_ACT_SIGMOID>{});
 }
 
-// a matrix whose rows do not start at 16-byte boundaries, copied to one whose rows do; the padding, and rows
-// up to rows_to, zeroed
+// Matrices whose rows do not start at 16-byte boundaries, copied to ones whose rows do; the padding, and rows up to
+// rows_to, zeroed.  One of up to three by blockIdx.y
 template <class T>
-__global__ __launch_bounds__(256) void k_pack(const size_t rows, const size_t cols, const T *__restrict__ p, const size_t ld,
-                                              T *__restrict__ q, const size_t to, const size_t rows_to) {
+struct Packs {
+  struct {
+    const T *p;
+    T *q;
+    size_t rows, cols, ld, to, rows_to;
+  } m[3];
+  unsigned n = 0;
+};
+template <class T>
+__global__ __launch_bounds__(256) void k_pack(const Packs<T> packs) {
   constexpr int E = 16 / sizeof(T);
-  const size_t per = to / E;
-  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < rows_to * per; i += (size_t)gridDim.x * 256) {
+  const auto &m = packs.m[blockIdx.y];
+  const size_t per = m.to / E;
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < m.rows_to * per; i += (size_t)gridDim.x * 256) {
     const size_t r = i / per, c = (i - r * per) * E;
-    *(i4 *)(q + r * to + c) = fetch16(p, ld, r, rows, c, cols);
+    *(i4 *)(m.q + r * m.to + c) = fetch16(m.p, m.ld, r, m.rows, c, m.cols);
   }
 }
 
@@ -678,19 +703,27 @@ bool in_place(const void *p, size_t ld, size_t cols, size_t e, bool columns) {
   return ((uintptr_t)p & 15) == 0 && (ld * e) % 16 == 0 && ld * e <= ROW_BYTES && (!columns || (cols * e) % 16 == 0);
 }
 
+// notes that `p` is to be copied, and makes it and its stride those of the copy
 template <class T>
-void pack(hipStream_t s, size_t rows, size_t cols, const T *&p, size_t ld, char *&ws, size_t rows_to) {
+void pack(Packs<T> &packs, size_t rows, size_t cols, const T *&p, size_t &ld, char *&ws, size_t rows_to) {
   const size_t to = padded(cols, sizeof(T));
-  if (rows) k_pack<T><<<blocks(rows_to * to * sizeof(T) / 16), 256, 0, s>>>(rows, cols, p, ld, (T *)ws, to, rows_to);
+  packs.m[packs.n++] = {p, (T *)ws, rows, cols, ld, to, rows_to};
   p = (const T *)ws;
+  ld = to;
   ws += pack_bytes(rows_to, cols, sizeof(T));
+}
+template <class T>
+void launch_pack(hipStream_t s, const Packs<T> &packs) {
+  size_t most = 0;
+  for (unsigned i = 0; i < packs.n; ++i) most = std::max(most, packs.m[i].rows_to * packs.m[i].to * sizeof(T) / 16);
+  if (packs.n && most) k_pack<T><<<dim3(blocks(most), packs.n), 256, 0, s>>>(packs);
 }
 
 template <class T, Kind KIND, int TM, int TN>
 void launch_gemm(hipStream_t s, GemmArgs<T> P) {
   P.row_tiles = tiles_of(P.rows, TM);
   P.col_tiles = tiles_of(P.cols, KIND == FWD ? TN / 2 : TN);
-  const unsigned tiles = P.row_tiles * P.col_tiles * (KIND == DW ? 2 * P.splits : 1);
+  const unsigned tiles = P.row_tiles * P.col_tiles * (KIND == FWD ? 1 : (KIND == DW ? 2 : 1) * P.splits);
   k_gemm<T, KIND, TM, TN><<<(tiles + 7) / 8 * 8, 256, 0, s>>>(P);
 }
 
@@ -700,7 +733,9 @@ constexpr unsigned CUS = 256;
 // Whether the forward pass takes the few-rows kernel: where tiles of 64 x 64 sums would leave half the compute units
 // without one, and up to one such tile of rows.  Few rows / tiles in us, back to back in a graph: k 1024, n 4096 bf16 1 row
 // 5.8 / 14.9, 64 9.8 / 14.6, 200 24 / 17; k 136, n 512 f32 100 rows 3.5 / 6.5, 512 5.8 / 6.7, 1000 8.3 / 7.0.
-bool few(size_t m, size_t n) { return m <= 64 || (size_t)tiles_of(m, 64) * tiles_of(2 * n, 64) <= CUS / 2; }
+bool few(size_t m, size_t n) {
+  return n < ((size_t)1 << 26) && (m <= 64 || (size_t)tiles_of(m, 64) * tiles_of(2 * n, 64) <= CUS / 2);
+}
 
 template <class T>
 void launch_few(hipStream_t s, const GemmArgs<T> &P) {
@@ -747,19 +782,27 @@ void gemm(hipStream_t s, const Tile t, const GemmArgs<T> &P) {
   launch_gemm<T, KIND, 64, 64>(s, P);
 }
 
-// The weights' gradients sum over all m rows: with few outputs the sum is split so that the launch fills the
-// compute units twice, in shares of at least 512 rows.
-void plan_dw(size_t e, size_t m, size_t k, size_t n, Tile &tile, unsigned &splits, unsigned &steps) {
-  const size_t kt = 128 / e, stages = (m + kt - 1) / kt;
-  const size_t most = m / 512 ? m / 512 : 1;
-  tile = tile_of(e, n, k, 2 * most, true);
-  const size_t out = 2 * (size_t)tiles_of(n, tile.rows) * tiles_of(k, tile.cols);
-  size_t want = 2 * CUS / out;  // (one workgroup more than that makes a compute unit work half as long again)
-  want = want < 1 ? 1 : want < most ? want : most;
-  steps = (unsigned)((stages + want - 1) / want);
-  if (!steps) steps = 1;
-  splits = (unsigned)((stages + steps - 1) / steps);
-  if (!splits) splits = 1;
+// How the gradients' products are made: `outs` matrices of rows x cols, sums of `stages` stages.  With few outputs the
+// sums are split so that the launch gives every compute unit two workgroups (not one more: a third makes it work half as
+// long again), in shares of at least eight stages.
+struct Plan {
+  Tile tile;
+  unsigned splits, steps;
+};
+Plan plan(size_t e, size_t rows, size_t cols, size_t outs, size_t stages) {
+  const size_t most = std::max<size_t>(stages / 8, 1);
+  Plan p;
+  p.tile = tile_of(e, rows, cols, outs * most, true);
+  const size_t one = std::max<size_t>(outs * tiles_of(rows, p.tile.rows) * tiles_of(cols, p.tile.cols), 1);  // (no rows)
+  const size_t want = std::min(std::max<size_t>(2 * CUS / one, 1), most);
+  p.steps = (unsigned)std::max<size_t>((stages + want - 1) / want, 1);
+  p.splits = (unsigned)std::max<size_t>((stages + p.steps - 1) / p.steps, 1);
+  return p;
+}
+Plan plan_dx(size_t e, size_t m, size_t k, size_t n) { return plan(e, m, k, 1, 2 * stages_of(n, e) * e / 128); }
+Plan plan_dw(size_t e, size_t m, size_t k, size_t n) { return plan(e, n, k, 2, (m * e + 127) / 128); }
+size_t part_bytes(const Plan &p, size_t rows, size_t cols, size_t outs) {
+  return p.splits > 1 ? round256(p.splits * outs * rows * cols * 4) : 0;
 }
 
 }  // namespace
@@ -789,7 +832,7 @@ extern "C" int qr_gated_ffn_async(int device, void *stream, int type, int act, s
   if (px || pw)
     if (int rc = qr_gated_ffn_workspace(type, m, k, n, &need)) return rc;
   QR_DENSE_ARG(!need || (workspace && workspace_bytes >= need),
-               "gated ffn: rows that do not start at 16-byte boundaries need the workspace");
+               "gated ffn: rows off 16-byte boundaries or more than 4 MB apart need the workspace");
   if (!few(m, n) && k * e > ROW_BYTES) return qr_dense_fail(QR_ERR_UNSUPPORTED, "gated ffn: rows longer than 4 MB");
   const void *out[4] = {h, gate, up, workspace};
   const size_t bytes[4] = {qr_dense_span(m, n, ldh, e), m * n * e, m * n * e, need};
@@ -809,8 +852,13 @@ extern "C" int qr_gated_ffn_async(int device, void *stream, int type, int act, s
     P.a[0] = (const T *)x, P.b[0] = (const T *)w_gate, P.b[1] = (const T *)w_up;
     P.lda = ldx, P.ldb = ldw, P.rows = m, P.cols = n, P.k = k;
     P.o[0] = (T *)h, P.o[1] = (T *)gate, P.o[2] = (T *)up, P.ldo = ldh, P.act = act;
-    if (px) pack(s, m, k, P.a[0], ldx, ws, m), P.lda = padded(k, e);
-    if (pw) pack(s, n, k, P.b[0], ldw, ws, n), pack(s, n, k, P.b[1], ldw, ws, n), P.ldb = padded(k, e);
+    Packs<T> packs;
+    if (px) pack(packs, m, k, P.a[0], P.lda, ws, m);
+    if (pw) {
+      size_t ld = ldw;
+      pack(packs, n, k, P.b[0], ld, ws, n), pack(packs, n, k, P.b[1], P.ldb, ws, n);
+    }
+    launch_pack(s, packs);
     if (few(m, n)) launch_few(s, P);
     else gemm<T, FWD>(s, tile_of(e, m, 2 * n, 1, false), P);
   });
@@ -821,11 +869,10 @@ extern "C" int qr_gated_ffn_backward_workspace(int type, size_t m, size_t k, siz
   QR_DENSE_ARG(bytes && qr_dense_type_ok(type) && k > 0 && n > 0 && qr_dense_fits(m, n, n) && qr_dense_fits(m, k, k) && qr_dense_fits(n, k, k),
                "gated ffn backward: bad size");
   const size_t e = qr_dense_size(type);
-  Tile tile;
-  unsigned splits, steps;
-  plan_dw(e, m, k, n, tile, splits, steps);
-  // dg, du, the partial sums, copies of x and the weights where their rows are not aligned
-  *bytes = m ? 2 * pack_bytes(m, stages_of(n, e), e) + round256(splits > 1 ? (size_t)splits * 2 * n * k * 4 : 0) + pack_bytes(m, k, e) +
+  // dg, du, the partial sums (dx is made before the weights' gradients), copies of x and the weights where their rows are
+  // not aligned
+  *bytes = m ? 2 * pack_bytes(m, stages_of(n, e), e) +
+                   std::max(part_bytes(plan_dx(e, m, k, n), m, k, 1), part_bytes(plan_dw(e, m, k, n), n, k, 2)) + pack_bytes(m, k, e) +
                    2 * pack_bytes(stages_of(n, e), k, e) + 256
              : 0;
   return QR_OK;
@@ -866,25 +913,30 @@ extern "C" int qr_gated_ffn_backward_async(int device, void *stream, int type, i
     T *const dg = (T *)ws, *const du = (T *)(ws + pack_bytes(m, ld, e));
     ws += 2 * pack_bytes(m, ld, e);
     if (m) gate_grad<T>(s, m, n, act, dh, lddh, gate, up, dg, du, ld);
+    const Plan px = plan_dx(e, m, k, n), pw = plan_dw(e, m, k, n);
+    float *const part = (float *)ws;
+    if (m) ws += std::max(part_bytes(px, m, k, 1), part_bytes(pw, n, k, 2));
+    GemmArgs<T> X{}, W{};
+    X.a[0] = dg, X.a[1] = du, X.b[0] = (const T *)w_gate, X.b[1] = (const T *)w_up;
+    X.lda = ld, X.ldb = ldw, X.rows = m, X.cols = k, X.k = ld, X.o[0] = (T *)dx, X.ldo = lddx;
+    W.a[0] = dg, W.a[1] = du, W.b[0] = (const T *)x;
+    W.lda = ld, W.ldb = ldx, W.rows = n, W.cols = k, W.k = m, W.o[0] = (T *)dw_gate, W.o[1] = (T *)dw_up, W.ldo = k;
+    Packs<T> packs;
+    if (dx && m && (ld != n || !in_place(w_gate, ldw, k, e, true) || !in_place(w_up, ldw, k, e, true))) {
+      size_t to = ldw;
+      pack(packs, n, k, X.b[0], to, ws, ld), pack(packs, n, k, X.b[1], X.ldb, ws, ld);
+    }
+    if (dw_gate && m && !in_place(x, ldx, k, e, true)) pack(packs, m, k, W.b[0], W.ldb, ws, m);
+    launch_pack(s, packs);
     if (dx && m) {
-      GemmArgs<T> P{};
-      P.a[0] = dg, P.a[1] = du, P.b[0] = (const T *)w_gate, P.b[1] = (const T *)w_up;
-      P.lda = ld, P.ldb = ldw, P.rows = m, P.cols = k, P.k = ld, P.o[0] = (T *)dx, P.ldo = lddx;
-      if (ld != n || !in_place(w_gate, ldw, k, e, true) || !in_place(w_up, ldw, k, e, true))
-        pack(s, n, k, P.b[0], ldw, ws, ld), pack(s, n, k, P.b[1], ldw, ws, ld), P.ldb = padded(k, e);
-      gemm<T, DX>(s, tile_of(e, m, k, 1, true), P);
+      X.splits = px.splits, X.steps = px.steps, X.part = px.splits > 1 ? part : nullptr;
+      gemm<T, DX>(s, px.tile, X);
+      if (X.part) join(s, part, m, k, 1, px.splits, (T *)dx, (T *)dx, lddx);
     }
     if (dw_gate) {
-      GemmArgs<T> P{};
-      Tile tile;
-      plan_dw(e, m, k, n, tile, P.splits, P.steps);
-      P.a[0] = dg, P.a[1] = du, P.b[0] = (const T *)x, P.lda = ld, P.ldb = ldx, P.rows = n, P.cols = k, P.k = m;
-      P.o[0] = (T *)dw_gate, P.o[1] = (T *)dw_up, P.ldo = k;
-      if (m && !in_place(x, ldx, k, e, true)) pack(s, m, k, P.b[0], ldx, ws, m), P.ldb = padded(k, e);
-      if (P.splits > 1) P.part = (float *)ws;
-      gemm<T, DW>(s, tile, P);
-      if (P.splits > 1)
-        k_join<T><<<blocks(2 * n * k), 256, 0, s>>>(P.part, n * k, P.splits, (T *)dw_gate, (T *)dw_up);
+      W.splits = pw.splits, W.steps = pw.steps, W.part = pw.splits > 1 ? part : nullptr;
+      gemm<T, DW>(s, pw.tile, W);
+      if (W.part) join(s, part, n, k, 2, pw.splits, (T *)dw_gate, (T *)dw_up, k);
     }
   });
   return qr_dense_launched("gated ffn backward");

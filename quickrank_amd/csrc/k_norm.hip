@@ -9,6 +9,7 @@
 // variance is taken from the mean, not from the squares.  The backward pass reads a row of dy and of x once for
 // dx and for the two column sums: a lane owns the same columns of every row its workgroup takes, adds them up in
 // registers, and the workgroups' sums are joined by a second launch in a fixed order.
+#include <algorithm>
 #include <type_traits>
 
 #include "qr_dense.h"
@@ -401,6 +402,8 @@ size_t parts_of(size_t rows, int lanes, int pieces) {
   return rows < most ? rows : most;
 }
 
+constexpr size_t COLS_MOST = (size_t)1 << 24;
+
 }  // namespace
 
 extern "C" int qr_layer_norm_async(int device, void *stream, int type, int param_type, size_t rows, size_t cols, const void *x,
@@ -409,6 +412,7 @@ extern "C" int qr_layer_norm_async(int device, void *stream, int type, int param
   QR_DENSE_ARG(qr_dense_type_ok(type), "layer norm: unknown element type");
   QR_DENSE_ARG(param_type == type || param_type == QR_F32, "layer norm: weight and bias have the rows' type or f32");
   QR_DENSE_ARG(cols > 0, "layer norm: rows of no columns");
+  if (cols > COLS_MOST) return qr_dense_fail(QR_ERR_UNSUPPORTED, "layer norm: rows of more than 2^24 columns");
   QR_DENSE_ARG(eps >= 0.f && eps < INFINITY, "layer norm: eps is a finite number of at least 0");
   QR_DENSE_ARG(qr_dense_fits(rows, cols, ldx) && qr_dense_fits(rows, cols, ldy), "layer norm: sizes out of range");
   QR_DENSE_ARG(rows < 2 || ldy >= cols, "layer norm: the stride of y is shorter than a row");
@@ -421,9 +425,13 @@ extern "C" int qr_layer_norm_async(int device, void *stream, int type, int param
     auto go = [&](auto p) {
       using P = decltype(p);
       const bool fits = by_row<false>(cols, sizeof(T), [&](auto G, auto N) {
-        constexpr size_t RPB = 256 / G();
-        k_norm<T, P, G(), N()><<<(unsigned)((rows + RPB - 1) / RPB), 256, 0, s>>>(rows, (int)cols, (const T *)x, ldx, (const P *)weight,
-                                                                                 (const P *)bias, eps, (T *)y, ldy, mean, rstd);
+        constexpr size_t RPB = 256 / G(), MOST = RPB << 23;  // (a launch has fewer than 2^32 threads)
+        for (size_t r = 0; r < rows; r += MOST) {
+          const size_t n = std::min(rows - r, MOST);
+          k_norm<T, P, G(), N()><<<(unsigned)((n + RPB - 1) / RPB), 256, 0, s>>>(
+              n, (int)cols, (const T *)x + r * ldx, ldx, (const P *)weight, (const P *)bias, eps, (T *)y + r * ldy, ldy,
+              mean ? mean + r : nullptr, rstd ? rstd + r : nullptr);
+        }
       });
       if (!fits)
         k_norm_any<T, P><<<(unsigned)(rows < 65536 ? rows : 65536), 256, 0, s>>>(rows, (int)cols, (const T *)x, ldx, (const P *)weight,
@@ -436,7 +444,7 @@ extern "C" int qr_layer_norm_async(int device, void *stream, int type, int param
 }
 
 extern "C" int qr_layer_norm_backward_workspace(size_t rows, size_t cols, size_t *bytes) {
-  QR_DENSE_ARG(bytes && cols > 0 && cols < ((size_t)1 << 31), "layer norm backward: bad size");
+  QR_DENSE_ARG(bytes && cols > 0 && cols <= COLS_MOST, "layer norm backward: bad size");
   *bytes = parts_of(rows, 1, 1) * 2 * cols * 4;
   return QR_OK;
 }
@@ -448,6 +456,7 @@ extern "C" int qr_layer_norm_backward_async(int device, void *stream, int type, 
   QR_DENSE_ARG(qr_dense_type_ok(type), "layer norm backward: unknown element type");
   QR_DENSE_ARG(param_type == type || param_type == QR_F32, "layer norm backward: weight and bias have the rows' type or f32");
   QR_DENSE_ARG(cols > 0, "layer norm backward: rows of no columns");
+  if (cols > COLS_MOST) return qr_dense_fail(QR_ERR_UNSUPPORTED, "layer norm backward: rows of more than 2^24 columns");
   QR_DENSE_ARG(qr_dense_fits(rows, cols, ldx) && qr_dense_fits(rows, cols, lddy) && qr_dense_fits(rows, cols, lddx),
                "layer norm backward: sizes out of range");
   QR_DENSE_ARG(!dx || rows < 2 || lddx >= cols, "layer norm backward: the stride of dx is shorter than a row");

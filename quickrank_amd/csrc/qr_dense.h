@@ -62,10 +62,12 @@ inline bool qr_dense_overlap(const void *p, size_t np, const void *q, size_t nq)
   return p && q && np && nq && a < b + nq && b < a + np;
 }
 // rows * cols elements of stride ld stay far below 2^63 bytes
-inline bool qr_dense_fits(size_t rows, size_t cols, size_t ld) {
+inline bool qr_dense_spans(size_t rows, size_t cols, size_t ld) {
   const size_t most = (size_t)1 << 58;
-  return cols < ((size_t)1 << 31) && (rows == 0 || (ld < most && cols < most && rows < most / ((ld > cols ? ld : cols) + 1)));
+  return rows == 0 || (ld < most && cols < most && rows < most / ((ld > cols ? ld : cols) + 1));
 }
+// ... and a row's elements below 2^31
+inline bool qr_dense_fits(size_t rows, size_t cols, size_t ld) { return cols < ((size_t)1 << 31) && qr_dense_spans(rows, cols, ld); }
 
 // `T` of a type code for a generic lambda: qr_dense_dispatch(type, [&](auto t) { using T = decltype(t); ... })
 template <class F>

@@ -641,3 +641,92 @@ def test_refusals_on_the_gpu(dense):
     x.requires_grad_(True)
     with torch.no_grad():
         dense.layer_norm(x, w)
+
+
+# ---- offsets beyond 32 bits ------------------------------------------------------------------------
+
+def test_dropout_beyond_2_32_elements(dense):
+    """The tail of 2^32 + 4099 elements equals a call of its own at its word's offset."""
+    n = (1 << 32) + 4099
+    x = torch.ones(n, dtype=torch.bfloat16, device="cuda")
+    y = dense.dropout(x, 0.3, 17, 5)
+    start = (1 << 32) - 8
+    tail = dense.dropout(x[start:].contiguous(), 0.3, 17, 5 + start // 4)
+    assert torch.equal(y[start:], tail) and torch.equal(y[:64], dense.dropout(x[:64], 0.3, 17, 5))
+    wide = y.view(1, n)
+    assert torch.equal(dense.dropout(x.view(1, n), 0.3, 17, 5)[0, start:], tail) and wide.shape == (1, n)
+
+
+def test_norm_beyond_2_32_elements(dense):
+    """Rows at the end of 2^32 + 2^20 elements, forward and backward."""
+    cols = 2048
+    rows = (1 << 21) + 512
+    x = torch.zeros((rows, cols), dtype=torch.bfloat16, device="cuda")
+    x[-3:] = rand(1, 3, cols, dtype=torch.bfloat16)
+    w, b = rand(2, cols), rand(3, cols)
+    y, mean, rstd = dense.layer_norm(x, w, b)
+    want = dense.layer_norm(x[-3:].clone(), w, b)
+    assert torch.equal(y[-3:], want[0]) and torch.equal(mean[-3:], want[1]) and torch.equal(rstd[-3:], want[2])
+    dy = y.zero_()
+    dy[-3:] = rand(4, 3, cols, dtype=torch.bfloat16)
+    got = dense.layer_norm_backward(dy, x, w, mean, rstd)
+    ref = dense.layer_norm_backward(dy[-3:].clone(), x[-3:].clone(), w, mean[-3:].clone(), rstd[-3:].clone())
+    assert torch.equal(got[0][-3:], ref[0])
+    for p, q in zip(got[1:], ref[1:]):
+        # (three addends a column, in another order: two additions and a product, each half a step of f32)
+        size = dy[-3:].double().abs().max() * 8 * 3
+        assert (p.double() - q.double()).abs().max() <= 8 * U32 * size
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_rows_far_apart(dense, dtype):
+    """Rows 2^24 elements apart: offsets beyond 2^31 elements, strides longer than the product kernel's tiles reach."""
+    m, k, n, far = 200, 72, 136, 1 << 24
+    x, wg, wu = ffn_inputs(1, m, k, n, dtype)
+    buf = torch.full(((m - 1) * far + k,), float("nan"), dtype=dtype, device="cuda")
+    v = buf.as_strided((m, k), (far, 1))
+    v.copy_(x)
+    w = rand(4, k)
+    assert all(torch.equal(p, q) for p, q in zip(dense.layer_norm(v, w), dense.layer_norm(x, w)))
+    assert torch.equal(dense.dropout(v, 0.4, 3), dense.dropout(x, 0.4, 3))
+    h = dense.gated_ffn(x, wg, wu, save=True)
+    assert all(torch.equal(p, q) for p, q in zip(dense.gated_ffn(v, wg, wu, save=True), h))
+    want = dense.gated_ffn_backward(h[0], x, wg, wu, *h[1:])
+    assert all(torch.equal(p, q) for p, q in zip(dense.gated_ffn_backward(h[0], v, wg, wu, *h[1:]), want))
+    many = rand(5, 4000, k, dtype=dtype)  # (the tiled kernels)
+    far_w = buf.as_strided((n, k), (far, 1))
+    far_w.copy_(wg)
+    far_u = torch.empty_like(buf).as_strided((n, k), (far, 1))
+    far_u.copy_(wu)
+    h = dense.gated_ffn(many, wg, wu, save=True)
+    assert all(torch.equal(p, q) for p, q in zip(dense.gated_ffn(many, far_w, far_u, save=True), h))
+    want = dense.gated_ffn_backward(h[0], many, wg, wu, *h[1:])
+    assert all(torch.equal(p, q) for p, q in zip(dense.gated_ffn_backward(h[0], many, far_w, far_u, *h[1:]), want))
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_ffn_broadcast_inputs(dense, dtype):
+    """One row for all rows of x, of dh, of the weights: strides of 0."""
+    x, wg, wu = ffn_inputs(1, 1, 72, 130, dtype)
+    many = x.expand(700, 72)
+    a, b = dense.gated_ffn(many, wg, wu, save=True), dense.gated_ffn(many.contiguous(), wg, wu, save=True)
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    dh = rand(2, 1, 130, dtype=dtype).expand(700, 130)
+    a = dense.gated_ffn_backward(dh, many, wg, wu, *b[1:])
+    b = dense.gated_ffn_backward(dh.contiguous(), many.contiguous(), wg, wu, *b[1:])
+    assert all(torch.equal(p, q) for p, q in zip(a, b))
+    one = wg[:1].expand(130, 72)
+    assert torch.equal(dense.gated_ffn(many, one, one), dense.gated_ffn(many.contiguous(), one.contiguous(), one.contiguous()))
+
+
+def test_f32_products_keep_24_bits(dense):
+    """Numbers whose low mantissa bits decide: (1 + 2^-23) (1 - 2^-23) summed against -1, in units that f32 holds."""
+    m, k, n = 130, 64, 130
+    x, w = torch.zeros(m, k, device="cuda"), torch.zeros(n, k, device="cuda")
+    x[:, 0], w[:, 0] = 1 + 2.0 ** -23, 1.0
+    x[:, 1], w[:, 1] = -1.0, 1.0
+    x[:, 2], w[:, 2] = 2.0 ** -40, 3.0
+    _, g, u = dense.gated_ffn(x, w, w, "relu", save=True)
+    want = torch.full_like(g, 2.0 ** -23 + 3 * 2.0 ** -40)
+    # the first two cancel exactly; what the split leaves out is below 2^-21 of the largest product
+    assert (g - want).abs().max() <= 2.0 ** -40 and torch.equal(g, u)
