@@ -163,11 +163,13 @@ __global__ __launch_bounds__(256) void k_norm(const size_t rows, const int cols,
   }
 }
 
-// part: [workgroup][2][cols] column sums of the rows a workgroup took, or NULL
+// part: [workgroup][2][cols] column sums of the rows a workgroup took, or NULL; of a single workgroup they go straight to
+// dw and db
 template <class T, class P, int G, int N>
 __global__ __launch_bounds__(G > 256 ? G : 256) void k_norm_grad(const size_t rows, const int cols, const T *dy, const size_t lddy, const T *x,
                                                    const size_t ldx, const P *__restrict__ w, const float *__restrict__ mean,
-                                                   const float *__restrict__ rstd, T *dx, const size_t lddx, float *__restrict__ part) {
+                                                   const float *__restrict__ rstd, T *dx, const size_t lddx, float *__restrict__ part,
+                                                   P *__restrict__ dw, P *__restrict__ db) {
   constexpr int V = Pieces<T, G>::V, RPB = G > 256 ? 1 : 256 / G;
   __shared__ float lds[32];
   const Pieces<T, G> S(cols);
@@ -235,6 +237,16 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void k_norm_grad(const size_t ro
     }
   }
   if (!part) return;
+  const bool direct = gridDim.x == 1;
+  auto keep = [&](const int j, const float vw, const float vb) {
+    if (direct) {
+      if (dw) dw[j] = (P)vw;
+      if (db) db[j] = (P)vb;
+    } else {
+      part[(size_t)blockIdx.x * 2 * cols + j] = vw;
+      part[((size_t)blockIdx.x * 2 + 1) * cols + j] = vb;
+    }
+  };
   // the groups of the workgroup one after the other (each column has one owner in a group)
   extern __shared__ float sum[];
   for (int g = 0; g < RPB; ++g) {
@@ -242,13 +254,12 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void k_norm_grad(const size_t ro
 #pragma unroll
       for (int i = 0; i < N; ++i) {
         if (!S.inner(i) && !S.any(i, l)) continue;
-        const int at = S.at(i, l), dup = S.inner(i) ? 0 : S.dup(i, l);
+        const int at = S.at(i, l), dup = S.dup(i, l);
 #pragma unroll
         for (int e = 0; e < V; ++e)
           if (e >= dup) {
             if (RPB == 1) {
-              part[(size_t)blockIdx.x * 2 * cols + at + e] = sw[i][e];
-              part[((size_t)blockIdx.x * 2 + 1) * cols + at + e] = sb[i][e];
+              keep(at + e, sw[i][e], sb[i][e]);
             } else {
               sum[at + e] = (g ? sum[at + e] : 0.f) + sw[i][e];
               sum[cols + at + e] = (g ? sum[cols + at + e] : 0.f) + sb[i][e];
@@ -259,7 +270,7 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void k_norm_grad(const size_t ro
     if (RPB > 1) __syncthreads();
   }
   if (RPB > 1)
-    for (int j = threadIdx.x; j < 2 * cols; j += 256) part[(size_t)blockIdx.x * 2 * cols + j] = sum[j];
+    for (int j = threadIdx.x; j < cols; j += 256) keep(j, sum[j], sum[cols + j]);
 }
 
 // 16 columns by 64 shares of the partial sums
@@ -401,6 +412,9 @@ size_t parts_of(size_t rows, int lanes, int pieces) {
   const size_t most = lanes > 256 ? 512 : pieces > 1 ? 1024 : 1536;
   return rows < most ? rows : most;
 }
+// Up to this many rows a workgroup takes at a time, one workgroup takes them all and no join follows: a second launch
+// costs more than the rows one after the other.
+constexpr size_t ALONE = 4;
 
 constexpr size_t COLS_MOST = (size_t)1 << 24;
 
@@ -477,10 +491,10 @@ extern "C" int qr_layer_norm_backward_async(int device, void *stream, int type, 
       const bool fits = !rows || by_row<true>(cols, sizeof(T), [&](auto G, auto N) {
         constexpr size_t RPB = G() > 256 ? 1 : 256 / G();
         const size_t want = (rows + RPB - 1) / RPB, parts = parts_of(rows, G(), N());
-        const unsigned grid = (unsigned)(want < parts ? want : parts);
+        const unsigned grid = want <= ALONE ? 1 : (unsigned)(want < parts ? want : parts);
         k_norm_grad<T, P, G(), N()><<<grid, G() > 256 ? G() : 256, RPB > 1 && sums ? 2 * cols * 4 : 0, s>>>(
-            rows, (int)cols, (const T *)dy, lddy, (const T *)x, ldx, (const P *)weight, mean, rstd, (T *)dx, lddx, part);
-        if (sums) k_norm_join<P><<<(unsigned)((2 * cols + 15) / 16), 1024, 0, s>>>((int)cols, (int)grid, part, (P *)dweight, (P *)dbias);
+            rows, (int)cols, (const T *)dy, lddy, (const T *)x, ldx, (const P *)weight, mean, rstd, (T *)dx, lddx, part, (P *)dweight, (P *)dbias);
+        if (sums && grid > 1) k_norm_join<P><<<(unsigned)((2 * cols + 15) / 16), 1024, 0, s>>>((int)cols, (int)grid, part, (P *)dweight, (P *)dbias);
       });
       if (fits && rows) return;
       // (the column sums first: dx may be written over dy or x)
