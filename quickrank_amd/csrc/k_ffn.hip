@@ -248,18 +248,25 @@ __device__ __forceinline__ void wait_all() { asm volatile("s_waitcnt vmcnt(0) lg
 __device__ __forceinline__ void barrier() { asm volatile("s_barrier" ::: "memory"); }
 __device__ __forceinline__ uint32_t lds_offset(const char *p) { return (uint32_t)(uintptr_t)(QR_LDS const char *)p; }
 
-// TM x TN sums (FWD: TM x TN / 2 of each product) by 2 x 2 waves.  While the matrix cores work on one stage the next is
-// on its way: the first operand's to the other half of its LDS buffer without passing registers, the second's in
-// registers, from where it is written to its single buffer behind a barrier.  (Both double-buffered, two workgroups of the
-// largest tile would not fit a compute unit, 160 KB; they do, and one's matrix instructions run under the other's waits,
-// first loads and epilogue.)  The last, partial stage of a sum is zero-filled.
-template <class T, Kind KIND, int TM, int TN>
-__global__ __launch_bounds__(256, 2) void k_gemm(const GemmArgs<T> P) {
-  constexpr bool AKS = KIND == DW, BKS = KIND != FWD;
-  constexpr int WM = 2, WN = 2, NT = 256, KT = 128 / sizeof(T), E = 16 / sizeof(T);
+// TM x TN sums (FWD: TM x TN / 2 of each product) by 2 x WN waves.  While the matrix cores work on one stage the next is
+// on its way.  WN = 2: the first operand's to the other half of its LDS buffer without passing registers, the second's in
+// registers, from where it is written to its single buffer behind a barrier.  (Both double-buffered, two workgroups of 256
+// x 128 would not fit a compute unit, 160 KB; they do, and one's matrix instructions run under the other's waits, first
+// loads and epilogue.)  WN = 4, 256 x 256: one workgroup fills the compute unit; both operands are double-buffered and
+// pass no registers, and the next stage is sent for in the first half of this one.  The last, partial stage of a sum is
+// zero-filled.
+//
+// What bounds it, 16-bit types: at 256 x 128 the way from L2 to the compute units (48 bytes a cycle and unit at the full
+// matrix rate, of 64), at 256 x 256 (32 bytes) the matrix cores at the clock that the card holds under them.  1490 TF at
+// 8192 x 8192 x (2 x 4096), where a large library product reaches 1320; 1170 TF at 32768 x 1024 x (2 x 4096), whose 16
+// stages leave a quarter of a tile's time to its first loads and its results.  f32: the six products per stage, 203 TF.
+template <class T, Kind KIND, int TM, int TN, int WN>
+__global__ __launch_bounds__(128 * WN, 2) void k_gemm(const GemmArgs<T> P) {
+  constexpr bool AKS = KIND == DW, BKS = KIND != FWD, BD = WN > 2;
+  constexpr int WM = 2, NT = 128 * WN, KT = 128 / sizeof(T), E = 16 / sizeof(T);
   constexpr int MI = TM / WM / 16, NI = TN / WN / 16, PA = TM * 8 / NT, PB = TN * 8 / NT;
   constexpr int COLS = KIND == FWD ? TN / 2 : TN;
-  constexpr uint32_t ABUF = TM * 128, LDS_BYTES = 2 * ABUF + TN * 128;
+  constexpr uint32_t ABUF = TM * 128, BBUF = BD ? TN * 128 : 0, LDS_BYTES = 2 * ABUF + TN * 128 + BBUF;
   __shared__ __align__(1024) char lds[LDS_BYTES];
 
   // consecutive workgroups go to the eight XCDs in turn: each XCD gets a run of tiles, and a run covers bands of
@@ -318,7 +325,7 @@ __global__ __launch_bounds__(256, 2) void k_gemm(const GemmArgs<T> P) {
   const unsigned second = KIND == DX && first >= kt_all ? 1 : 0;
   const size_t k0 = (size_t)(first - (second ? kt_all : 0)) * KT;
   const char *sa = (const char *)(P.a[KIND == DW ? z : second] + (AKS ? k0 * P.lda + r0 : r0 * P.lda + k0));
-  const char *sb = (const char *)(P.b[KIND == FWD ? wave >> 1 : second] + (BKS ? k0 * P.ldb + c0 : c0 * P.ldb + k0));
+  const char *sb = (const char *)(P.b[KIND == FWD ? (wave >> 1) & 1 : second] + (BKS ? k0 * P.ldb + c0 : c0 * P.ldb + k0));
   // stages are loaded in order
   auto next_a = [&](const unsigned t) {
     sa += (AKS ? KT * P.lda : (size_t)KT) * sizeof(T);
@@ -329,6 +336,7 @@ __global__ __launch_bounds__(256, 2) void k_gemm(const GemmArgs<T> P) {
     if (KIND == DX && t + 1 == kt_all) sb = (const char *)(P.b[1] + c0);
   };
   auto load_a = [&](const int d, const uint32_t to) { dma16(sa, offa[d], to + (d * NT + wave * 64) * 16); };
+  auto dma_b = [&](const int d, const uint32_t to) { dma16(sb, offb[d], to + (d * NT + wave * 64) * 16); };
   // the partial stage's
   auto fill_a = [&](const unsigned t, char *to) {
 #pragma unroll 1
@@ -337,6 +345,19 @@ __global__ __launch_bounds__(256, 2) void k_gemm(const GemmArgs<T> P) {
       piece_of<T, TM, AKS>(q, r, k);
       const size_t kk = (size_t)t * KT + k;
       *(i4 *)(to + q * 16) = AKS ? fetch16(a0, P.lda, kk, P.k, r0 + r, P.rows) : fetch16(a0, P.lda, r0 + r, P.rows, kk, P.k);
+    }
+  };
+  auto fill_b = [&](const unsigned t, char *to) {
+#pragma unroll 1
+    for (int q = tid; q < TN * 8; q += NT) {
+      int r, k;
+      size_t row;
+      bool up;
+      piece_of<T, TN, BKS>(q, r, k);
+      b_row(r, row, up);
+      const size_t kk = (size_t)t * KT + k;
+      const T *p = P.b[up ? 1 : 0];
+      *(i4 *)(to + q * 16) = BKS ? fetch16(p, P.ldb, kk, P.k, row, P.cols) : fetch16(p, P.ldb, row, P.cols, kk, P.k);
     }
   };
   i4 vb[PB];
@@ -373,12 +394,12 @@ __global__ __launch_bounds__(256, 2) void k_gemm(const GemmArgs<T> P) {
   const uint32_t base_a = frag_base<T, TM, AKS>(lds_offset(lds), wm * MI);
   const uint32_t base_b = frag_base<T, TN, BKS>(lds_offset(lds) + 2 * ABUF, wn * NI);
   auto read_a = [&](const uint32_t ra, const int m, const int half) { return frag<T, TM, AKS>(ra, wm * MI, m, half); };
-  auto read_b = [&](const int n, const int half) { return frag<T, TN, BKS>(base_b, wn * NI, n, half); };
   // 16-bit types: a stage's 2 x MI rows of blocks, the first operand's fragments read D ahead of their use.
   // f32: its MI rows of blocks, split into three parts, one ahead.  In the steady state the next stage's loads are spread
   // over the rows.
-  auto compute = [&](auto steady, const uint32_t ra, const uint32_t to) {
+  auto compute = [&](auto steady, const uint32_t ra, const uint32_t rb, const uint32_t to, const uint32_t to_b) {
     constexpr bool STEADY = decltype(steady)::value;
+    auto read_b = [&](const int n, const int half) { return frag<T, TN, BKS>(rb, wn * NI, n, half); };
     if constexpr (sizeof(T) == 4) {
       Split fb[NI];
       i4 next[2] = {read_a(ra, 0, 0), read_a(ra, 0, 1)};
@@ -400,7 +421,7 @@ __global__ __launch_bounds__(256, 2) void k_gemm(const GemmArgs<T> P) {
         __builtin_amdgcn_sched_barrier(0);
       }
     } else {
-      constexpr int D = MI > 3 ? 3 : MI - 1;
+      constexpr int D = MI > 3 ? 3 : MI - 1, ROWS = BD ? MI : 2 * MI;  // rows over which the loads are spread
       i4 fa[D + 1], fb[2][NI];
 #pragma unroll
       for (int n = 0; n < NI; ++n) fb[0][n] = read_b(n, 0);
@@ -414,52 +435,69 @@ __global__ __launch_bounds__(256, 2) void k_gemm(const GemmArgs<T> P) {
           for (int n = q * NI / MI; n < (q + 1) * NI / MI; ++n) fb[1][n] = read_b(n, 1);
         if constexpr (STEADY)
 #pragma unroll
-          for (int d = q * PA / MI / 2; d < (q + 1) * PA / MI / 2; ++d) load_a(d, to);
+          for (int d = q * PA / ROWS; d < (q + 1) * PA / ROWS && d < PA; ++d) load_a(d, to);
+        if constexpr (STEADY && BD)
+#pragma unroll
+          for (int d = q * PB / ROWS; d < (q + 1) * PB / ROWS && d < PB; ++d) dma_b(d, to_b);
 #pragma unroll
         for (int n = 0; n < NI; ++n) acc[q % MI][n] = mma<T>(fb[q / MI][n], fa[q % (D + 1)], acc[q % MI][n]);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
   };
+  const uint32_t at_a = lds_offset(lds), at_b = at_a + 2 * ABUF;
   if (first < last) {
     if (KIND == DX || first < whole) {
 #pragma unroll
-      for (int d = 0; d < PA; ++d) load_a(d, lds_offset(lds));
+      for (int d = 0; d < PA; ++d) load_a(d, at_a);
       next_a(first);
     } else {
       fill_a(first, lds);
     }
-    load_b(first);
-    keep_b();
-    uint32_t cur = 0;
-    unsigned t = first;
-    for (; t + 1 < whole; ++t, cur ^= ABUF) {
-      wait_all();
-      barrier();  // stage t is there, and every wave is done with the first operand's stage t - 1
-      load_b(t + 1);
-      compute(std::true_type{}, base_a + cur, lds_offset(lds) + (cur ^ ABUF));
-      next_a(t + 1);
-      barrier();  // every wave is done with the second operand's stage t
+    if (!BD) {
+      load_b(first);
       keep_b();
+    } else if (KIND == DX || first < whole) {
+#pragma unroll
+      for (int d = 0; d < PB; ++d) dma_b(d, at_b);
+      next_b(first);
+    } else {
+      fill_b(first, lds + 2 * ABUF);
     }
-    for (; t < last; ++t, cur ^= ABUF) {
+    uint32_t cur = 0, cur_b = 0;
+    unsigned t = first;
+    for (; t + 1 < whole; ++t, cur ^= ABUF, cur_b ^= BBUF) {
+      wait_all();
+      barrier();  // stage t is there, and every wave is done with stage t - 1 where there are two buffers
+      if (!BD) load_b(t + 1);
+      compute(std::true_type{}, base_a + cur, base_b + cur_b, at_a + (cur ^ ABUF), at_b + (cur_b ^ BBUF));
+      next_a(t + 1);
+      if (BD) {
+        next_b(t + 1);
+      } else {
+        barrier();  // every wave is done with the second operand's stage t
+        keep_b();
+      }
+    }
+    for (; t < last; ++t, cur ^= ABUF, cur_b ^= BBUF) {
       wait_all();
       barrier();
       if (t + 1 < last) {
         fill_a(t + 1, lds + (cur ^ ABUF));
-        load_b(t + 1);
+        if (BD) fill_b(t + 1, lds + 2 * ABUF + (cur_b ^ BBUF));
+        else load_b(t + 1);
       }
-      compute(std::false_type{}, base_a + cur, 0);
-      barrier();
-      if (t + 1 < last) keep_b();
+      compute(std::false_type{}, base_a + cur, base_b + cur_b, 0, 0);
+      if (!BD || t + 1 == last) barrier();
+      if (!BD && t + 1 < last) keep_b();
     }
   }
 
   // Results pass through the wave's own share of the LDS, so that a lane ends with eight neighbours of a row: one
   // wide store, and one copy of the activation's code.  Pieces of four are moved by the row against bank conflicts.
-  constexpr int WTN = NI * 16, PIECES = WTN / 4, SHARE = LDS_BYTES / 4 / (16 * WTN * 4) * (16 * WTN * 4);
+  constexpr int WTN = NI * 16, PIECES = WTN / 4, SHARE = LDS_BYTES / (WM * WN) / (16 * WTN * 4) * (16 * WTN * 4);
   constexpr int FIT = SHARE / (16 * WTN * 4), MB = FIT >= MI ? MI : FIT >= MI / 2 ? MI / 2 : MI / 4;  // blocks of 16 rows at a time
-  static_assert(MB > 0 && MB <= FIT && MI % MB == 0 && PA % MI == 0, "blocks fit the waves' shares");
+  static_assert(MB > 0 && MB <= FIT && MI % MB == 0 && (BD || PA % MI == 0), "blocks fit the waves' shares");
   char *const own = lds + wave * SHARE;
   auto at = [&](const int row, const int piece) -> f4 * {
     const int r = row & 15, c = (PIECES & (PIECES - 1)) == 0 ? piece ^ (r & (PIECES - 1)) : (piece + r) % PIECES;
@@ -719,12 +757,12 @@ void launch_pack(hipStream_t s, const Packs<T> &packs) {
   if (packs.n && most) k_pack<T><<<dim3(blocks(most), packs.n), 256, 0, s>>>(packs);
 }
 
-template <class T, Kind KIND, int TM, int TN>
+template <class T, Kind KIND, int TM, int TN, int WN = 2>
 void launch_gemm(hipStream_t s, GemmArgs<T> P) {
   P.row_tiles = tiles_of(P.rows, TM);
   P.col_tiles = tiles_of(P.cols, KIND == FWD ? TN / 2 : TN);
   const unsigned tiles = P.row_tiles * P.col_tiles * (KIND == FWD ? 1 : (KIND == DW ? 2 : 1) * P.splits);
-  k_gemm<T, KIND, TM, TN><<<(tiles + 7) / 8 * 8, 256, 0, s>>>(P);
+  k_gemm<T, KIND, TM, TN, WN><<<(tiles + 7) / 8 * 8, 128 * WN, 0, s>>>(P);
 }
 
 
@@ -770,7 +808,7 @@ Tile tile_of(size_t e, size_t rows, size_t cols, size_t times, bool narrow) {
 template <class T, Kind KIND>
 void gemm(hipStream_t s, const Tile t, const GemmArgs<T> &P) {
   if constexpr (sizeof(T) == 2)
-    if (t.rows == 256) return launch_gemm<T, KIND, 256, 128>(s, P);
+    if (t.rows == 256) return t.cols == 256 ? launch_gemm<T, KIND, 256, 256, 4>(s, P) : launch_gemm<T, KIND, 256, 128>(s, P);
   if (t.rows == 128 && t.cols == 128) return launch_gemm<T, KIND, 128, 128>(s, P);
   if constexpr (KIND != FWD) {
     if (t.rows == 128 && t.cols == 64) return launch_gemm<T, KIND, 128, 64>(s, P);
@@ -782,6 +820,32 @@ void gemm(hipStream_t s, const Tile t, const GemmArgs<T> &P) {
   launch_gemm<T, KIND, 64, 64>(s, P);
 }
 
+// 256 x 256 sums a workgroup instead of 256 x 128, one workgroup a compute unit instead of two: a third less to load for
+// each product, but a tile's first loads and its results' way out have nothing beside them.  In hundredths of a stage's
+// time (1.39 us with every compute unit at work), fitted to times measured between 2 and 64 stages: a full round of the
+// large tiles takes 100 a stage and `edge`, one of the small 118 a stage and `edge` less 110 (290 where three matrices are
+// stored); a part of a round takes 3 / 4 of one, a small tile alone on its compute unit 1 / 2.  `large`, `small`: the
+// launches' workgroups and stages.  Measured: 8192 x 8192 x (2 x 4096) 740 us against 845, 32768 x 1024 x (2 x 4096) 459
+// against 490 (with g and u stored 528 against 545), their gradients for half the rows 564 against 604; but 8192 x 4096 x
+// (2 x 1152), 288 large tiles, 176 against 161.
+struct Launch {
+  size_t groups, stages;
+};
+bool larger(const Launch large, const Launch small, const bool saves) {
+  const size_t rounds = large.groups / CUS, rest = small.groups % (2 * CUS);
+  const size_t edge = saves ? (rounds < 8 ? 890 : 780) : 530;  // (over many rounds the workgroups' stores come apart)
+  const size_t of_large = rounds * 4 + (large.groups % CUS ? 3 : 0);
+  const size_t of_small = small.groups / (2 * CUS) * 4 + (rest ? rest > CUS ? 4 : 2 : 0);
+  return of_large * (large.stages * 100 + edge) < of_small * (small.stages * 118 + edge - (saves ? rounds < 8 ? 290 : 230 : 110));
+}
+
+Tile tile_forward(size_t e, size_t m, size_t k, size_t n, bool saves) {
+  const Tile t = tile_of(e, m, 2 * n, 1, false);
+  const size_t rows = tiles_of(m, 256), stages = (k * e + 127) / 128;
+  if (t.rows < 256 || !larger({rows * tiles_of(2 * n, 256), stages}, {rows * tiles_of(2 * n, 128), stages}, saves)) return t;
+  return {256, 256};
+}
+
 // How the gradients' products are made: `outs` matrices of rows x cols, sums of `stages` stages.  With few outputs the
 // sums are split so that the launch gives every compute unit two workgroups (not one more: a third makes it work half as
 // long again), in shares of at least eight stages.
@@ -791,13 +855,15 @@ struct Plan {
 };
 Plan plan(size_t e, size_t rows, size_t cols, size_t outs, size_t stages) {
   const size_t most = std::max<size_t>(stages / 8, 1);
-  Plan p;
-  p.tile = tile_of(e, rows, cols, outs * most, true);
-  const size_t one = std::max<size_t>(outs * tiles_of(rows, p.tile.rows) * tiles_of(cols, p.tile.cols), 1);  // (no rows)
-  const size_t want = std::min(std::max<size_t>(2 * CUS / one, 1), most);
-  p.steps = (unsigned)std::max<size_t>((stages + want - 1) / want, 1);
-  p.splits = (unsigned)std::max<size_t>((stages + p.steps - 1) / p.steps, 1);
-  return p;
+  auto with = [&](const Tile t, const size_t groups) {
+    const size_t one = std::max<size_t>(outs * tiles_of(rows, t.rows) * tiles_of(cols, t.cols), 1);  // (no rows)
+    const size_t want = std::min(std::max<size_t>(groups / one, 1), most);
+    Plan p{t, 1, (unsigned)std::max<size_t>((stages + want - 1) / want, 1)};
+    p.splits = (unsigned)std::max<size_t>((stages + p.steps - 1) / p.steps, 1);
+    return std::pair<Plan, Launch>(p, {one * p.splits, p.steps});
+  };
+  const auto small = with(tile_of(e, rows, cols, outs * most, true), 2 * CUS), large = with({256, 256}, CUS);
+  return small.first.tile.rows == 256 && larger(large.second, small.second, false) ? large.first : small.first;
 }
 Plan plan_dx(size_t e, size_t m, size_t k, size_t n) { return plan(e, m, k, 1, 2 * stages_of(n, e) * e / 128); }
 Plan plan_dw(size_t e, size_t m, size_t k, size_t n) { return plan(e, n, k, 2, (m * e + 127) / 128); }
@@ -860,7 +926,7 @@ extern "C" int qr_gated_ffn_async(int device, void *stream, int type, int act, s
     }
     launch_pack(s, packs);
     if (few(m, n)) launch_few(s, P);
-    else gemm<T, FWD>(s, tile_of(e, m, 2 * n, 1, false), P);
+    else gemm<T, FWD>(s, tile_forward(e, m, k, n, gate != nullptr), P);
   });
   return qr_dense_launched("gated ffn");
 }

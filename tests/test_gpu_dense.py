@@ -382,6 +382,15 @@ def test_ffn_many_tiles(dense, dtype, m, k, n):
     ffn_backward_check(dense, dtype, "silu", x, wg, wu)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("m,k,n", [(4090, 2040, 2044), (2000, 2041, 4090), (8192, 512, 1024), (4001, 1000, 2009), (1030, 2016, 8190)])
+def test_ffn_large_tiles(dense, dtype, m, k, n):
+    """Sizes whose products, forward or backward, are made in tiles of 256 x 256: whole and partial tiles and stages."""
+    x, wg, wu = ffn_inputs(14, m, k, n, dtype)
+    ffn_forward_check(dense, dtype, "silu", x, wg, wu)
+    ffn_backward_check(dense, dtype, "gelu", x, wg, wu)
+
+
 def test_ffn_broken_values_stay_in_their_row_and_column(dense):
     x, wg, wu = ffn_inputs(1, 130, 72, 200, torch.bfloat16)
     ref = dense.gated_ffn(x, wg, wu)
