@@ -11,6 +11,7 @@ A tensor of rows is f32, bf16 or f16 and is read as a matrix of its last dimensi
 row stride (0 included), or contiguous with any leading dimensions.
 """
 import ctypes as C
+from operator import index
 
 import torch
 
@@ -137,10 +138,14 @@ def _dropout(x, p, seed, offset, residual, counter):
         _refuse("counter is one int64 on the device of x")
     if not 0.0 <= p <= 1.0:
         _refuse("dropout: p is a number of 0 to 1")
+    try:
+        seed, offset = index(seed) & 0xFFFFFFFFFFFFFFFF, index(offset) & 0xFFFFFFFFFFFFFFFF
+    except TypeError:
+        _refuse("dropout: seed and offset are whole numbers")
     y = x.new_empty(x.shape)
     rc = lib().qr_dropout_async(x.device.index, _stream(x), TYPES[x.dtype], rows, cols, x.data_ptr(), ld,
                                 residual.data_ptr() if residual is not None else None, ldr, y.data_ptr(), cols, p,
-                                seed & 0xFFFFFFFFFFFFFFFF, offset & 0xFFFFFFFFFFFFFFFF,
+                                seed, offset,
                                 counter.data_ptr() if counter is not None else None)
     if rc:
         _fail(rc)

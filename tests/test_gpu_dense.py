@@ -739,3 +739,14 @@ def test_f32_products_keep_24_bits(dense):
     want = torch.full_like(g, 2.0 ** -23 + 3 * 2.0 ** -40)
     # the first two cancel exactly; what the split leaves out is below 2^-21 of the largest product
     assert (g - want).abs().max() <= 2.0 ** -40 and torch.equal(g, u)
+
+
+def test_dropout_seeds_of_numpy(dense):
+    np = pytest.importorskip("numpy")
+    x = rand(70, 9, 40)
+    want = dense.dropout(x, 0.5, 7, offset=3)
+    assert torch.equal(dense.dropout(x, 0.5, np.int64(7), offset=np.int32(3)), want)
+    assert torch.equal(dense.dropout(x, 0.5, np.uint64(7), offset=np.int64(3)), want)
+    assert torch.equal(dense.dropout(x, 0.5, np.int64(-1)), dense.dropout(x, 0.5, 2 ** 64 - 1))
+    with pytest.raises(dense.QrError):
+        dense.dropout(x, 0.5, 7.0)
