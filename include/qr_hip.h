@@ -510,8 +510,9 @@ int qr_dropout_async(int device, void *hip_stream, int type, size_t rows, size_t
 /* h [m][n] = act(x w_gate^T) * (x w_up^T); x [m][k], weights [n][k] of stride ldw.        */
 /* gate / up: NULL (serving), or [m][n] contiguous: the two products, rounded to `type`,    */
 /* for the backward pass.  Outputs must not overlap each other or an input.  The workspace   */
-/* is used (NULL, 0 will do otherwise) where a row of x or of a weight does not start at a    */
-/* 16-byte boundary or lies more than 4 MB behind the one before: such matrices are copied.    */
+/* is used (NULL, 0 will do otherwise) where a row of x or of a weight does not start and end  */
+/* at 16-byte boundaries or lies more than 4 MB behind the one before: such matrices are       */
+/* copied.                                                                                    */
 int qr_gated_ffn_workspace(int type, size_t m, size_t k, size_t n, size_t *bytes);
 int qr_gated_ffn_async(int device, void *hip_stream, int type, int act, size_t m, size_t k, size_t n,
                        const void *x, size_t ldx, const void *w_gate, const void *w_up, size_t ldw, void *h,

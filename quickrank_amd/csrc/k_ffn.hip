@@ -337,49 +337,37 @@ __global__ __launch_bounds__(128 * WN, 2) void k_gemm(const GemmArgs<T> P) {
   };
   auto load_a = [&](const int d, const uint32_t to) { dma16(sa, offa[d], to + (d * NT + wave * 64) * 16); };
   auto dma_b = [&](const int d, const uint32_t to) { dma16(sb, offb[d], to + (d * NT + wave * 64) * 16); };
-  // the partial stage's
-  auto fill_a = [&](const unsigned t, char *to) {
-#pragma unroll 1
-    for (int q = tid; q < TM * 8; q += NT) {
-      int r, k;
-      piece_of<T, TM, AKS>(q, r, k);
-      const size_t kk = (size_t)t * KT + k;
-      *(i4 *)(to + q * 16) = AKS ? fetch16(a0, P.lda, kk, P.k, r0 + r, P.rows) : fetch16(a0, P.lda, r0 + r, P.rows, kk, P.k);
+  // The partial stage's: pieces inside the sum (none lies across its end) come as a whole stage's do, the others are zero
+  auto inside = [&](const auto tile, const bool columns, const unsigned t, const int d) {
+    int r, k;
+    if (columns) piece_of<T, tile(), true>(d * NT + tid, r, k);
+    else piece_of<T, tile(), false>(d * NT + tid, r, k);
+    return (size_t)t * KT + k < P.k;
+  };
+  constexpr std::integral_constant<int, TM> tile_a;
+  constexpr std::integral_constant<int, TN> tile_b;
+  auto part_a = [&](const unsigned t, const uint32_t to) {
+#pragma unroll
+    for (int d = 0; d < PA; ++d) {
+      if (inside(tile_a, AKS, t, d)) load_a(d, to);
+      else *(QR_LDS i4 *)(to + (d * NT + tid) * 16) = i4{0, 0, 0, 0};
     }
   };
-  auto fill_b = [&](const unsigned t, char *to) {
-#pragma unroll 1
-    for (int q = tid; q < TN * 8; q += NT) {
-      int r, k;
-      size_t row;
-      bool up;
-      piece_of<T, TN, BKS>(q, r, k);
-      b_row(r, row, up);
-      const size_t kk = (size_t)t * KT + k;
-      const T *p = P.b[up ? 1 : 0];
-      *(i4 *)(to + q * 16) = BKS ? fetch16(p, P.ldb, kk, P.k, row, P.cols) : fetch16(p, P.ldb, row, P.cols, kk, P.k);
+  auto part_b = [&](const unsigned t, const uint32_t to) {
+#pragma unroll
+    for (int d = 0; d < PB; ++d) {
+      if (inside(tile_b, BKS, t, d)) dma_b(d, to);
+      else *(QR_LDS i4 *)(to + (d * NT + tid) * 16) = i4{0, 0, 0, 0};
     }
   };
   i4 vb[PB];
   auto load_b = [&](const unsigned t) {
-    if (KIND == DX || t < whole) {
 #pragma unroll
-      for (int d = 0; d < PB; ++d) {
-        vb[d] = *(const QR_GLB i4 *)((const QR_GLB char *)sb + offb[d]);
-      }
-      next_b(t);
-    } else {
-#pragma unroll
-      for (int d = 0; d < PB; ++d) {
-        int r, k;
-        size_t row;
-        bool up;
-        piece_of<T, TN, BKS>(d * NT + tid, r, k);
-        b_row(r, row, up);
-        const size_t kk = (size_t)t * KT + k;
-        vb[d] = BKS ? fetch16(P.b[up ? 1 : 0], P.ldb, kk, P.k, row, P.cols) : fetch16(P.b[up ? 1 : 0], P.ldb, row, P.cols, kk, P.k);
-      }
+    for (int d = 0; d < PB; ++d) {
+      vb[d] = i4{0, 0, 0, 0};
+      if (KIND == DX || t < whole || inside(tile_b, BKS, t, d)) vb[d] = *(const QR_GLB i4 *)((const QR_GLB char *)sb + offb[d]);
     }
+    next_b(t);
   };
   auto keep_b = [&]() {
 #pragma unroll
@@ -452,7 +440,7 @@ __global__ __launch_bounds__(128 * WN, 2) void k_gemm(const GemmArgs<T> P) {
       for (int d = 0; d < PA; ++d) load_a(d, at_a);
       next_a(first);
     } else {
-      fill_a(first, lds);
+      part_a(first, at_a);
     }
     if (!BD) {
       load_b(first);
@@ -462,7 +450,7 @@ __global__ __launch_bounds__(128 * WN, 2) void k_gemm(const GemmArgs<T> P) {
       for (int d = 0; d < PB; ++d) dma_b(d, at_b);
       next_b(first);
     } else {
-      fill_b(first, lds + 2 * ABUF);
+      part_b(first, at_b);
     }
     uint32_t cur = 0, cur_b = 0;
     unsigned t = first;
@@ -483,8 +471,8 @@ __global__ __launch_bounds__(128 * WN, 2) void k_gemm(const GemmArgs<T> P) {
       wait_all();
       barrier();
       if (t + 1 < last) {
-        fill_a(t + 1, lds + (cur ^ ABUF));
-        if (BD) fill_b(t + 1, lds + 2 * ABUF + (cur_b ^ BBUF));
+        part_a(t + 1, at_a + (cur ^ ABUF));
+        if (BD) part_b(t + 1, at_b + (cur_b ^ BBUF));
         else load_b(t + 1);
       }
       compute(std::false_type{}, base_a + cur, base_b + cur_b, 0, 0);
@@ -625,20 +613,38 @@ __global__ __launch_bounds__(512) void k_few(const GemmArgs<T> P) {
     }
 }
 
-// Partial sums joined in the order of the splits: `outs` matrices of [rows][cols], rows of stride ldo.  V = 4: four
-// neighbours of a row a thread (cols a multiple of four)
-template <class T, int V>
+constexpr unsigned CUS = 256;
+
+// Partial sums joined in a fixed order: `outs` matrices of [rows][cols], rows of stride ldo.  V = 4: four neighbours of a
+// row a thread (cols a multiple of four); P shares of the splits, of threads of their own
+template <class T, int V, int P>
 __global__ __launch_bounds__(256) void k_join(const float *__restrict__ part, const size_t rows, const size_t cols, const unsigned outs,
                                               const unsigned splits, T *__restrict__ o0, T *__restrict__ o1, const size_t ldo) {
+  constexpr int W = 256 / P;
   const size_t n = rows * cols;
-  for (size_t i = ((size_t)blockIdx.x * 256 + threadIdx.x) * V; i < outs * n; i += (size_t)gridDim.x * 256 * V) {
+  const unsigned w = threadIdx.x % W, q = threadIdx.x / W;
+  __shared__ float lds[P][W][V];
+  for (size_t i0 = (size_t)blockIdx.x * W * V; i0 < outs * n; i0 += (size_t)gridDim.x * W * V) {
+    const size_t i = i0 + (size_t)w * V;
     float s[V] = {}, v[V];
+    if (i < outs * n)
 #pragma unroll 4
-    for (unsigned p = 0; p < splits; ++p) {
-      __builtin_memcpy(v, part + p * outs * n + i, sizeof v);
+      for (unsigned p = q; p < splits; p += P) {
+        __builtin_memcpy(v, part + p * outs * n + i, sizeof v);
 #pragma unroll
-      for (int e = 0; e < V; ++e) s[e] += v[e];
+        for (int e = 0; e < V; ++e) s[e] += v[e];
+      }
+    if constexpr (P > 1) {
+      __builtin_memcpy(lds[q][w], s, sizeof s);
+      __syncthreads();
+      if (q == 0)
+#pragma unroll
+        for (int p = 1; p < P; ++p)
+#pragma unroll
+          for (int e = 0; e < V; ++e) s[e] += lds[p][w][e];
+      __syncthreads();
     }
+    if (q || i >= outs * n) continue;
     const size_t j = i < n ? i : i - n, r = n <= 0xFFFFFFFFu ? (uint32_t)j / (uint32_t)cols : j / cols;
     T t[V];
 #pragma unroll
@@ -646,12 +652,20 @@ __global__ __launch_bounds__(256) void k_join(const float *__restrict__ part, co
     __builtin_memcpy((i < n ? o0 : o1) + r * ldo + (j - r * cols), t, sizeof t);
   }
 }
+// 16 shares where there are at least as many splits and one thread an output would not fill the chip's waves
 template <class T>
 void join(hipStream_t s, const float *part, size_t rows, size_t cols, unsigned outs, unsigned splits, T *o0, T *o1, size_t ldo) {
-  const size_t n = outs * rows * cols;
-  const auto grid = [](size_t t) { return (unsigned)std::min<size_t>((t + 255) / 256, 65536); };
-  if (cols % 4 == 0) k_join<T, 4><<<grid(n / 4), 256, 0, s>>>(part, rows, cols, outs, splits, o0, o1, ldo);
-  else k_join<T, 1><<<grid(n), 256, 0, s>>>(part, rows, cols, outs, splits, o0, o1, ldo);
+  const auto go = [&](auto v, auto p) {
+    constexpr int V = decltype(v)::value, P = decltype(p)::value;
+    const size_t groups = (outs * rows * cols / V + 256 / P - 1) / (256 / P);
+    k_join<T, V, P><<<(unsigned)std::min<size_t>(groups, 65536), 256, 0, s>>>(part, rows, cols, outs, splits, o0, o1, ldo);
+  };
+  using one = std::integral_constant<int, 1>;
+  using four = std::integral_constant<int, 4>;
+  using sixteen = std::integral_constant<int, 16>;
+  const bool shares = splits >= 16 && outs * rows * cols < CUS * 2048;
+  if (cols % 4 == 0) shares ? go(four{}, sixteen{}) : go(four{}, one{});
+  else shares ? go(one{}, sixteen{}) : go(one{}, one{});
 }
 
 // dg, du in rows of stride ld, their padding zeroed; eight elements a thread.  (The padding is at least as long as what
@@ -735,10 +749,9 @@ unsigned blocks(size_t n) { return (unsigned)((n + 255) / 256 < 65536 ? (n + 255
 // longest row the product kernel takes: a tile's 256 rows lie within 2^31 bytes
 constexpr size_t ROW_BYTES = (size_t)1 << 22;
 
-// whether the product kernel can read a matrix where it lies: rows at 16-byte boundaries and, where the columns are
-// what it moves in pieces (the columns layout), none cut by the row's end
-bool in_place(const void *p, size_t ld, size_t cols, size_t e, bool columns) {
-  return ((uintptr_t)p & 15) == 0 && (ld * e) % 16 == 0 && ld * e <= ROW_BYTES && (!columns || (cols * e) % 16 == 0);
+// whether the product kernel can read a matrix where it lies: rows of whole pieces of 16 bytes at 16-byte boundaries
+bool in_place(const void *p, size_t ld, size_t cols, size_t e) {
+  return ((uintptr_t)p & 15) == 0 && (ld * e) % 16 == 0 && ld * e <= ROW_BYTES && (cols * e) % 16 == 0;
 }
 
 // notes that `p` is to be copied, and makes it and its stride those of the copy
@@ -766,7 +779,6 @@ void launch_gemm(hipStream_t s, GemmArgs<T> P) {
 }
 
 
-constexpr unsigned CUS = 256;
 
 // Whether the forward pass takes the few-rows kernel: where tiles of 64 x 64 sums would leave half the compute units
 // without one, and up to one such tile of rows.  Few rows / tiles in us, back to back in a graph: k 1024, n 4096 bf16 1 row
@@ -800,8 +812,9 @@ Tile tile_of(size_t e, size_t rows, size_t cols, size_t times, bool narrow) {
     const size_t cost = tiles_of(cols, v) * (e == 2 ? v : mat > vec ? mat : vec);
     if (cost <= least && v <= (e == 2 ? 128 : 160)) least = cost, w = v;
   }
-  if (e == 2 && w == 128 && (size_t)tiles_of(rows, 256) * tiles_of(cols, 128) * times >= CUS) return {256, 128};
-  if ((size_t)tiles_of(rows, 128) * tiles_of(cols, w) * times >= CUS) return {128, (int)w};
+  const bool tall = tiles_of(rows, 256) * 14 <= tiles_of(rows, 128) * 8;
+  if (e == 2 && w == 128 && tall && (size_t)tiles_of(rows, 256) * tiles_of(cols, 128) * times >= CUS) return {256, 128};
+  if (rows > 64 && (size_t)tiles_of(rows, 128) * tiles_of(cols, w) * times >= CUS) return {128, (int)w};
   return {64, 64};
 }
 
@@ -893,12 +906,12 @@ extern "C" int qr_gated_ffn_async(int device, void *stream, int type, int act, s
   if (!m) return QR_OK;
   QR_DENSE_ARG(x && w_gate && w_up && h, "gated ffn: x, a weight or h is NULL");
   const size_t e = qr_dense_size(type);
-  const bool px = !few(m, n) && !in_place(x, ldx, k, e, false), pw = !few(m, n) && (!in_place(w_gate, ldw, k, e, false) || !in_place(w_up, ldw, k, e, false));
+  const bool px = !few(m, n) && !in_place(x, ldx, k, e), pw = !few(m, n) && (!in_place(w_gate, ldw, k, e) || !in_place(w_up, ldw, k, e));
   size_t need = 0;
   if (px || pw)
     if (int rc = qr_gated_ffn_workspace(type, m, k, n, &need)) return rc;
   QR_DENSE_ARG(!need || (workspace && workspace_bytes >= need),
-               "gated ffn: rows off 16-byte boundaries or more than 4 MB apart need the workspace");
+               "gated ffn: rows that start or end off 16-byte boundaries or lie more than 4 MB apart need the workspace");
   if (!few(m, n) && k * e > ROW_BYTES) return qr_dense_fail(QR_ERR_UNSUPPORTED, "gated ffn: rows longer than 4 MB");
   const void *out[4] = {h, gate, up, workspace};
   const size_t bytes[4] = {qr_dense_span(m, n, ldh, e), m * n * e, m * n * e, need};
@@ -988,11 +1001,11 @@ extern "C" int qr_gated_ffn_backward_async(int device, void *stream, int type, i
     W.a[0] = dg, W.a[1] = du, W.b[0] = (const T *)x;
     W.lda = ld, W.ldb = ldx, W.rows = n, W.cols = k, W.k = m, W.o[0] = (T *)dw_gate, W.o[1] = (T *)dw_up, W.ldo = k;
     Packs<T> packs;
-    if (dx && m && (ld != n || !in_place(w_gate, ldw, k, e, true) || !in_place(w_up, ldw, k, e, true))) {
+    if (dx && m && (ld != n || !in_place(w_gate, ldw, k, e) || !in_place(w_up, ldw, k, e))) {
       size_t to = ldw;
       pack(packs, n, k, X.b[0], to, ws, ld), pack(packs, n, k, X.b[1], X.ldb, ws, ld);
     }
-    if (dw_gate && m && !in_place(x, ldx, k, e, true)) pack(packs, m, k, W.b[0], W.ldb, ws, m);
+    if (dw_gate && m && !in_place(x, ldx, k, e)) pack(packs, m, k, W.b[0], W.ldb, ws, m);
     launch_pack(s, packs);
     if (dx && m) {
       X.splits = px.splits, X.steps = px.steps, X.part = px.splits > 1 ? part : nullptr;

@@ -247,56 +247,61 @@ __global__ __launch_bounds__(G > 256 ? G : 256) void k_norm_grad(const size_t ro
       part[((size_t)blockIdx.x * 2 + 1) * cols + j] = vb;
     }
   };
-  // the groups of the workgroup one after the other (each column has one owner in a group)
+  // a wave's groups are added by their lanes, the four waves' sums through LDS (each column has one owner in a group)
   extern __shared__ float sum[];
-  for (int g = 0; g < RPB; ++g) {
-    if (grp == g) {
+  float *const own = sum + (threadIdx.x >> 6) * 2 * cols;
 #pragma unroll
-      for (int i = 0; i < N; ++i) {
-        if (!S.inner(i) && !S.any(i, l)) continue;
-        const int at = S.at(i, l), dup = S.dup(i, l);
+  for (int i = 0; i < N; ++i) {
+    if (!S.inner(i) && !S.any(i, l)) continue;
+    const int at = S.at(i, l), dup = S.dup(i, l);
 #pragma unroll
-        for (int e = 0; e < V; ++e)
-          if (e >= dup) {
-            if (RPB == 1) {
-              keep(at + e, sw[i][e], sb[i][e]);
-            } else {
-              sum[at + e] = (g ? sum[at + e] : 0.f) + sw[i][e];
-              sum[cols + at + e] = (g ? sum[cols + at + e] : 0.f) + sb[i][e];
-            }
-          }
+    for (int e = 0; e < V; ++e) {
+      float vw = sw[i][e], vb = sb[i][e];
+      if constexpr (G < 64) {
+        vw += __shfl_xor(vw, 16), vb += __shfl_xor(vb, 16);
+        vw += __shfl_xor(vw, 32), vb += __shfl_xor(vb, 32);
       }
+      if (e < dup || (threadIdx.x & 63) >= G) continue;
+      if constexpr (RPB == 1) keep(at + e, vw, vb);
+      else own[at + e] = vw, own[cols + at + e] = vb;
     }
-    if (RPB > 1) __syncthreads();
   }
-  if (RPB > 1)
-    for (int j = threadIdx.x; j < cols; j += 256) keep(j, sum[j], sum[cols + j]);
+  if constexpr (RPB > 1) {
+    __syncthreads();
+    for (int j = threadIdx.x; j < cols; j += 256) {
+      const float *const v = sum + j, *const u = v + cols;
+      keep(j, (v[0] + v[2 * cols]) + (v[4 * cols] + v[6 * cols]), (u[0] + u[2 * cols]) + (u[4 * cols] + u[6 * cols]));
+    }
+  }
 }
 
-// 16 columns by 64 shares of the partial sums
-template <class P>
+// Partial sums joined in a fixed order: 1024 / Q columns by Q shares
+template <class P, int Q>
 __global__ __launch_bounds__(1024) void k_norm_join(const int cols, const int parts, const float *__restrict__ part, P *__restrict__ dw,
                                                     P *__restrict__ db) {
-  __shared__ float lds[64][17];
-  const int c = threadIdx.x & 15, q = threadIdx.x >> 4;
-  const size_t j = (size_t)blockIdx.x * 16 + c, n = 2 * (size_t)cols;
+  constexpr int W = 1024 / Q;
+  __shared__ float lds[Q][W + 1];
+  const int c = threadIdx.x % W, q = threadIdx.x / W;
+  const size_t j = (size_t)blockIdx.x * W + c, n = 2 * (size_t)cols;
   float s = 0.f;
   if (j < n)
 #pragma unroll 4
-    for (int p = q; p < parts; p += 64) s += part[p * n + j];
+    for (int p = q; p < parts; p += Q) s += part[p * n + j];
   lds[q][c] = s;
   __syncthreads();
-  if (threadIdx.x < 256) {
-    // four shares a thread, then the four quarters of a column's sixteen
-    const int h = threadIdx.x >> 4;
-    s = (lds[4 * h][c] + lds[4 * h + 1][c]) + (lds[4 * h + 2][c] + lds[4 * h + 3][c]);
-    s += __shfl_xor(s, 16);
-    s += __shfl_xor(s, 32);
+  if constexpr (Q == 64) {
+    if (threadIdx.x < 256) {
+      // four shares a thread, then the four quarters of a column's sixteen
+      const int h = threadIdx.x >> 4;
+      s = (lds[4 * h][c] + lds[4 * h + 1][c]) + (lds[4 * h + 2][c] + lds[4 * h + 3][c]);
+      s += __shfl_xor(s, 16);
+      s += __shfl_xor(s, 32);
+    }
+    __syncthreads();
+    if (threadIdx.x < 256 && (threadIdx.x & 63) < 16) lds[threadIdx.x >> 6][c] = s;
+    __syncthreads();
   }
-  __syncthreads();
-  if (threadIdx.x < 256 && (threadIdx.x & 63) < 16) lds[threadIdx.x >> 6][c] = s;
-  __syncthreads();
-  if (threadIdx.x < 16 && j < n) {
+  if (threadIdx.x < W && j < n) {
     s = (lds[0][c] + lds[1][c]) + (lds[2][c] + lds[3][c]);
     if (j < (size_t)cols) {
       if (dw) dw[j] = (P)s;
@@ -305,31 +310,37 @@ __global__ __launch_bounds__(1024) void k_norm_join(const int cols, const int pa
     }
   }
 }
+// 64 shares, or four where there are few parts: 5 rows of 12089 columns bf16, forward and join, JOINUS
+template <class P>
+void norm_join(hipStream_t s, size_t cols, size_t parts, const float *part, void *dw, void *db) {
+  if (parts >= 64) k_norm_join<P, 64><<<(unsigned)((2 * cols + 15) / 16), 1024, 0, s>>>((int)cols, (int)parts, part, (P *)dw, (P *)db);
+  else k_norm_join<P, 4><<<(unsigned)((2 * cols + 255) / 256), 1024, 0, s>>>((int)cols, (int)parts, part, (P *)dw, (P *)db);
+}
 
 // ---- rows that no workgroup's registers hold (and rows of less than 16 bytes): read again for every step ----------
 
-// the sum over a workgroup of 256, in every thread
+// the sum over a workgroup of 1024, in every thread
 __device__ __forceinline__ float block_sum(float v) {
-  __shared__ float lds[8];
-  return group_sum<256>(v, lds);
+  __shared__ float lds[32];
+  return group_sum<1024>(v, lds);
 }
 
 template <class T, class P>
-__global__ __launch_bounds__(256) void k_norm_any(const size_t rows, const int cols, const T *x, const size_t ldx,
+__global__ __launch_bounds__(1024) void k_norm_any(const size_t rows, const int cols, const T *x, const size_t ldx,
                                                   const P *__restrict__ w, const P *__restrict__ b, const float eps, T *y,
                                                   const size_t ldy, float *__restrict__ mean, float *__restrict__ rstd) {
   for (size_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const T *xr = x + r * ldx;
     float s = 0.f;
-    for (int j = threadIdx.x; j < cols; j += 256) s += (float)xr[j];
+    for (int j = threadIdx.x; j < cols; j += 1024) s += (float)xr[j];
     const float mu = block_sum(s) / (float)cols;
     s = 0.f;
-    for (int j = threadIdx.x; j < cols; j += 256) {
+    for (int j = threadIdx.x; j < cols; j += 1024) {
       const float d = (float)xr[j] - mu;
       s = fmaf(d, d, s);
     }
     const float rs = 1.f / sqrtf(block_sum(s) / (float)cols + eps);
-    for (int j = threadIdx.x; j < cols; j += 256)
+    for (int j = threadIdx.x; j < cols; j += 1024)
       y[r * ldy + j] = (T)fmaf(((float)xr[j] - mu) * rs, w ? (float)w[j] : 1.f, b ? (float)b[j] : 0.f);
     if (threadIdx.x == 0) {
       if (mean) mean[r] = mu;
@@ -339,20 +350,20 @@ __global__ __launch_bounds__(256) void k_norm_any(const size_t rows, const int c
 }
 
 template <class T, class P>
-__global__ __launch_bounds__(256) void k_norm_grad_any(const size_t rows, const int cols, const T *dy, const size_t lddy, const T *x,
+__global__ __launch_bounds__(1024) void k_norm_grad_any(const size_t rows, const int cols, const T *dy, const size_t lddy, const T *x,
                                                        const size_t ldx, const P *__restrict__ w, const float *__restrict__ mean,
                                                        const float *__restrict__ rstd, T *dx, const size_t lddx) {
   for (size_t r = blockIdx.x; r < rows; r += gridDim.x) {
     const float mu = mean[r], rs = rstd[r];
     float a = 0.f, c = 0.f;
-    for (int j = threadIdx.x; j < cols; j += 256) {
+    for (int j = threadIdx.x; j < cols; j += 1024) {
       const float g = (float)dy[r * lddy + j] * (w ? (float)w[j] : 1.f), h = ((float)x[r * ldx + j] - mu) * rs;
       a += g;
       c = fmaf(g, h, c);
     }
     a = block_sum(a) / (float)cols;
     c = block_sum(c) / (float)cols;
-    for (int j = threadIdx.x; j < cols; j += 256) {
+    for (int j = threadIdx.x; j < cols; j += 1024) {
       const float g = (float)dy[r * lddy + j] * (w ? (float)w[j] : 1.f), h = ((float)x[r * ldx + j] - mu) * rs;
       dx[r * lddx + j] = (T)(rs * (g - a - h * c));
     }
@@ -448,7 +459,7 @@ extern "C" int qr_layer_norm_async(int device, void *stream, int type, int param
         }
       });
       if (!fits)
-        k_norm_any<T, P><<<(unsigned)(rows < 65536 ? rows : 65536), 256, 0, s>>>(rows, (int)cols, (const T *)x, ldx, (const P *)weight,
+        k_norm_any<T, P><<<(unsigned)(rows < 65536 ? rows : 65536), 1024, 0, s>>>(rows, (int)cols, (const T *)x, ldx, (const P *)weight,
                                                                                 (const P *)bias, eps, (T *)y, ldy, mean, rstd);
     };
     if (param_type == QR_F32) go(float{});
@@ -492,9 +503,9 @@ extern "C" int qr_layer_norm_backward_async(int device, void *stream, int type, 
         constexpr size_t RPB = G() > 256 ? 1 : 256 / G();
         const size_t want = (rows + RPB - 1) / RPB, parts = parts_of(rows, G(), N());
         const unsigned grid = want <= ALONE ? 1 : (unsigned)(want < parts ? want : parts);
-        k_norm_grad<T, P, G(), N()><<<grid, G() > 256 ? G() : 256, RPB > 1 && sums ? 2 * cols * 4 : 0, s>>>(
+        k_norm_grad<T, P, G(), N()><<<grid, G() > 256 ? G() : 256, RPB > 1 && sums ? 8 * cols * 4 : 0, s>>>(
             rows, (int)cols, (const T *)dy, lddy, (const T *)x, ldx, (const P *)weight, mean, rstd, (T *)dx, lddx, part, (P *)dweight, (P *)dbias);
-        if (sums && grid > 1) k_norm_join<P><<<(unsigned)((2 * cols + 15) / 16), 1024, 0, s>>>((int)cols, (int)grid, part, (P *)dweight, (P *)dbias);
+        if (sums && grid > 1) norm_join<P>(s, cols, grid, part, dweight, dbias);
       });
       if (fits && rows) return;
       // (the column sums first: dx may be written over dy or x)
@@ -502,9 +513,9 @@ extern "C" int qr_layer_norm_backward_async(int device, void *stream, int type, 
         k_norm_cols<T><<<dim3((unsigned)((cols + 255) / 256), any), 256, 0, s>>>(rows, (int)cols, (const T *)dy, lddy, (const T *)x,
                                                                                   ldx, mean, rstd, part);
       if (sums)
-        k_norm_join<P><<<(unsigned)((2 * cols + 15) / 16), 1024, 0, s>>>((int)cols, (int)any, part, (P *)dweight, (P *)dbias);
+        norm_join<P>(s, cols, any, part, dweight, dbias);
       if (rows && dx)
-        k_norm_grad_any<T, P><<<(unsigned)(rows < 65536 ? rows : 65536), 256, 0, s>>>(
+        k_norm_grad_any<T, P><<<(unsigned)(rows < 65536 ? rows : 65536), 1024, 0, s>>>(
             rows, (int)cols, (const T *)dy, lddy, (const T *)x, ldx, (const P *)weight, mean, rstd, (T *)dx, lddx);
     };
     if (param_type == QR_F32) go(float{});

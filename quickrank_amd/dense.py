@@ -199,8 +199,8 @@ def gated_ffn(x, w_gate, w_up, act="silu", save=False):
     g, u = (x.new_empty(shape), x.new_empty(shape)) if save else (None, None)
     px, pg, pu, e = x.data_ptr(), w_gate.data_ptr(), w_up.data_ptr(), x.element_size()
     ws, need, rc = None, C.c_size_t(), 0
-    # rows that do not start at 16-byte boundaries or lie more than 4 MB apart are copied first
-    if (px | pg | pu | ldx * e | ldw * e) & 15 or max(ldx, ldw) * e > 1 << 22:
+    # rows that do not start and end at 16-byte boundaries or lie more than 4 MB apart are copied first
+    if (px | pg | pu | ldx * e | ldw * e | k * e) & 15 or max(ldx, ldw) * e > 1 << 22:
         rc = lib().qr_gated_ffn_workspace(TYPES[x.dtype], m, k, n, C.byref(need))
         ws = x.new_empty(need.value, dtype=torch.uint8)
     rc = rc or lib().qr_gated_ffn_async(x.device.index, _stream(x), TYPES[x.dtype], a, m, k, n, px, ldx, pg, pu, ldw, h.data_ptr(), n,
