@@ -201,17 +201,20 @@ __device__ __forceinline__ i4 fetch16(const T *p, const size_t ld, const size_t 
   return v;
 }
 
-// Eight results of one row, rounded; the row's base need not be aligned.  STREAM: past the caches, for outputs that are
-// far larger and would push the operands out of the L2 (32768 x 1024 x 4096 bf16 with both products kept: 716 -> 599 us).
-typedef int u4 __attribute__((ext_vector_type(4), aligned(4)));
-template <bool STREAM, class T>
-__device__ __forceinline__ void store8(T *p, const float (&v)[8], const size_t at, const size_t len) {
+// Eight results of one row, rounded; the row's base need not be aligned.  `stream`: past the caches
+typedef int u4 __attribute__((ext_vector_type(4)));
+template <class T>
+__device__ __forceinline__ void store8(const bool stream, T *p, const float (&v)[8], const size_t at, const size_t len) {
   if (at + 8 <= len) {
     T t[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) t[e] = (T)v[e];
-    if constexpr (STREAM && sizeof(T) == 2) __builtin_nontemporal_store(__builtin_bit_cast(u4, t), (u4 *)(p + at));
-    else __builtin_memcpy(p + at, t, sizeof t);
+    if constexpr (sizeof(T) == 2)
+      if (stream) {
+        __builtin_nontemporal_store(__builtin_bit_cast(u4, t), (u4 *)(p + at));
+        return;
+      }
+    __builtin_memcpy(p + at, t, sizeof t);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; ++e)
@@ -231,6 +234,7 @@ struct GemmArgs {
   float *part;           // partial sums, DX [split][rows][cols], DW [split][2][rows][cols], where the sums are split
   size_t ldo;
   int act;
+  bool stream;           // results go past the caches
   unsigned row_tiles, col_tiles, splits, steps;  // steps: k tiles of one split
 };
 
@@ -492,6 +496,7 @@ __global__ __launch_bounds__(128 * WN, 2) void k_gemm(const GemmArgs<T> P) {
     return (f4 *)(own + (row * PIECES + c) * 16);
   };
   const int l = tid & 63;
+  const bool stream = sizeof(T) == 2 && P.stream;
 #pragma unroll
   for (int m0 = 0; m0 < MI; m0 += MB) {
 #pragma unroll
@@ -520,15 +525,15 @@ __global__ __launch_bounds__(128 * WN, 2) void k_gemm(const GemmArgs<T> P) {
         take((s >> 1) * 8 + (s & 1) * 2, v);
         take((s >> 1) * 8 + 4 + (s & 1) * 2, u);
         gated8(P.act, v, u, h);
-        store8<(TM > 128)>(P.o[0] + row * P.ldo, h, col, P.cols);
+        store8(stream, P.o[0] + row * P.ldo, h, col, P.cols);
         if (P.o[1]) {
-          store8<(TM > 128)>(P.o[1] + row * P.cols, v, col, P.cols);
-          store8<(TM > 128)>(P.o[2] + row * P.cols, u, col, P.cols);
+          store8(stream, P.o[1] + row * P.cols, v, col, P.cols);
+          store8(stream, P.o[2] + row * P.cols, u, col, P.cols);
         }
       } else {
         take(s * 2, v);
-        if (P.part) store8<(TM > 128)>(P.part + ((size_t)(split * OUTS + z) * P.rows + row) * P.cols, v, col, P.cols);
-        else store8<(TM > 128)>(P.o[z] + row * P.ldo, v, col, P.cols);
+        if (P.part) store8(stream, P.part + ((size_t)(split * OUTS + z) * P.rows + row) * P.cols, v, col, P.cols);
+        else store8(stream, P.o[z] + row * P.ldo, v, col, P.cols);
       }
     }
     __builtin_amdgcn_wave_barrier();
@@ -770,9 +775,23 @@ void launch_pack(hipStream_t s, const Packs<T> &packs) {
   if (packs.n && most) k_pack<T><<<dim3(blocks(most), packs.n), 256, 0, s>>>(packs);
 }
 
+// Whether results go past the caches, so that they do not push the operands out.  Only in whole parts of 64 bytes, what
+// the memory writes at once (65536 x 256 x 1000 bf16, both products kept: 356 us past the caches, 174 through them).  Where
+// the three results are kept, the caches' 256 MB take some of them up: past the caches where the sums are long, or not short
+// and the results larger than that.  Past / through, 16384 x 32 x 4096 121 / 102 us, 32768 x 256 x 1024 69 / 58, 16384 x 256
+// x 4096 125 / 149, 32768 x 1024 x 4096 542 / 596; one result, 32768 x 32 x 1024 33 / 35, 8192 x 8192 x 4096 740 / 799.
+template <class T>
+bool streams(const GemmArgs<T> &P, const size_t outs) {
+  bool whole = (P.ldo * sizeof(T)) % 64 == 0 && (P.cols * sizeof(T)) % 64 == 0;
+  for (size_t i = 0; i < outs; ++i) whole &= ((uintptr_t)P.o[i] & 63) == 0;
+  const size_t sum = P.k * sizeof(T), bytes = outs * P.rows * P.cols * sizeof(T);
+  return whole && (outs < 3 || sum >= 1024 || (sum >= 256 && bytes > ((size_t)256 << 20)));
+}
+
 template <class T, Kind KIND, int TM, int TN, int WN = 2>
 void launch_gemm(hipStream_t s, GemmArgs<T> P) {
   P.row_tiles = tiles_of(P.rows, TM);
+  P.stream = streams(P, KIND == FWD ? (P.o[1] ? 3 : 1) : KIND == DW ? 2 : 1);
   P.col_tiles = tiles_of(P.cols, KIND == FWD ? TN / 2 : TN);
   const unsigned tiles = P.row_tiles * P.col_tiles * (KIND == FWD ? 1 : (KIND == DW ? 2 : 1) * P.splits);
   k_gemm<T, KIND, TM, TN, WN><<<(tiles + 7) / 8 * 8, 128 * WN, 0, s>>>(P);
