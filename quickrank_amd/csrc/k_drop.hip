@@ -7,6 +7,9 @@
 //
 // The scale is that of the probability the 16 bits can express, so the expectation is x exactly.
 // The backward pass is the same call on dy.
+//
+// Bound by memory: some thirty integer instructions a word of four elements hide behind it.  65536 x 2048 bf16 with a
+// residual 151 us (5.3 TB/s), 99991 x 1145 f16 without 83 us (5.5), where a copy reaches 4.9 to 5.4; 100 x 512 f32 2.7 us.
 #include "qr_dense.h"
 
 namespace {
@@ -28,7 +31,8 @@ __device__ __forceinline__ T dropped(const T x, const float r, const uint32_t bi
   return (T)((bits >= t ? (float)x * scale : 0.f) + r);
 }
 
-// rows without gaps: a thread takes pieces of 16 bytes of the whole, U of them under way at a time
+// rows without gaps: a thread takes pieces of 16 bytes of the whole, U of them under way at a time (their loads' latency
+// is what a wave would wait for)
 template <class T, bool RES, int U>
 __global__ __launch_bounds__(256) void k_drop_flat(const size_t n, const T *x, const T *res, T *y, const uint32_t t, const float scale,
                                                    const uint64_t key, const uint64_t offset, const uint64_t *__restrict__ counter) {

@@ -80,7 +80,7 @@ __device__ __forceinline__ f4 mma(const i4 a, const i4 b, f4 c) {
 // f32 operands of the product kernel as three bf16 each: 24 bits of mantissa are 8 + 8 + 8, so high + mid + low IS the
 // number (down to 2^-110; an infinite one has NaN parts).  Of the nine products the six largest are taken, each exact in
 // f32; those left out are below 2^-21 of the whole, 2^-23.5 on average.  Six bf16 matrix instructions take 96 cycles for
-// 16 x 16 x 32 where the f32 ones take 256, for 5.5 vector instructions an element, which run under them.
+// 16 x 16 x 32 where the f32 ones take 256, at 5.5 vector instructions an element of each fragment.
 struct Split {
   b8 part[3];
 };
@@ -261,9 +261,10 @@ __device__ __forceinline__ uint32_t lds_offset(const char *p) { return (uint32_t
 // zero-filled.
 //
 // What bounds it, 16-bit types: at 256 x 128 the way from L2 to the compute units (48 bytes a cycle and unit at the full
-// matrix rate, of 64), at 256 x 256 (32 bytes) the matrix cores at the clock that the card holds under them.  1490 TF at
-// 8192 x 8192 x (2 x 4096), where a large library product reaches 1320; 1170 TF at 32768 x 1024 x (2 x 4096), whose 16
-// stages leave a quarter of a tile's time to its first loads and its results.  f32: the six products per stage, 203 TF.
+// matrix rate, of 64), at 256 x 256 (32 bytes) the matrix cores at the clock that the card holds under them, 1.9 GHz.  1490
+// TF at 8192 x 8192 x (2 x 4096) bf16, where a large library product reaches 1320; 1180 TF at 32768 x 1024 x (2 x 4096),
+// whose 16 stages leave a quarter of a tile's time to its first loads and its results (1020 TF with g and u stored too).
+// f32: the six products and the splits before them, whose times add up (matrix cores 59 % busy): 190 to 200 TF.
 template <class T, Kind KIND, int TM, int TN, int WN>
 __global__ __launch_bounds__(128 * WN, 2) void k_gemm(const GemmArgs<T> P) {
   constexpr bool AKS = KIND == DW, BKS = KIND != FWD, BD = WN > 2;
@@ -543,7 +544,7 @@ __global__ __launch_bounds__(128 * WN, 2) void k_gemm(const GemmArgs<T> P) {
 // The forward pass of few rows: bound by reading the weights once and by latency, so no tile is staged.  A workgroup
 // makes 16 columns of h for 16 MB rows; its eight waves share the sum over k in steps of 128 bytes, read straight into
 // fragments (any alignment: a lane takes 32 consecutive bytes of a row, in x and in the weights alike), and are joined in
-// LDS in a fixed order.
+// LDS in a fixed order.  One row of k 1024, n 4096 bf16 (16.8 MB of weights) 5.2 us, 3.2 TB/s; 100 x 136 x 512 f32 4.0 us.
 template <class T, int MB>
 __global__ __launch_bounds__(512) void k_few(const GemmArgs<T> P) {
   constexpr int W = 8, KT = 128 / sizeof(T), E = 16 / sizeof(T);
@@ -673,7 +674,10 @@ void join(hipStream_t s, const float *part, size_t rows, size_t cols, unsigned o
   else shares ? go(one{}, sixteen{}) : go(one{}, one{});
 }
 
-// dg, du in rows of stride ld, their padding zeroed; eight elements a thread.  (The padding is at least as long as what
+// dg, du in rows of stride ld, their padding zeroed; eight elements a thread.  Bound by memory: five matrices, 16384 x 4096
+// bf16 111 us, 100000 x 512 f32 168 us (6.1 TB/s, some of it from the caches).  They are rounded to T so that the products
+// take them as they are: an f32 dx or dW is as exact as without, a 16-bit one is off by 2^1/2 times its own rounding (what
+// adds up is the rounding of each of many terms).  In 32 bits they would be twice the bytes and three products for one.  (The padding is at least as long as what
 // a row's last eight reach over.)
 template <class T, int ACT>
 __global__ __launch_bounds__(256) void k_gate_grad(const size_t m, const size_t n, const T *__restrict__ dh, const size_t lddh,
@@ -720,7 +724,7 @@ void gate_grad(hipStream_t s, size_t m, size_t n, int act, const void *dh, size_
 }
 
 // Matrices whose rows do not start at 16-byte boundaries, copied to ones whose rows do; the padding, and rows up to
-// rows_to, zeroed.  One of up to three by blockIdx.y
+// rows_to, zeroed.  One of up to three by blockIdx.y.  Bound by memory: 101549 x 609 f16 49 us (5.0 TB/s)
 template <class T>
 struct Packs {
   struct {

