@@ -36,21 +36,14 @@ __device__ __forceinline__ void act_of(const int act, const float g, float &a, f
   }
 }
 
-template <int ACT>
-__device__ __forceinline__ void gated8_of(const float (&g)[8], const float (&u)[8], float (&h)[8]) {
-#pragma unroll
-  for (int e = 0; e < 8; ++e) {
-    float a, d;
-    act_of(ACT, g[e], a, d);
-    h[e] = a * u[e];
-  }
-}
-__device__ __forceinline__ void gated8(const int act, const float (&g)[8], const float (&u)[8], float (&h)[8]) {
-  if (act == QR_ACT_SILU) gated8_of<QR_ACT_SILU>(g, u, h);
-  else if (act == QR_ACT_GELU) gated8_of<QR_ACT_GELU>(g, u, h);
-  else if (act == QR_ACT_GELU_TANH) gated8_of<QR_ACT_GELU_TANH>(g, u, h);
-  else if (act == QR_ACT_RELU) gated8_of<QR_ACT_RELU>(g, u, h);
-  else gated8_of<QR_ACT_SIGMOID>(g, u, h);
+// f(activation) as a constant
+template <class F>
+__host__ __device__ __forceinline__ void by_act(const int act, F &&f) {
+  if (act == QR_ACT_SILU) f(std::integral_constant<int, QR_ACT_SILU>{});
+  else if (act == QR_ACT_GELU) f(std::integral_constant<int, QR_ACT_GELU>{});
+  else if (act == QR_ACT_GELU_TANH) f(std::integral_constant<int, QR_ACT_GELU_TANH>{});
+  else if (act == QR_ACT_RELU) f(std::integral_constant<int, QR_ACT_RELU>{});
+  else f(std::integral_constant<int, QR_ACT_SIGMOID>{});
 }
 
 typedef float f4 __attribute__((ext_vector_type(4)));
@@ -201,23 +194,23 @@ __device__ __forceinline__ i4 fetch16(const T *p, const size_t ld, const size_t 
   return v;
 }
 
-// Eight results of one row, rounded; the row's base need not be aligned.  `stream`: past the caches
-typedef int u4 __attribute__((ext_vector_type(4)));
-template <class T>
-__device__ __forceinline__ void store8(const bool stream, T *p, const float (&v)[8], const size_t at, const size_t len) {
-  if (at + 8 <= len) {
-    T t[8];
+// V neighbouring results of one row, rounded; the row's base need not be aligned.  `stream`: past the caches
+template <class T, int V>
+__device__ __forceinline__ void store(const bool stream, T *p, const float (&v)[V], const size_t at, const size_t len) {
+  typedef int words __attribute__((ext_vector_type(V / 2)));
+  if (at + V <= len) {
+    T t[V];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) t[e] = (T)v[e];
+    for (int e = 0; e < V; ++e) t[e] = (T)v[e];
     if constexpr (sizeof(T) == 2)
       if (stream) {
-        __builtin_nontemporal_store(__builtin_bit_cast(u4, t), (u4 *)(p + at));
+        __builtin_nontemporal_store(__builtin_bit_cast(words, t), (words *)(p + at));
         return;
       }
     __builtin_memcpy(p + at, t, sizeof t);
   } else {
 #pragma unroll
-    for (int e = 0; e < 8; ++e)
+    for (int e = 0; e < V; ++e)
       if (at + e < len) p[at + e] = (T)v[e];
   }
 }
@@ -271,6 +264,7 @@ __global__ __launch_bounds__(128 * WN, 2) void k_gemm(const GemmArgs<T> P) {
   constexpr int WM = 2, NT = 128 * WN, KT = 128 / sizeof(T), E = 16 / sizeof(T);
   constexpr int MI = TM / WM / 16, NI = TN / WN / 16, PA = TM * 8 / NT, PB = TN * 8 / NT;
   constexpr int COLS = KIND == FWD ? TN / 2 : TN;
+  constexpr bool DIRECT = KIND == FWD && sizeof(T) == 2;  // results are stored from the registers of the sums
   constexpr uint32_t ABUF = TM * 128, BBUF = BD ? TN * 128 : 0, LDS_BYTES = 2 * ABUF + TN * 128 + BBUF;
   __shared__ __align__(1024) char lds[LDS_BYTES];
 
@@ -292,7 +286,9 @@ __global__ __launch_bounds__(128 * WN, 2) void k_gemm(const GemmArgs<T> P) {
   // a row of the second operand's tile: the output column it makes, and (FWD) of which product
   auto b_row = [&](int r, size_t &row, bool &up) {
     up = KIND == FWD && ((r >> 4) & 1);
-    row = KIND == FWD ? c0 + (r >> 5) * 16 + (r & 15) : c0 + r;
+    row = c0 + r;
+    // (of a wave's two pairs of blocks, 16-bit types: by fours in turn, so that a lane's sums of both are eight neighbours)
+    if (KIND == FWD) row = c0 + (DIRECT && NI == 4 ? (r >> 6) * 32 + ((r >> 2) & 3) * 8 + ((r >> 5) & 1) * 4 + (r & 3) : (r >> 5) * 16 + (r & 15));
   };
   const unsigned kt_all = (unsigned)((P.k + KT - 1) / KT);  // stages of one sum
   unsigned first = 0, last = KIND == DX ? 2 * kt_all : kt_all;
@@ -486,8 +482,38 @@ __global__ __launch_bounds__(128 * WN, 2) void k_gemm(const GemmArgs<T> P) {
     }
   }
 
+  const int l = tid & 63;
+  const bool stream = sizeof(T) == 2 && P.stream;
+  if constexpr (DIRECT) {
+    // A lane has g and u of V neighbours of a row, for each block of 16 rows; four lanes make 64 bytes of a row.  (Through
+    // LDS 466 us where this takes 438, 32768 x 1024 x 4096 bf16; f32 results, twice as wide, come out faster through LDS:
+    // 158 against 205 us, 100000 x 32 x 512 with g and u.)
+    constexpr int V = NI * 2;
+    auto finish = [&](auto act) {
+#pragma unroll
+      for (int m = 0; m < MI; ++m) {
+        const size_t row = r0 + (wm * MI + m) * 16 + (l & 15), col = c0 + wn * (NI * 8) + (l >> 4) * V;
+        if (row >= P.rows || col >= P.cols) continue;
+        float g[V], u[V], h[V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          float a, d;
+          g[e] = acc[m][e / 4 * 2][e % 4], u[e] = acc[m][e / 4 * 2 + 1][e % 4];
+          act_of(act(), g[e], a, d);
+          h[e] = a * u[e];
+        }
+        store(stream, P.o[0] + row * P.ldo, h, col, P.cols);
+        if (P.o[1]) {
+          store(stream, P.o[1] + row * P.cols, g, col, P.cols);
+          store(stream, P.o[2] + row * P.cols, u, col, P.cols);
+        }
+      }
+    };
+    by_act(P.act, finish);
+    return;
+  }
   // Results pass through the wave's own share of the LDS, so that a lane ends with eight neighbours of a row: one
-  // wide store, and one copy of the activation's code.  Pieces of four are moved by the row against bank conflicts.
+  // wide store.  Pieces of four are moved by the row against bank conflicts.
   constexpr int WTN = NI * 16, PIECES = WTN / 4, SHARE = LDS_BYTES / (WM * WN) / (16 * WTN * 4) * (16 * WTN * 4);
   constexpr int FIT = SHARE / (16 * WTN * 4), MB = FIT >= MI ? MI : FIT >= MI / 2 ? MI / 2 : MI / 4;  // blocks of 16 rows at a time
   static_assert(MB > 0 && MB <= FIT && MI % MB == 0 && (BD || PA % MI == 0), "blocks fit the waves' shares");
@@ -496,8 +522,6 @@ __global__ __launch_bounds__(128 * WN, 2) void k_gemm(const GemmArgs<T> P) {
     const int r = row & 15, c = (PIECES & (PIECES - 1)) == 0 ? piece ^ (r & (PIECES - 1)) : (piece + r) % PIECES;
     return (f4 *)(own + (row * PIECES + c) * 16);
   };
-  const int l = tid & 63;
-  const bool stream = sizeof(T) == 2 && P.stream;
 #pragma unroll
   for (int m0 = 0; m0 < MI; m0 += MB) {
 #pragma unroll
@@ -511,6 +535,7 @@ __global__ __launch_bounds__(128 * WN, 2) void k_gemm(const GemmArgs<T> P) {
     for (int q = l; q < MB * 16 * SEGS; q += 64) {
       const int r = q / SEGS, s = q % SEGS;
       const size_t row = r0 + (wm * MI + m0) * 16 + r, col = c0 + wn * (SEGS * 8) + s * 8;
+      if (row >= P.rows || col >= P.cols) continue;
       auto take = [&](int piece, float (&v)[8]) {
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
@@ -519,22 +544,28 @@ __global__ __launch_bounds__(128 * WN, 2) void k_gemm(const GemmArgs<T> P) {
           for (int e = 0; e < 4; ++e) v[h * 4 + e] = x[e];
         }
       };
-      if (row >= P.rows || col >= P.cols) continue;
       float v[8];
       if constexpr (KIND == FWD) {
         float u[8], h[8];
         take((s >> 1) * 8 + (s & 1) * 2, v);
         take((s >> 1) * 8 + 4 + (s & 1) * 2, u);
-        gated8(P.act, v, u, h);
-        store8(stream, P.o[0] + row * P.ldo, h, col, P.cols);
+        by_act(P.act, [&](auto act) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            float a, d;
+            act_of(act(), v[e], a, d);
+            h[e] = a * u[e];
+          }
+        });
+        store(stream, P.o[0] + row * P.ldo, h, col, P.cols);
         if (P.o[1]) {
-          store8(stream, P.o[1] + row * P.cols, v, col, P.cols);
-          store8(stream, P.o[2] + row * P.cols, u, col, P.cols);
+          store(stream, P.o[1] + row * P.cols, v, col, P.cols);
+          store(stream, P.o[2] + row * P.cols, u, col, P.cols);
         }
       } else {
         take(s * 2, v);
-        if (P.part) store8(stream, P.part + ((size_t)(split * OUTS + z) * P.rows + row) * P.cols, v, col, P.cols);
-        else store8(stream, P.o[z] + row * P.ldo, v, col, P.cols);
+        if (P.part) store(stream, P.part + ((size_t)(split * OUTS + z) * P.rows + row) * P.cols, v, col, P.cols);
+        else store(stream, P.o[z] + row * P.ldo, v, col, P.cols);
       }
     }
     __builtin_amdgcn_wave_barrier();
@@ -716,11 +747,7 @@ void gate_grad(hipStream_t s, size_t m, size_t n, int act, const void *dh, size_
   const auto go = [&](auto a) {
     k_gate_grad<T, decltype(a)::value><<<grid, 256, 0, s>>>(m, n, (const T *)dh, lddh, (const T *)g, (const T *)u, dg, du, ld);
   };
-  if (act == QR_ACT_SILU) go(std::integral_constant<int, QR_ACT_SILU>{});
-  else if (act == QR_ACT_GELU) go(std::integral_constant<int, QR_ACT_GELU>{});
-  else if (act == QR_ACT_GELU_TANH) go(std::integral_constant<int, QR_ACT_GELU_TANH>{});
-  else if (act == QR_ACT_RELU) go(std::integral_constant<int, QR_ACT_RELU>{});
-  else go(std::integral_constant<int, QR_ACT_SIGMOID>{});
+  by_act(act, go);
 }
 
 // Matrices whose rows do not start at 16-byte boundaries, copied to ones whose rows do; the padding, and rows up to
