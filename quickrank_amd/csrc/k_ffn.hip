@@ -254,9 +254,10 @@ __device__ __forceinline__ uint32_t lds_offset(const char *p) { return (uint32_t
 // zero-filled.
 //
 // What bounds it, 16-bit types: at 256 x 128 the way from L2 to the compute units (48 bytes a cycle and unit at the full
-// matrix rate, of 64), at 256 x 256 (32 bytes) the matrix cores at the clock that the card holds under them, 1.9 GHz.  1490
-// TF at 8192 x 8192 x (2 x 4096) bf16, where a large library product reaches 1320; 1180 TF at 32768 x 1024 x (2 x 4096),
-// whose 16 stages leave a quarter of a tile's time to its first loads and its results (1020 TF with g and u stored too).
+// matrix rate, of 64), at 256 x 256 (32 bytes) the matrix cores at the clock that the card holds under them, 1.9 GHz.  1530
+// TF at 8192 x 8192 x (2 x 4096) bf16, where a large library product reaches 1320; 1270 TF at 32768 x 1024 x (2 x 4096),
+// whose 16 stages leave a fifth of a tile's time to its first loads and its results (1020 TF with g and u stored too: 805
+// MB whose writing overlaps little).
 // f32: the six products and the splits before them, whose times add up (matrix cores 59 % busy): 190 to 200 TF.
 template <class T, Kind KIND, int TM, int TN, int WN>
 __global__ __launch_bounds__(128 * WN, 2) void k_gemm(const GemmArgs<T> P) {
@@ -888,8 +889,8 @@ void gemm(hipStream_t s, const Tile t, const GemmArgs<T> &P) {
 // time (1.39 us with every compute unit at work), fitted to times measured between 2 and 64 stages: a full round of the
 // large tiles takes 100 a stage and `edge`, one of the small 118 a stage and `edge` less 110 (290 where three matrices are
 // stored); a part of a round takes 3 / 4 of one, a small tile alone on its compute unit 1 / 2.  `large`, `small`: the
-// launches' workgroups and stages.  Measured: 8192 x 8192 x (2 x 4096) 740 us against 845, 32768 x 1024 x (2 x 4096) 459
-// against 490 (with g and u stored 528 against 545), their gradients for half the rows 564 against 604; but 8192 x 4096 x
+// launches' workgroups and stages.  Measured: 8192 x 8192 x (2 x 4096) 740 us against 845, 32768 x 1024 x (2 x 4096) 445
+// against 476 (with g and u stored 532 against 549), their gradients for half the rows 564 against 604; but 8192 x 4096 x
 // (2 x 1152), 288 large tiles, 176 against 161.
 struct Launch {
   size_t groups, stages;
