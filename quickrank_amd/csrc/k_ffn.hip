@@ -706,17 +706,54 @@ void join(hipStream_t s, const float *part, size_t rows, size_t cols, unsigned o
   else shares ? go(one{}, sixteen{}) : go(one{}, one{});
 }
 
+// Matrices whose rows do not start or end at 16-byte boundaries, copied to ones whose rows do; the padding, and rows up to
+// rows_to, zeroed.  Each has workgroups of its own.  Bound by memory: 101549 x 609 f16 49 us (5.0 TB/s)
+template <class T>
+struct Packs {
+  struct {
+    const T *p;
+    T *q;
+    size_t rows, cols, ld, to, rows_to;
+    unsigned groups;
+  } m[3] = {};
+  unsigned n = 0, groups = 0;
+};
+template <class T>
+__device__ __forceinline__ void pack_group(const Packs<T> &packs, unsigned group) {
+  constexpr int E = 16 / sizeof(T);
+#pragma unroll
+  for (int j = 0; j < 3; ++j) {
+    const auto &m = packs.m[j];
+    if (group < m.groups) {
+      const size_t per = m.to / E;
+      for (size_t i = (size_t)group * 256 + threadIdx.x; i < m.rows_to * per; i += (size_t)m.groups * 256) {
+        const size_t r = i / per, c = (i - r * per) * E;
+        *(i4 *)(m.q + r * m.to + c) = fetch16(m.p, m.ld, r, m.rows, c, m.cols);
+      }
+      return;
+    }
+    group -= m.groups;
+  }
+}
+template <class T>
+__global__ __launch_bounds__(256) void k_pack(const Packs<T> packs) {
+  pack_group(packs, blockIdx.x);
+}
+
 // dg, du in rows of stride ld, their padding zeroed; eight elements a thread.  Bound by memory: five matrices, 16384 x 4096
 // bf16 111 us, 100000 x 512 f32 168 us (6.1 TB/s, some of it from the caches).  They are rounded to T so that the products
 // take them as they are: an f32 dx or dW is as exact as without, a 16-bit one is off by 2^1/2 times its own rounding (what
-// adds up is the rounding of each of many terms).  In 32 bits they would be twice the bytes and three products for one.  (The padding is at least as long as what
+// adds up is the rounding of each of many terms).  In 32 bits they would be twice the bytes and three products for one.
+// Matrices to be copied for the products are copied by the launch's first workgroups.  (The padding is at least as long as what
 // a row's last eight reach over.)
 template <class T, int ACT>
 __global__ __launch_bounds__(256) void k_gate_grad(const size_t m, const size_t n, const T *__restrict__ dh, const size_t lddh,
                                                    const T *__restrict__ g, const T *__restrict__ u, T *__restrict__ dg,
-                                                   T *__restrict__ du, const size_t ld) {
+                                                   T *__restrict__ du, const size_t ld, const Packs<T> packs) {
+  if (blockIdx.x < packs.groups) return pack_group(packs, blockIdx.x);
   const size_t per = ld / 8;
-  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < m * per; i += (size_t)gridDim.x * 256) {
+  const unsigned group = blockIdx.x - packs.groups, groups = gridDim.x - packs.groups;
+  for (size_t i = (size_t)group * 256 + threadIdx.x; i < m * per; i += (size_t)groups * 256) {
     const size_t r = i / per, c = (i - r * per) * 8;
     T vh[8] = {}, vg[8] = {}, vu[8] = {}, og[8], ou[8];
     if (c + 8 <= n) {
@@ -742,35 +779,14 @@ __global__ __launch_bounds__(256) void k_gate_grad(const size_t m, const size_t 
 }
 template <class T>
 void gate_grad(hipStream_t s, size_t m, size_t n, int act, const void *dh, size_t lddh, const void *g, const void *u, T *dg, T *du,
-               size_t ld) {
+               size_t ld, const Packs<T> &packs) {
   const size_t threads = m * (ld / 8);
   const unsigned grid = (unsigned)((threads + 255) / 256 < 65536 ? (threads + 255) / 256 : 65536);
   const auto go = [&](auto a) {
-    k_gate_grad<T, decltype(a)::value><<<grid, 256, 0, s>>>(m, n, (const T *)dh, lddh, (const T *)g, (const T *)u, dg, du, ld);
+    k_gate_grad<T, decltype(a)::value><<<packs.groups + grid, 256, 0, s>>>(m, n, (const T *)dh, lddh, (const T *)g, (const T *)u, dg, du, ld,
+                                                                               packs);
   };
   by_act(act, go);
-}
-
-// Matrices whose rows do not start at 16-byte boundaries, copied to ones whose rows do; the padding, and rows up to
-// rows_to, zeroed.  One of up to three by blockIdx.y.  Bound by memory: 101549 x 609 f16 49 us (5.0 TB/s)
-template <class T>
-struct Packs {
-  struct {
-    const T *p;
-    T *q;
-    size_t rows, cols, ld, to, rows_to;
-  } m[3];
-  unsigned n = 0;
-};
-template <class T>
-__global__ __launch_bounds__(256) void k_pack(const Packs<T> packs) {
-  constexpr int E = 16 / sizeof(T);
-  const auto &m = packs.m[blockIdx.y];
-  const size_t per = m.to / E;
-  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < m.rows_to * per; i += (size_t)gridDim.x * 256) {
-    const size_t r = i / per, c = (i - r * per) * E;
-    *(i4 *)(m.q + r * m.to + c) = fetch16(m.p, m.ld, r, m.rows, c, m.cols);
-  }
 }
 
 bool act_ok(int act) { return act >= QR_ACT_SILU && act <= QR_ACT_SIGMOID; }
@@ -795,18 +811,13 @@ bool in_place(const void *p, size_t ld, size_t cols, size_t e) {
 template <class T>
 void pack(Packs<T> &packs, size_t rows, size_t cols, const T *&p, size_t &ld, char *&ws, size_t rows_to) {
   const size_t to = padded(cols, sizeof(T));
-  packs.m[packs.n++] = {p, (T *)ws, rows, cols, ld, to, rows_to};
+  const unsigned groups = blocks(rows_to * to * sizeof(T) / 16);
+  packs.m[packs.n++] = {p, (T *)ws, rows, cols, ld, to, rows_to, groups};
+  packs.groups += groups;
   p = (const T *)ws;
   ld = to;
   ws += pack_bytes(rows_to, cols, sizeof(T));
 }
-template <class T>
-void launch_pack(hipStream_t s, const Packs<T> &packs) {
-  size_t most = 0;
-  for (unsigned i = 0; i < packs.n; ++i) most = std::max(most, packs.m[i].rows_to * packs.m[i].to * sizeof(T) / 16);
-  if (packs.n && most) k_pack<T><<<dim3(blocks(most), packs.n), 256, 0, s>>>(packs);
-}
-
 // Whether results go past the caches, so that they do not push the operands out.  Only in whole parts of 64 bytes, what
 // the memory writes at once (65536 x 256 x 1000 bf16, both products kept: 356 us past the caches, 174 through them).  Where
 // the three results are kept, the caches' 256 MB take some of them up: past the caches where the sums are long, or not short
@@ -988,7 +999,7 @@ extern "C" int qr_gated_ffn_async(int device, void *stream, int type, int act, s
       size_t ld = ldw;
       pack(packs, n, k, P.b[0], ld, ws, n), pack(packs, n, k, P.b[1], P.ldb, ws, n);
     }
-    launch_pack(s, packs);
+    if (packs.groups) k_pack<T><<<packs.groups, 256, 0, s>>>(packs);
     if (few(m, n)) launch_few(s, P);
     else gemm<T, FWD>(s, tile_forward(e, m, k, n, gate != nullptr), P);
   });
@@ -1042,7 +1053,6 @@ extern "C" int qr_gated_ffn_backward_async(int device, void *stream, int type, i
     const size_t ld = stages_of(n, e);
     T *const dg = (T *)ws, *const du = (T *)(ws + pack_bytes(m, ld, e));
     ws += 2 * pack_bytes(m, ld, e);
-    if (m) gate_grad<T>(s, m, n, act, dh, lddh, gate, up, dg, du, ld);
     const Plan px = plan_dx(e, m, k, n), pw = plan_dw(e, m, k, n);
     float *const part = (float *)ws;
     if (m) ws += std::max(part_bytes(px, m, k, 1), part_bytes(pw, n, k, 2));
@@ -1057,7 +1067,7 @@ extern "C" int qr_gated_ffn_backward_async(int device, void *stream, int type, i
       pack(packs, n, k, X.b[0], to, ws, ld), pack(packs, n, k, X.b[1], X.ldb, ws, ld);
     }
     if (dw_gate && m && !in_place(x, ldx, k, e)) pack(packs, m, k, W.b[0], W.ldb, ws, m);
-    launch_pack(s, packs);
+    if (m) gate_grad<T>(s, m, n, act, dh, lddh, gate, up, dg, du, ld, packs);
     if (dx && m) {
       X.splits = px.splits, X.steps = px.steps, X.part = px.splits > 1 ? part : nullptr;
       gemm<T, DX>(s, px.tile, X);
