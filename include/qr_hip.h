@@ -511,7 +511,7 @@ int qr_dropout_async(int device, void *hip_stream, int type, size_t rows, size_t
 /* gate / up: NULL (serving), or [m][n] contiguous: the two products, rounded to `type`,    */
 /* for the backward pass.  Outputs must not overlap each other or an input.  The workspace   */
 /* is used (NULL, 0 will do otherwise) where a row of x or of a weight does not start and end  */
-/* at 16-byte boundaries or lies more than 4 MB behind the one before: such matrices are       */
+/* at 16-byte boundaries or lies more than 4 MB behind the one before: such matrices may be    */
 /* copied.                                                                                    */
 int qr_gated_ffn_workspace(int type, size_t m, size_t k, size_t n, size_t *bytes);
 int qr_gated_ffn_async(int device, void *hip_stream, int type, int act, size_t m, size_t k, size_t n,

@@ -251,7 +251,7 @@ __device__ __forceinline__ uint32_t lds_offset(const char *p) { return (uint32_t
 // x 128 would not fit a compute unit, 160 KB; they do, and one's matrix instructions run under the other's waits, first
 // loads and epilogue.)  WN = 4, 256 x 256: one workgroup fills the compute unit; both operands are double-buffered and
 // pass no registers, and the next stage is sent for in the first half of this one.  The last, partial stage of a sum is
-// zero-filled.
+// zero-filled.  RAG (FWD, WN = 2): rows at any alignment, both operands through registers.
 //
 // What bounds it, 16-bit types: at 256 x 128 the way from L2 to the compute units (48 bytes a cycle and unit at the full
 // matrix rate, of 64), at 256 x 256 (32 bytes) the matrix cores at the clock that the card holds under them, 1.9 GHz.  1530
@@ -259,7 +259,7 @@ __device__ __forceinline__ uint32_t lds_offset(const char *p) { return (uint32_t
 // whose 16 stages leave a fifth of a tile's time to its first loads and its results (1020 TF with g and u stored too: 805
 // MB whose writing overlaps little).
 // f32: the six products and the splits before them, whose times add up (matrix cores 59 % busy): 190 to 200 TF.
-template <class T, Kind KIND, int TM, int TN, int WN>
+template <class T, Kind KIND, int TM, int TN, int WN, bool RAG>
 __global__ __launch_bounds__(128 * WN, 2) void k_gemm(const GemmArgs<T> P) {
   constexpr bool AKS = KIND == DW, BKS = KIND != FWD, BD = WN > 2;
   constexpr int WM = 2, NT = 128 * WN, KT = 128 / sizeof(T), E = 16 / sizeof(T);
@@ -337,8 +337,22 @@ __global__ __launch_bounds__(128 * WN, 2) void k_gemm(const GemmArgs<T> P) {
     sb += (BKS ? KT * P.ldb : (size_t)KT) * sizeof(T);
     if (KIND == DX && t + 1 == kt_all) sb = (const char *)(P.b[1] + c0);
   };
+  i4 va[RAG ? PA : 1], vb[PB];
   auto load_a = [&](const int d, const uint32_t to) { dma16(sa, offa[d], to + (d * NT + wave * 64) * 16); };
   auto dma_b = [&](const int d, const uint32_t to) { dma16(sb, offb[d], to + (d * NT + wave * 64) * 16); };
+  // A piece of a row at any alignment (RAG); in the partial stage one that lies across the sum's end is put together
+  auto ragged = [&](const char *p, const unsigned t, const int d) {
+    i4 v;
+    if (t < whole) {
+      typedef int loose __attribute__((ext_vector_type(4), aligned(2)));
+      v = *(const QR_GLB loose *)(const QR_GLB char *)p;
+    } else {
+      int r, k;
+      piece_of<T, TM, false>(d * NT + tid, r, k);
+      v = fetch16((const T *)p - k, 0, 0, 1, k, P.k - (size_t)t * KT);
+    }
+    return v;
+  };
   // The partial stage's: pieces inside the sum (none lies across its end) come as a whole stage's do, the others are zero
   auto inside = [&](const auto tile, const bool columns, const unsigned t, const int d) {
     int r, k;
@@ -362,18 +376,30 @@ __global__ __launch_bounds__(128 * WN, 2) void k_gemm(const GemmArgs<T> P) {
       else *(QR_LDS i4 *)(to + (d * NT + tid) * 16) = i4{0, 0, 0, 0};
     }
   };
-  i4 vb[PB];
   auto load_b = [&](const unsigned t) {
 #pragma unroll
     for (int d = 0; d < PB; ++d) {
-      vb[d] = i4{0, 0, 0, 0};
-      if (KIND == DX || t < whole || inside(tile_b, BKS, t, d)) vb[d] = *(const QR_GLB i4 *)((const QR_GLB char *)sb + offb[d]);
+      if constexpr (RAG) {
+        vb[d] = ragged(sb + offb[d], t, d);
+      } else {
+        vb[d] = i4{0, 0, 0, 0};
+        if (KIND == DX || t < whole || inside(tile_b, BKS, t, d)) vb[d] = *(const QR_GLB i4 *)((const QR_GLB char *)sb + offb[d]);
+      }
     }
     next_b(t);
   };
   auto keep_b = [&]() {
 #pragma unroll
     for (int d = 0; d < PB; ++d) *(i4 *)(lds + 2 * ABUF + (d * NT + tid) * 16) = vb[d];
+  };
+  auto ragged_a = [&](const unsigned t) {
+#pragma unroll
+    for (int d = 0; d < PA; ++d) va[d] = ragged(sa + offa[d], t, d);
+    next_a(t);
+  };
+  auto keep_a = [&](const uint32_t to) {
+#pragma unroll
+    for (int d = 0; d < PA; ++d) *(i4 *)(lds + to + (d * NT + tid) * 16) = va[d];
   };
 
   f4 acc[MI][NI];
@@ -401,7 +427,7 @@ __global__ __launch_bounds__(128 * WN, 2) void k_gemm(const GemmArgs<T> P) {
         if (m + 1 < MI) next[0] = read_a(ra, m + 1, 0), next[1] = read_a(ra, m + 1, 1);
         if constexpr (STEADY)
 #pragma unroll
-          for (int d = m * PA / MI; d < (m + 1) * PA / MI; ++d) load_a(d, to);
+          for (int d = m * PA / MI; d < (m + 1) * PA / MI && !RAG; ++d) load_a(d, to);
         constexpr int HI[6] = {1, 0, 2, 0, 1, 0}, LO[6] = {1, 2, 0, 1, 0, 0};  // the smallest first
 #pragma unroll
         for (int p = 0; p < 6; ++p)
@@ -425,7 +451,7 @@ __global__ __launch_bounds__(128 * WN, 2) void k_gemm(const GemmArgs<T> P) {
           for (int n = q * NI / MI; n < (q + 1) * NI / MI; ++n) fb[1][n] = read_b(n, 1);
         if constexpr (STEADY)
 #pragma unroll
-          for (int d = q * PA / ROWS; d < (q + 1) * PA / ROWS && d < PA; ++d) load_a(d, to);
+          for (int d = q * PA / ROWS; d < (q + 1) * PA / ROWS && d < PA && !RAG; ++d) load_a(d, to);
         if constexpr (STEADY && BD)
 #pragma unroll
           for (int d = q * PB / ROWS; d < (q + 1) * PB / ROWS && d < PB; ++d) dma_b(d, to_b);
@@ -437,7 +463,10 @@ __global__ __launch_bounds__(128 * WN, 2) void k_gemm(const GemmArgs<T> P) {
   };
   const uint32_t at_a = lds_offset(lds), at_b = at_a + 2 * ABUF;
   if (first < last) {
-    if (KIND == DX || first < whole) {
+    if (RAG) {
+      ragged_a(first);
+      keep_a(0);
+    } else if (KIND == DX || first < whole) {
 #pragma unroll
       for (int d = 0; d < PA; ++d) load_a(d, at_a);
       next_a(first);
@@ -459,9 +488,11 @@ __global__ __launch_bounds__(128 * WN, 2) void k_gemm(const GemmArgs<T> P) {
     for (; t + 1 < whole; ++t, cur ^= ABUF, cur_b ^= BBUF) {
       wait_all();
       barrier();  // stage t is there, and every wave is done with stage t - 1 where there are two buffers
+      if (RAG) ragged_a(t + 1);
       if (!BD) load_b(t + 1);
       compute(std::true_type{}, base_a + cur, base_b + cur_b, at_a + (cur ^ ABUF), at_b + (cur_b ^ BBUF));
-      next_a(t + 1);
+      if (RAG) keep_a(cur ^ ABUF);
+      else next_a(t + 1);
       if (BD) {
         next_b(t + 1);
       } else {
@@ -473,13 +504,17 @@ __global__ __launch_bounds__(128 * WN, 2) void k_gemm(const GemmArgs<T> P) {
       wait_all();
       barrier();
       if (t + 1 < last) {
-        part_a(t + 1, at_a + (cur ^ ABUF));
+        if (RAG) ragged_a(t + 1);
+        else part_a(t + 1, at_a + (cur ^ ABUF));
         if (BD) part_b(t + 1, at_b + (cur_b ^ BBUF));
         else load_b(t + 1);
       }
       compute(std::false_type{}, base_a + cur, base_b + cur_b, 0, 0);
       if (!BD || t + 1 == last) barrier();
-      if (!BD && t + 1 < last) keep_b();
+      if (!BD && t + 1 < last) {
+        if (RAG) keep_a(cur ^ ABUF);
+        keep_b();
+      }
     }
   }
 
@@ -831,13 +866,13 @@ bool streams(const GemmArgs<T> &P, const size_t outs) {
   return whole && (outs < 3 || sum >= 1024 || (sum >= 256 && bytes > ((size_t)256 << 20)));
 }
 
-template <class T, Kind KIND, int TM, int TN, int WN = 2>
+template <class T, Kind KIND, int TM, int TN, int WN = 2, bool RAG = false>
 void launch_gemm(hipStream_t s, GemmArgs<T> P) {
   P.row_tiles = tiles_of(P.rows, TM);
   P.stream = streams(P, KIND == FWD ? (P.o[1] ? 3 : 1) : KIND == DW ? 2 : 1);
   P.col_tiles = tiles_of(P.cols, KIND == FWD ? TN / 2 : TN);
   const unsigned tiles = P.row_tiles * P.col_tiles * (KIND == FWD ? 1 : (KIND == DW ? 2 : 1) * P.splits);
-  k_gemm<T, KIND, TM, TN, WN><<<(tiles + 7) / 8 * 8, 128 * WN, 0, s>>>(P);
+  k_gemm<T, KIND, TM, TN, WN, RAG><<<(tiles + 7) / 8 * 8, 128 * WN, 0, s>>>(P);
 }
 
 
@@ -946,6 +981,15 @@ size_t part_bytes(const Plan &p, size_t rows, size_t cols, size_t outs) {
   return p.splits > 1 ? round256(p.splits * outs * rows * cols * 4) : 0;
 }
 
+// Whether the forward pass reads rows off 16-byte boundaries as they lie, through registers, instead of copying them first:
+// where few tiles read a row again, or few tiles are made and a launch is what counts.  As they lie / copied, us a call:
+// 100000 x 601 x 64 bf16 45 / 64, 20000 x 1023 x 64 24 / 30, 1000 x 601 x 500 11 / 14, f32 100000 x 601 x 200 360 / 425;
+// but 4000 x 1023 x 4000 bf16 124 / 66, 100000 x 65 x 200 48 / 42, f32 20000 x 65 x 4000 240 / 222.
+bool as_they_lie(size_t e, size_t m, size_t n) {
+  const size_t cols = tiles_of(2 * n, 128);
+  return cols <= (e == 2 ? 2 : 8) || (size_t)tiles_of(m, 128) * cols <= 2 * CUS;
+}
+
 }  // namespace
 
 extern "C" int qr_gated_ffn_workspace(int type, size_t m, size_t k, size_t n, size_t *bytes) {
@@ -969,8 +1013,9 @@ extern "C" int qr_gated_ffn_async(int device, void *stream, int type, int act, s
   QR_DENSE_ARG(x && w_gate && w_up && h, "gated ffn: x, a weight or h is NULL");
   const size_t e = qr_dense_size(type);
   const bool px = !few(m, n) && !in_place(x, ldx, k, e), pw = !few(m, n) && (!in_place(w_gate, ldw, k, e) || !in_place(w_up, ldw, k, e));
+  const bool direct = (px || pw) && ldx * e <= ROW_BYTES && ldw * e <= ROW_BYTES && as_they_lie(e, m, n);
   size_t need = 0;
-  if (px || pw)
+  if (px || pw)  // (asked for by the rows alone, whichever way they are then read)
     if (int rc = qr_gated_ffn_workspace(type, m, k, n, &need)) return rc;
   QR_DENSE_ARG(!need || (workspace && workspace_bytes >= need),
                "gated ffn: rows that start or end off 16-byte boundaries or lie more than 4 MB apart need the workspace");
@@ -994,6 +1039,10 @@ extern "C" int qr_gated_ffn_async(int device, void *stream, int type, int act, s
     P.lda = ldx, P.ldb = ldw, P.rows = m, P.cols = n, P.k = k;
     P.o[0] = (T *)h, P.o[1] = (T *)gate, P.o[2] = (T *)up, P.ldo = ldh, P.act = act;
     Packs<T> packs;
+    if (direct) {
+      const Tile t = tile_of(e, m, 2 * n, 1, false);
+      return t.rows > 64 ? launch_gemm<T, FWD, 128, 128, 2, true>(s, P) : launch_gemm<T, FWD, 64, 64, 2, true>(s, P);
+    }
     if (px) pack(packs, m, k, P.a[0], P.lda, ws, m);
     if (pw) {
       size_t ld = ldw;

@@ -750,3 +750,14 @@ def test_dropout_seeds_of_numpy(dense):
     assert torch.equal(dense.dropout(x, 0.5, np.int64(-1)), dense.dropout(x, 0.5, 2 ** 64 - 1))
     with pytest.raises(dense.QrError):
         dense.dropout(x, 0.5, 7.0)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k,n", [(3000, 601, 64), (700, 65, 333), (2500, 129, 50), (300, 1023, 1000), (4100, 63, 4000), (9000, 8, 127),
+                                   (65, 5, 9000)])
+def test_ffn_rows_off_boundaries(dense, dtype, m, k, n):
+    """Odd rows, rows of whole pieces at odd strides and bases: read as they lie or copied, by the sizes."""
+    x, wg, wu = ffn_inputs(31, m, k, n, dtype)
+    ffn_forward_check(dense, dtype, "gelu_tanh", x, wg, wu,
+                      [(padded(x, 3), padded(wg, 5), padded(wu, 5)), (shifted(x, 1), shifted(wg, 3), shifted(wu, 2)),
+                       (x, padded(wg, 1), padded(wu, 1)), (padded(x, 1), wg, wu)])
