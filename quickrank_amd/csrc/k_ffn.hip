@@ -611,7 +611,7 @@ __global__ __launch_bounds__(128 * WN, 2) void k_gemm(const GemmArgs<T> P) {
 // The forward pass of few rows: bound by reading the weights once and by latency, so no tile is staged.  A workgroup
 // makes 16 columns of h for 16 MB rows; its eight waves share the sum over k in steps of 128 bytes, read straight into
 // fragments (any alignment: a lane takes 32 consecutive bytes of a row, in x and in the weights alike), and are joined in
-// LDS in a fixed order.  One row of k 1024, n 4096 bf16 (16.8 MB of weights) 5.2 us, 3.2 TB/s; 100 x 136 x 512 f32 4.0 us.
+// LDS in a fixed order.  One row of k 1024, n 4096 bf16 (16.8 MB of weights) 5.3 us, 3.2 TB/s; 100 x 136 x 512 f32 4.0 us.
 template <class T, int MB>
 __global__ __launch_bounds__(512) void k_few(const GemmArgs<T> P) {
   constexpr int W = 8, KT = 128 / sizeof(T), E = 16 / sizeof(T);
@@ -877,19 +877,22 @@ void launch_gemm(hipStream_t s, GemmArgs<T> P) {
 
 
 
-// Whether the forward pass takes the few-rows kernel: where tiles of 64 x 64 sums would leave half the compute units
-// without one, and up to one such tile of rows.  Few rows / tiles in us, back to back in a graph: k 1024, n 4096 bf16 1 row
-// 5.8 / 14.9, 64 9.8 / 14.6, 200 24 / 17; k 136, n 512 f32 100 rows 3.5 / 6.5, 512 5.8 / 6.7, 1000 8.3 / 7.0.
-bool few(size_t m, size_t n) {
-  return n < ((size_t)1 << 26) && (m <= 64 || (size_t)tiles_of(m, 64) * tiles_of(2 * n, 64) <= CUS / 2);
+// Whether the forward pass takes the few-rows kernel: where tiles of 64 x 64 sums would leave half the compute units (16-bit
+// types: three quarters) without one, and up to 64 (32) rows.  Few rows / tiles in us, back to back in a graph: k 1024, n
+// 4096 bf16 1 row 5.3 / 7.4, 32 7.0 / 7.7, 64 9.5 / 8.0, 200 25 / 10; k 2048, n 1024 bf16 100 rows 10.4 / 12.1, 200 14.4 /
+// 12.4; k 136, n 512 f32 100 rows 4.0 / 7.0, 512 6.5 / 7.1, 1000 9.0 / 7.6.
+bool few(size_t e, size_t m, size_t n) {
+  const size_t rows = e == 2 ? 32 : 64, tiles = e == 2 ? CUS / 4 : CUS / 2;
+  return n < ((size_t)1 << 26) && (m <= rows || (size_t)tiles_of(m, 64) * tiles_of(2 * n, 64) <= tiles);
 }
 
 template <class T>
 void launch_few(hipStream_t s, const GemmArgs<T> &P) {
   const unsigned cols = tiles_of(P.cols, 16);
-  // the most rows a workgroup that still leave every compute unit one
-  if (P.rows > 32 && (size_t)cols * tiles_of(P.rows, 64) >= CUS) k_few<T, 4><<<dim3(cols, tiles_of(P.rows, 64)), 512, 0, s>>>(P);
-  else if (P.rows > 16 && (size_t)cols * tiles_of(P.rows, 32) >= CUS) k_few<T, 2><<<dim3(cols, tiles_of(P.rows, 32)), 512, 0, s>>>(P);
+  // the most rows a workgroup that still leave every compute unit one (16-bit types: 64 rows never do)
+  if constexpr (sizeof(T) == 4)
+    if (P.rows > 32 && (size_t)cols * tiles_of(P.rows, 64) >= CUS) return k_few<T, 4><<<dim3(cols, tiles_of(P.rows, 64)), 512, 0, s>>>(P);
+  if (P.rows > 16 && (size_t)cols * tiles_of(P.rows, 32) >= CUS) k_few<T, 2><<<dim3(cols, tiles_of(P.rows, 32)), 512, 0, s>>>(P);
   else k_few<T, 1><<<dim3(cols, tiles_of(P.rows, 16)), 512, 0, s>>>(P);
 }
 
@@ -1012,14 +1015,14 @@ extern "C" int qr_gated_ffn_async(int device, void *stream, int type, int act, s
   if (!m) return QR_OK;
   QR_DENSE_ARG(x && w_gate && w_up && h, "gated ffn: x, a weight or h is NULL");
   const size_t e = qr_dense_size(type);
-  const bool px = !few(m, n) && !in_place(x, ldx, k, e), pw = !few(m, n) && (!in_place(w_gate, ldw, k, e) || !in_place(w_up, ldw, k, e));
+  const bool px = !few(e, m, n) && !in_place(x, ldx, k, e), pw = !few(e, m, n) && (!in_place(w_gate, ldw, k, e) || !in_place(w_up, ldw, k, e));
   const bool direct = (px || pw) && ldx * e <= ROW_BYTES && ldw * e <= ROW_BYTES && as_they_lie(e, m, n);
   size_t need = 0;
   if (px || pw)  // (asked for by the rows alone, whichever way they are then read)
     if (int rc = qr_gated_ffn_workspace(type, m, k, n, &need)) return rc;
   QR_DENSE_ARG(!need || (workspace && workspace_bytes >= need),
                "gated ffn: rows that start or end off 16-byte boundaries or lie more than 4 MB apart need the workspace");
-  if (!few(m, n) && k * e > ROW_BYTES) return qr_dense_fail(QR_ERR_UNSUPPORTED, "gated ffn: rows longer than 4 MB");
+  if (!few(e, m, n) && k * e > ROW_BYTES) return qr_dense_fail(QR_ERR_UNSUPPORTED, "gated ffn: rows longer than 4 MB");
   const void *out[4] = {h, gate, up, workspace};
   const size_t bytes[4] = {qr_dense_span(m, n, ldh, e), m * n * e, m * n * e, need};
   for (int i = 0; i < 4; ++i) {
@@ -1049,7 +1052,7 @@ extern "C" int qr_gated_ffn_async(int device, void *stream, int type, int act, s
       pack(packs, n, k, P.b[0], ld, ws, n), pack(packs, n, k, P.b[1], P.ldb, ws, n);
     }
     if (packs.groups) k_pack<T><<<packs.groups, 256, 0, s>>>(packs);
-    if (few(m, n)) launch_few(s, P);
+    if (few(e, m, n)) launch_few(s, P);
     else gemm<T, FWD>(s, tile_forward(e, m, k, n, gate != nullptr), P);
   });
   return qr_dense_launched("gated ffn");
