@@ -504,7 +504,8 @@ int qr_dropout_async(int device, void *hip_stream, int type, size_t rows, size_t
                      const void *residual, size_t ldr, void *y, size_t ldy, double p, uint64_t seed,
                      uint64_t offset, const uint64_t *counter);
 
-/* (Rows of x and the weights, and backward of h, up to 4 MB: QR_ERR_UNSUPPORTED beyond.)   */
+/* (Rows of x and the weights, and backward of h, up to 4 MB, up to 2^30 rows of x and 2^28   */
+/* of the weights: QR_ERR_UNSUPPORTED beyond.)                                                */
 /* f32 products: as exact as f32 sums are; an infinite factor gives NaN, numbers below        */
 /* 2^-110 lose bits.                                                                          */
 /* h [m][n] = act(x w_gate^T) * (x w_up^T); x [m][k], weights [n][k] of stride ldw.        */

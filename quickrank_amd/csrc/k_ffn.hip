@@ -836,6 +836,8 @@ unsigned blocks(size_t n) { return (unsigned)((n + 255) / 256 < 65536 ? (n + 255
 
 // longest row the product kernel takes: a tile's 256 rows lie within 2^31 bytes
 constexpr size_t ROW_BYTES = (size_t)1 << 22;
+// most rows and most outputs of a row: a launch has fewer than 2^32 threads
+constexpr size_t ROWS_MOST = (size_t)1 << 30, OUTS_MOST = (size_t)1 << 28;
 
 // whether the product kernel can read a matrix where it lies: rows of whole pieces of 16 bytes at 16-byte boundaries
 bool in_place(const void *p, size_t ld, size_t cols, size_t e) {
@@ -1022,6 +1024,7 @@ extern "C" int qr_gated_ffn_async(int device, void *stream, int type, int act, s
     if (int rc = qr_gated_ffn_workspace(type, m, k, n, &need)) return rc;
   QR_DENSE_ARG(!need || (workspace && workspace_bytes >= need),
                "gated ffn: rows that start or end off 16-byte boundaries or lie more than 4 MB apart need the workspace");
+  if (m > ROWS_MOST || n > OUTS_MOST) return qr_dense_fail(QR_ERR_UNSUPPORTED, "gated ffn: more than 2^30 rows or 2^28 outputs");
   if (!few(e, m, n) && k * e > ROW_BYTES) return qr_dense_fail(QR_ERR_UNSUPPORTED, "gated ffn: rows longer than 4 MB");
   const void *out[4] = {h, gate, up, workspace};
   const size_t bytes[4] = {qr_dense_span(m, n, ldh, e), m * n * e, m * n * e, need};
@@ -1087,6 +1090,7 @@ extern "C" int qr_gated_ffn_backward_async(int device, void *stream, int type, i
   if (int rc = qr_gated_ffn_backward_workspace(type, m, k, n, &need)) return rc;
   QR_DENSE_ARG(!need || (workspace && workspace_bytes >= need), "gated ffn backward: the workspace is too small");
   const size_t e = qr_dense_size(type);
+  if (m > ROWS_MOST) return qr_dense_fail(QR_ERR_UNSUPPORTED, "gated ffn backward: more than 2^30 rows");
   if (k * e > ROW_BYTES || stages_of(n, e) * e > ROW_BYTES)
     return qr_dense_fail(QR_ERR_UNSUPPORTED, "gated ffn backward: rows longer than 4 MB");
   const void *out[4] = {dx, dw_gate, dw_up, workspace}, *in[6] = {dh, x, w_gate, w_up, gate, up};

@@ -430,6 +430,13 @@ size_t parts_of(size_t rows, int lanes, int pieces) {
   const size_t most = lanes > 256 ? 512 : pieces > 1 ? 1024 : 1536;
   return rows < most ? rows : most;
 }
+// ... of rows that no registers hold: as many as give 2^21 threads a share of a column, up to 512
+size_t parts_any(size_t rows, size_t cols) {
+  const size_t most = std::max<size_t>(std::min<size_t>(((size_t)1 << 21) / cols, 512), 1);
+  return rows < most ? rows : most;
+}
+// columns that the registers of a workgroup hold at most, of any type
+constexpr size_t COLS_HELD = 16384;
 // Up to this many rows a workgroup takes at a time, one workgroup takes them all and no join follows: a second launch
 // costs more than the rows one after the other.
 constexpr size_t ALONE = 4;
@@ -477,7 +484,7 @@ extern "C" int qr_layer_norm_async(int device, void *stream, int type, int param
 
 extern "C" int qr_layer_norm_backward_workspace(size_t rows, size_t cols, size_t *bytes) {
   QR_DENSE_ARG(bytes && cols > 0 && cols <= COLS_MOST, "layer norm backward: bad size");
-  *bytes = parts_of(rows, 1, 1) * 2 * cols * 4;
+  *bytes = (cols <= COLS_HELD ? parts_of(rows, 1, 1) : parts_any(rows, cols)) * 2 * cols * 4;
   return QR_OK;
 }
 
@@ -500,7 +507,7 @@ extern "C" int qr_layer_norm_backward_async(int device, void *stream, int type, 
   if (!rows && !sums) return QR_OK;
   QR_DENSE_DEVICE(device);
   const hipStream_t s = (hipStream_t)stream;
-  const unsigned any = (unsigned)parts_of(rows, 1024, 1);
+  const unsigned any = (unsigned)parts_any(rows, cols);
   qr_dense_dispatch(type, [&](auto t) {
     using T = decltype(t);
     auto go = [&](auto p) {

@@ -137,3 +137,18 @@ def test_python_refuses_host_tensors():
         with pytest.raises(QrError) as e:
             call()
         assert e.value.code == ARG
+
+
+def test_ffn_of_more_rows_or_outputs_than_a_launch_has_threads_for_is_unsupported(L):
+    big = 1 << 52
+    assert ffn(L, m=(1 << 30) + 1, h=big) == 5 and "2^30 rows" in message(L)
+    n = (1 << 28) + 1
+    assert ffn(L, m=100, n=n, ldh=n, wg=1 << 50, wu=1 << 51, h=big) == 5 and "2^28 outputs" in message(L)
+    assert ffn_back(L, m=(1 << 30) + 1, ws=big, nbytes=1 << 50) == 5 and "2^30 rows" in message(L)
+
+
+def test_norm_workspace_of_long_rows_stays_small(L):
+    n = C.c_size_t()
+    for cols in (16385, 100_000, 1 << 24):
+        assert L.qr_layer_norm_backward_workspace(1 << 20, cols, C.byref(n)) == 0
+        assert 2 * cols * 4 <= n.value <= 2 * max(cols, 1 << 21) * 4

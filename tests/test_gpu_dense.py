@@ -761,3 +761,9 @@ def test_ffn_rows_off_boundaries(dense, dtype, m, k, n):
     ffn_forward_check(dense, dtype, "gelu_tanh", x, wg, wu,
                       [(padded(x, 3), padded(wg, 5), padded(wu, 5)), (shifted(x, 1), shifted(wg, 3), shifted(wu, 2)),
                        (x, padded(wg, 1), padded(wu, 1)), (padded(x, 1), wg, wu)])
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("rows,cols", [(700, 8200), (600, 16400), (300, 40_001), (3, 2_100_000)])
+def test_norm_backward_of_rows_that_no_registers_hold(dense, dtype, rows, cols):
+    norm_grad_check(dense, dtype, dtype, rows, cols)
