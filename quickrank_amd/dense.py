@@ -177,10 +177,11 @@ def dropout_words(x):
 def _weights(x, k, w_gate, w_up, device):
     _check(w_gate, "w_gate", device)
     _check(w_up, "w_up", device)
-    shape, stride = w_gate.shape, w_gate.stride()
+    shape, stride, other = w_gate.shape, w_gate.stride(), w_up.stride()
     if len(shape) != 2 or shape[1] != k or w_gate.dtype != x.dtype or (stride[1] != 1 and k > 1):
         _refuse("w_gate is a matrix of contiguous rows, [n][columns of x], of the type of x")
-    if w_up.shape != shape or w_up.dtype != x.dtype or (w_up.stride() != stride and shape[0] > 1 and k > 1):
+    # (the kernels read both by one row stride; the stride of a dimension of one element is not read)
+    if w_up.shape != shape or w_up.dtype != x.dtype or (other[1] != 1 and k > 1) or (other[0] != stride[0] and shape[0] > 1):
         _refuse("w_up differs from w_gate in shape, stride or type")
     if k == 0 or shape[0] == 0:
         _refuse("gated ffn: no columns")

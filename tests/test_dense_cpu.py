@@ -152,3 +152,30 @@ def test_norm_workspace_of_long_rows_stays_small(L):
     for cols in (16385, 100_000, 1 << 24):
         assert L.qr_layer_norm_backward_workspace(1 << 20, cols, C.byref(n)) == 0
         assert 2 * cols * 4 <= n.value <= 2 * max(cols, 1 << 21) * 4
+
+
+def _laid_out(n, k, sn, sk):
+    return torch.zeros(n * max(sn, 1) + k * max(sk, 1)).as_strided((n, k), (sn, sk))
+
+
+@pytest.mark.parametrize("n,k,gate,up", [
+    (50, 1, (64, 1), (1, 1)), (50, 1, (1, 1), (64, 1)), (50, 1, (64, 1), (64 * 2, 64)), (50, 1, (0, 1), (1, 1)),  # one feature
+    (1, 8, (8, 1), (1, 2)), (1, 8, (1, 1), (1, 50)), (1, 8, (8, 2), (8, 1)),                                      # one unit
+    (5, 8, (8, 1), (9, 1)), (5, 8, (8, 1), (8, 2)), (5, 8, (8, 1), (0, 1)), (5, 8, (1, 5), (1, 5))])
+def test_weights_of_two_layouts_are_refused(monkeypatch, n, k, gate, up):
+    """Both weights are read by w_gate's row stride and in contiguous rows, also where a matrix has one row or one column."""
+    from quickrank_amd import QrError, dense
+    monkeypatch.setattr(dense, "_check", lambda t, what, device=None: 0)
+    with pytest.raises(QrError) as e:
+        dense._weights(torch.zeros(3, k), k, _laid_out(n, k, *gate), _laid_out(n, k, *up), 0)
+    assert e.value.code == ARG and "w_" in str(e.value)
+
+
+@pytest.mark.parametrize("n,k,gate,up,ldw", [
+    (50, 1, (64, 1), (64, 1), 64), (50, 1, (64, 7), (64, 1), 64), (50, 1, (0, 1), (0, 1), 0), (1, 8, (8, 1), (99, 1), 8),
+    (1, 1, (5, 3), (2, 9), 1), (5, 8, (11, 1), (11, 1), 11), (5, 8, (0, 1), (0, 1), 0)])
+def test_weights_of_one_layout(monkeypatch, n, k, gate, up, ldw):
+    """Strides of a dimension of one element say nothing about where its element lies."""
+    from quickrank_amd import dense
+    monkeypatch.setattr(dense, "_check", lambda t, what, device=None: 0)
+    assert dense._weights(torch.zeros(3, k), k, _laid_out(n, k, *gate), _laid_out(n, k, *up), 0) == (n, ldw)

@@ -767,3 +767,23 @@ def test_ffn_rows_off_boundaries(dense, dtype, m, k, n):
 @pytest.mark.parametrize("rows,cols", [(700, 8200), (600, 16400), (300, 40_001), (3, 2_100_000)])
 def test_norm_backward_of_rows_that_no_registers_hold(dense, dtype, rows, cols):
     norm_grad_check(dense, dtype, dtype, rows, cols)
+
+
+def test_ffn_of_one_feature_or_one_unit_and_views(dense):
+    """One column of wider weights, one row: both weights of one layout are read as they lie, others are refused."""
+    from quickrank_amd import QrError
+    x, dh = rand(1, 40, 1), rand(2, 40, 50)
+    wide = rand(3, 2, 50, 64)
+    wg, wu = wide[0][:, 5:6], wide[1][:, 5:6]
+    want = dense.gated_ffn(x, wg.contiguous(), wu.contiguous(), save=True)
+    got = dense.gated_ffn(x, wg, wu, save=True)
+    assert all(torch.equal(p, q) for p, q in zip(got, want))
+    back = [dense.gated_ffn_backward(dh, x, *w, *want[1:]) for w in ((wg, wu), (wg.contiguous(), wu.contiguous()))]
+    assert all(torch.equal(p, q) for p, q in zip(*back))
+    row = rand(4, 8, 2)
+    y, dh1 = rand(5, 40, 8), rand(6, 40, 1)
+    bad = [(x, wg, wu.contiguous(), dh), (x, wg.contiguous(), wu, dh), (y, row.t()[:1].contiguous(), row.t()[:1], dh1)]
+    for v, a, b, d in bad:
+        for call in (lambda: dense.gated_ffn(v, a, b), lambda: dense.gated_ffn_backward(d, v, a, b, d, d)):
+            with pytest.raises(QrError):
+                call()
