@@ -519,7 +519,10 @@ int qr_gated_ffn_async(int device, void *hip_stream, int type, int act, size_t m
                        const void *x, size_t ldx, const void *w_gate, const void *w_up, size_t ldw, void *h,
                        size_t ldh, void *gate, void *up, void *workspace, size_t workspace_bytes);
 /* dx [m][k] (NULL = skip), dw_gate, dw_up [n][k] contiguous (both or neither).  The         */
-/* gradients of the two products pass through the workspace rounded to `type`.               */
+/* gradients of the two products pass through the workspace rounded to `type`: a 16-bit       */
+/* result is off by some 2^1/2 times its own rounding.  f16: they are held times a power of    */
+/* two made from the call's largest finite one, so that none leaves f16's range: each keeps    */
+/* 11 bits, or 2^-39 of the largest.                                                           */
 int qr_gated_ffn_backward_workspace(int type, size_t m, size_t k, size_t n, size_t *bytes);
 int qr_gated_ffn_backward_async(int device, void *hip_stream, int type, int act, size_t m, size_t k, size_t n,
                                 const void *dh, size_t lddh, const void *x, size_t ldx, const void *w_gate,

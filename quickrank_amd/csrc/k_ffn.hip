@@ -225,6 +225,7 @@ struct GemmArgs {
   size_t rows, cols, k;  // outputs (FWD: of h; DW: of one dW), length of one sum (DX: of each of its two, whole stages)
   T *o[3];               // FWD: h, g, u.  DX: dx.  DW: dWg, dWu
   float *part;           // partial sums, DX [split][rows][cols], DW [split][2][rows][cols], where the sums are split
+  const float *back;     // f16 DX, DW: what the sums are multiplied by (dg and du are held times its reciprocal), or NULL
   size_t ldo;
   int act;
   bool stream;           // results go past the caches
@@ -600,6 +601,11 @@ __global__ __launch_bounds__(128 * WN, 2) void k_gemm(const GemmArgs<T> P) {
         }
       } else {
         take(s * 2, v);
+        if constexpr (__is_same(T, _Float16)) {
+          const float back = P.back ? *P.back : 1.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] *= back;
+        }
         if (P.part) store(stream, P.part + ((size_t)(split * OUTS + z) * P.rows + row) * P.cols, v, col, P.cols);
         else store(stream, P.o[z] + row * P.ldo, v, col, P.cols);
       }
@@ -775,6 +781,66 @@ __global__ __launch_bounds__(256) void k_pack(const Packs<T> packs) {
   pack_group(packs, blockIdx.x);
 }
 
+// Eight neighbours of dg and du, from column c of row r on; behind the row's end zeros
+template <class T, int ACT>
+__device__ __forceinline__ void gate_piece(const size_t n, const T *__restrict__ dh, const size_t lddh, const T *__restrict__ g,
+                                           const T *__restrict__ u, const size_t r, const size_t c, float (&dg)[8], float (&du)[8]) {
+  T vh[8] = {}, vg[8] = {}, vu[8] = {};
+  if (c + 8 <= n) {
+    __builtin_memcpy(vh, dh + r * lddh + c, sizeof vh);
+    __builtin_memcpy(vg, g + r * n + c, sizeof vg);
+    __builtin_memcpy(vu, u + r * n + c, sizeof vu);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e)
+      if (c + e < n) vh[e] = dh[r * lddh + c + e], vg[e] = g[r * n + c + e], vu[e] = u[r * n + c + e];
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    float a, d;
+    act_of(ACT, (float)vg[e], a, d);
+    const float v = (float)vh[e];
+    dg[e] = v * (float)vu[e] * d;
+    du[e] = v * a;
+  }
+}
+
+// f16 has five bits of exponent: gradients of the products below 2^-14 would lose bits and those above 65504 become infinite,
+// though dx and dW are well inside.  So dg and du are held times a power of two that brings the largest finite one of both to
+// 2^14 .. 2^15 (one scale, for dx adds up products of both), and the products' sums are multiplied by its reciprocal: an
+// element keeps f16's 11 bits, or 2^-39 of the call's largest.  The largest is found first, by a launch that reads what the
+// gate gradient reads, the part of a workgroup to a place of its own; every workgroup of the gate gradient takes the largest of
+// those.  Bound by memory: with it 16384 x 1024 x 4096 takes 666 us (without 578), 100000 x 136 x 512 310 (253), 300 x 136 x
+// 512 27 (25).  (Read backwards by the gate gradient, for what the caches still hold, or by twice the workgroups: the same.)
+constexpr unsigned MAXIMA = 1024;  // workgroups of that launch at most
+__device__ __forceinline__ float block_max(float v) {  // of 256 threads, none of them negative, in every thread
+  __shared__ float lds[4];
+#pragma unroll
+  for (int s = 1; s < 64; s *= 2) v = fmaxf(v, __shfl_xor(v, s));
+  if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+  __syncthreads();
+  return fmaxf(fmaxf(lds[0], lds[1]), fmaxf(lds[2], lds[3]));
+}
+template <class T, int ACT>
+__global__ __launch_bounds__(256) void k_gate_max(const size_t m, const size_t n, const T *__restrict__ dh, const size_t lddh,
+                                                  const T *__restrict__ g, const T *__restrict__ u, float *__restrict__ maxima) {
+  const size_t per = (n + 7) / 8;
+  float most = 0.f;
+  for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < m * per; i += (size_t)gridDim.x * 256) {
+    const size_t r = i / per;
+    float dg[8], du[8];
+    gate_piece<T, ACT>(n, dh, lddh, g, u, r, (i - r * per) * 8, dg, du);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float a = fabsf(dg[e]), b = fabsf(du[e]);
+      most = a < INFINITY ? fmaxf(most, a) : most;  // (false for NaN)
+      most = b < INFINITY ? fmaxf(most, b) : most;
+    }
+  }
+  most = block_max(most);
+  if (threadIdx.x == 0) maxima[blockIdx.x] = most;
+}
+
 // dg, du in rows of stride ld, their padding zeroed; eight elements a thread.  Bound by memory: five matrices, 16384 x 4096
 // bf16 111 us, 100000 x 512 f32 168 us (6.1 TB/s, some of it from the caches).  They are rounded to T so that the products
 // take them as they are: an f32 dx or dW is as exact as without, a 16-bit one is off by 2^1/2 times its own rounding (what
@@ -784,42 +850,43 @@ __global__ __launch_bounds__(256) void k_pack(const Packs<T> packs) {
 template <class T, int ACT>
 __global__ __launch_bounds__(256) void k_gate_grad(const size_t m, const size_t n, const T *__restrict__ dh, const size_t lddh,
                                                    const T *__restrict__ g, const T *__restrict__ u, T *__restrict__ dg,
-                                                   T *__restrict__ du, const size_t ld, const Packs<T> packs) {
+                                                   T *__restrict__ du, const size_t ld, const Packs<T> packs,
+                                                   const float *__restrict__ maxima, const unsigned parts, float *__restrict__ back) {
   if (blockIdx.x < packs.groups) return pack_group(packs, blockIdx.x);
   const size_t per = ld / 8;
   const unsigned group = blockIdx.x - packs.groups, groups = gridDim.x - packs.groups;
+  float scale = 1.f;
+  if constexpr (__is_same(T, _Float16)) {
+    float most = 0.f;
+    for (unsigned p = threadIdx.x; p < parts; p += 256) most = fmaxf(most, maxima[p]);
+    // 2^(14 - the exponent), between 2^-100 and 2^100
+    const int e = 268 - (int)(__builtin_bit_cast(uint32_t, block_max(most)) >> 23), bits = e < 27 ? 27 : e > 227 ? 227 : e;
+    scale = __builtin_bit_cast(float, bits << 23);
+    if (group == 0 && threadIdx.x == 0) *back = __builtin_bit_cast(float, (254 - bits) << 23);
+  }
   for (size_t i = (size_t)group * 256 + threadIdx.x; i < m * per; i += (size_t)groups * 256) {
     const size_t r = i / per, c = (i - r * per) * 8;
-    T vh[8] = {}, vg[8] = {}, vu[8] = {}, og[8], ou[8];
-    if (c + 8 <= n) {
-      __builtin_memcpy(vh, dh + r * lddh + c, sizeof vh);
-      __builtin_memcpy(vg, g + r * n + c, sizeof vg);
-      __builtin_memcpy(vu, u + r * n + c, sizeof vu);
-    } else {
+    float vg[8], vu[8];
+    T og[8], ou[8];
+    gate_piece<T, ACT>(n, dh, lddh, g, u, r, c, vg, vu);
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
-        if (c + e < n) vh[e] = dh[r * lddh + c + e], vg[e] = g[r * n + c + e], vu[e] = u[r * n + c + e];
-    }
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      float a, d;
-      act_of(ACT, (float)vg[e], a, d);
-      const float v = (float)vh[e];
-      og[e] = (T)(v * (float)vu[e] * d);
-      ou[e] = (T)(v * a);
-    }
+    for (int e = 0; e < 8; ++e) og[e] = (T)(vg[e] * scale), ou[e] = (T)(vu[e] * scale);
     __builtin_memcpy(dg + r * ld + c, og, sizeof og);
     __builtin_memcpy(du + r * ld + c, ou, sizeof ou);
   }
 }
+// maxima, back: f16 only, MAXIMA floats and one
 template <class T>
 void gate_grad(hipStream_t s, size_t m, size_t n, int act, const void *dh, size_t lddh, const void *g, const void *u, T *dg, T *du,
-               size_t ld, const Packs<T> &packs) {
-  const size_t threads = m * (ld / 8);
-  const unsigned grid = (unsigned)((threads + 255) / 256 < 65536 ? (threads + 255) / 256 : 65536);
+               size_t ld, const Packs<T> &packs, float *maxima, float *back) {
+  const auto groups = [](size_t threads, size_t most) { return (unsigned)std::min((threads + 255) / 256, most); };
+  constexpr bool scaled = __is_same(T, _Float16);
+  const unsigned grid = groups(m * (ld / 8), scaled ? 4096 : 65536), parts = scaled ? groups(m * ((n + 7) / 8), MAXIMA) : 0;
   const auto go = [&](auto a) {
-    k_gate_grad<T, decltype(a)::value><<<packs.groups + grid, 256, 0, s>>>(m, n, (const T *)dh, lddh, (const T *)g, (const T *)u, dg, du, ld,
-                                                                               packs);
+    constexpr int ACT = decltype(a)::value;
+    if constexpr (scaled) k_gate_max<T, ACT><<<parts, 256, 0, s>>>(m, n, (const T *)dh, lddh, (const T *)g, (const T *)u, maxima);
+    k_gate_grad<T, ACT><<<packs.groups + grid, 256, 0, s>>>(m, n, (const T *)dh, lddh, (const T *)g, (const T *)u, dg, du, ld, packs, maxima,
+                                                            parts, back);
   };
   by_act(act, go);
 }
@@ -832,6 +899,8 @@ size_t padded(size_t cols, size_t e) { return (cols + 16 / e - 1) / (16 / e) * (
 // the length of one of DX's two sums, in whole stages
 size_t stages_of(size_t n, size_t e) { return (n + 128 / e - 1) / (128 / e) * (128 / e); }
 size_t pack_bytes(size_t rows, size_t cols, size_t e) { return round256(rows * padded(cols, e) * e); }
+// f16: the workgroups' largest gradients and what the products are multiplied by
+size_t scale_bytes(int type) { return type == QR_F16 ? round256((MAXIMA + 1) * 4) : 0; }
 unsigned blocks(size_t n) { return (unsigned)((n + 255) / 256 < 65536 ? (n + 255) / 256 : 65536); }
 
 // longest row the product kernel takes: a tile's 256 rows lie within 2^31 bytes
@@ -1065,9 +1134,9 @@ extern "C" int qr_gated_ffn_backward_workspace(int type, size_t m, size_t k, siz
   QR_DENSE_ARG(bytes && qr_dense_type_ok(type) && k > 0 && n > 0 && qr_dense_fits(m, n, n) && qr_dense_fits(m, k, k) && qr_dense_fits(n, k, k),
                "gated ffn backward: bad size");
   const size_t e = qr_dense_size(type);
-  // dg, du, the partial sums (dx is made before the weights' gradients), copies of x and the weights where their rows are
-  // not aligned
-  *bytes = m ? 2 * pack_bytes(m, stages_of(n, e), e) +
+  // the scale, dg, du, the partial sums (dx is made before the weights' gradients), copies of x and the weights where their
+  // rows are not aligned
+  *bytes = m ? scale_bytes(type) + 2 * pack_bytes(m, stages_of(n, e), e) +
                    std::max(part_bytes(plan_dx(e, m, k, n), m, k, 1), part_bytes(plan_dw(e, m, k, n), n, k, 2)) + pack_bytes(m, k, e) +
                    2 * pack_bytes(stages_of(n, e), k, e) + 256
              : 0;
@@ -1107,6 +1176,8 @@ extern "C" int qr_gated_ffn_backward_async(int device, void *stream, int type, i
     using T = decltype(t);
     char *ws = (char *)(((uintptr_t)workspace + 255) & ~(uintptr_t)255);
     const size_t ld = stages_of(n, e);
+    float *const maxima = (float *)ws, *const back = maxima + MAXIMA;
+    if (m) ws += scale_bytes(type);
     T *const dg = (T *)ws, *const du = (T *)(ws + pack_bytes(m, ld, e));
     ws += 2 * pack_bytes(m, ld, e);
     const Plan px = plan_dx(e, m, k, n), pw = plan_dw(e, m, k, n);
@@ -1123,7 +1194,8 @@ extern "C" int qr_gated_ffn_backward_async(int device, void *stream, int type, i
       pack(packs, n, k, X.b[0], to, ws, ld), pack(packs, n, k, X.b[1], X.ldb, ws, ld);
     }
     if (dw_gate && m && !in_place(x, ldx, k, e)) pack(packs, m, k, W.b[0], W.ldb, ws, m);
-    if (m) gate_grad<T>(s, m, n, act, dh, lddh, gate, up, dg, du, ld, packs);
+    if (m) gate_grad<T>(s, m, n, act, dh, lddh, gate, up, dg, du, ld, packs, maxima, back);
+    X.back = W.back = m && scale_bytes(type) ? back : nullptr;
     if (dx && m) {
       X.splits = px.splits, X.steps = px.steps, X.part = px.splits > 1 ? part : nullptr;
       gemm<T, DX>(s, px.tile, X);

@@ -787,3 +787,83 @@ def test_ffn_of_one_feature_or_one_unit_and_views(dense):
         for call in (lambda: dense.gated_ffn(v, a, b), lambda: dense.gated_ffn_backward(d, v, a, b, d, d)):
             with pytest.raises(QrError):
                 call()
+
+
+# (m, k, n; scales of dh, x, the weights, gate, up): the gradients of the products lie far below f16's normal numbers or above
+# its largest, the results do not
+F16_RANGE = [(0, 2.0 ** -20, 2.0 ** 8, 2.0 ** -8, 1.0, 1.0), (1, 2.0 ** -20, 2.0 ** -8, 2.0 ** 8, 1.0, 1.0),
+             (2, 2.0 ** -23, 2.0 ** 10, 2.0 ** -3, 1.0, 2.0 ** -6), (3, 300.0, 2.0 ** -12, 2.0 ** -12, 4.0, 400.0),
+             (4, 2.0 ** 13, 2.0 ** -14, 2.0 ** -14, 2.0 ** 6, 2.0 ** -8)]
+
+
+def f16_gradient(dh, x, wg, wu, g, u, act="silu"):
+    """The gradients in 64 bits and what rounding dg and du once, to 11 bits or 2^-39 of the largest, and one rounding of the
+    result may do to them."""
+    dh, x, wg, wu, g, u = (t.double() for t in (dh, x, wg, wu, g, u))
+    a, d = act64(act, g)
+    dg, du = dh * u * d, dh * a
+    te = ACT_STEPS * U32 * (1 + g.abs())
+    big = max(float(dg.abs().max()), float(du.abs().max()))
+    tg, tu = (2.0 ** -11 * 1.01 * v.abs() + te * w.abs() + 4 * U32 * v.abs() + 2.0 ** -39 * big for v, w in ((dg, dh * u), (du, dh)))
+    m, n = dh.shape
+    dx = dg @ wg + du @ wu
+    tx = tg @ wg.abs() + tu @ wu.abs() + 2 * U32 * (2 * n + 8) * (dg.abs() @ wg.abs() + du.abs() @ wu.abs())
+    dw = [v.T @ x for v in (dg, du)]
+    tw = [t.T @ x.abs() + 2 * U32 * (m + 8) * (v.abs().T @ x.abs()) for t, v in ((tg, dg), (tu, du))]
+    return (dx, *dw), (tx, *tw)
+
+
+@pytest.mark.parametrize("m,k,n", [(20000, 64, 32), (70, 33, 31), (3000, 136, 512), (2048, 2040, 1032)])
+@pytest.mark.parametrize("number,sdh,sx,sw,sg,su", F16_RANGE)
+def test_ffn_backward_of_f16_keeps_what_f16_cannot_hold(dense, m, k, n, number, sdh, sx, sw, sg, su):
+    t = torch.float16
+    x, wg, wu = rand(1, m, k, dtype=t, scale=sx), rand(2, n, k, dtype=t, scale=sw), rand(3, n, k, dtype=t, scale=sw)
+    dh, g, u = rand(4, m, n, dtype=t, scale=sdh), rand(5, m, n, dtype=t, scale=sg), rand(6, m, n, dtype=t, scale=su)
+    want, tol = f16_gradient(dh, x, wg, wu, g, u)
+    got = dense.gated_ffn_backward(dh, x, wg, wu, g, u)
+    for i, what in enumerate(("dx", "dw_gate", "dw_up")):
+        assert want[i].abs().max() < 60000
+        close(got[i], want[i], tol[i], t, what)
+        # as a whole: two roundings of 2^-11 / 3^1/2 each where the results are normal numbers, within 2 of that
+        normal = want[i].abs() > 2.0 ** -14
+        if normal.double().mean() > 0.5:
+            e = (got[i].double() - want[i])[normal].norm() / want[i][normal].norm()
+            assert e < 2 * 2 ** 0.5 * 2.0 ** -11 / 3 ** 0.5, (what, float(e))
+
+
+def test_ffn_backward_of_f16_with_broken_and_zero_gradients(dense):
+    """The scale comes from the finite numbers: what is not finite stays in its row and column, and zeros stay zeros."""
+    t, m, k, n = torch.float16, 600, 72, 96
+    x, wg, wu = ffn_inputs(1, m, k, n, t)
+    g, u, dh = rand(2, m, n, dtype=t), rand(3, m, n, dtype=t), rand(4, m, n, dtype=t, scale=1e-5)
+    ref = dense.gated_ffn_backward(dh, x, wg, wu, g, u)
+    bad = dh.clone()
+    bad[17, 5], bad[400, 90] = float("inf"), float("nan")
+    got = dense.gated_ffn_backward(bad, x, wg, wu, g, u)
+    rows, cols = torch.ones(m, dtype=torch.bool), torch.ones(n, dtype=torch.bool)
+    rows[[17, 400]], cols[[5, 90]] = False, False
+    assert torch.equal(got[0][rows], ref[0][rows]) and not torch.isfinite(got[0][~rows]).any()
+    for p, q in zip(got[1:], ref[1:]):
+        assert torch.equal(p[cols], q[cols]) and not torch.isfinite(p[~cols]).any()
+    none = dense.gated_ffn_backward(torch.zeros_like(dh), x, wg, wu, g, u)
+    assert not any(v.any() for v in none)
+
+
+def test_ffn_backward_of_f16_captured(dense):
+    """Replayed on gradients of other sizes, each time among eager work: the scale is made anew."""
+    t = torch.float16
+    x, wg, wu = ffn_inputs(1, 900, 136, 200, t)
+    _, g, u = dense.gated_ffn(x, wg, wu, save=True)
+    base, dh = rand(4, 900, 200), torch.zeros(900, 200, dtype=t, device="cuda")
+    dense.gated_ffn_backward(dh, x, wg, wu, g, u)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = dense.gated_ffn_backward(dh, x, wg, wu, g, u)
+    for scale in (1.0, 2.0 ** -18, 2.0 ** 9, 0.0, 2.0 ** -3):
+        dh.copy_(base * scale)
+        want = [v.clone() for v in dense.gated_ffn_backward(dh, x, wg, wu, g, u)]
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, want)), scale
