@@ -30,9 +30,11 @@ __device__ __forceinline__ void act_of(const int act, const float g, float &a, f
     // one step of f32, the product in exp2's argument to |g| steps
     const float c2 = 1.5957691216057308f, z = act == QR_ACT_GELU_TANH ? c2 * fmaf(0.044715f * g * g, g, g) : g;
     const float s = __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * z));
+    // s' / z'.  Where it is 0 (far from zero, in f32) the derivative is s, though z' may be infinite
+    const float t = s * (1.f - s);
     a = act == QR_ACT_SIGMOID ? s : g * s;
-    d = act == QR_ACT_SIGMOID ? s * (1.f - s)
-                              : fmaf(g * (act == QR_ACT_GELU_TANH ? c2 * fmaf(3.f * 0.044715f * g, g, 1.f) : 1.f), s * (1.f - s), s);
+    d = act == QR_ACT_SIGMOID ? t
+                              : t == 0.f ? s : fmaf(g * (act == QR_ACT_GELU_TANH ? c2 * fmaf(3.f * 0.044715f * g, g, 1.f) : 1.f), t, s);
   }
 }
 

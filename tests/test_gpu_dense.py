@@ -867,3 +867,37 @@ def test_ffn_backward_of_f16_captured(dense):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(p, q) for p, q in zip(out, want)), scale
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("act", ACTS)
+def test_ffn_backward_of_far_activations(dense, dtype, act):
+    """Gates of up to 2^100 on either side of zero: the derivative is 0 or 1 (a sigmoid's 0) there, whatever its factors are."""
+    far = [s * 2.0 ** e for e in (5, 6, 7, 20, 43, 44, 50, 62, 63, 65, 100) for s in (1, -1)]
+    n, m = len(far), 40
+    g = torch.tensor(far, device="cuda").expand(m, n).contiguous().to(dtype)
+    u, dh = rand(1, m, n, dtype=dtype), rand(2, m, n, dtype=dtype)
+    x, w = torch.eye(m, device="cuda", dtype=dtype), torch.eye(n, device="cuda", dtype=dtype)[:, :n]
+    # (products with unit matrices: dw_gate^T is dg, dw_up^T is du, each rounded once)
+    _, dwg, dwu = dense.gated_ffn_backward(dh, x, torch.zeros(n, m, device="cuda", dtype=dtype), torch.zeros(n, m, device="cuda", dtype=dtype),
+                                           g, u, act)
+    s, one = (g > 0).double(), dh.double() * u.double()
+    slope = torch.zeros_like(s) if act == "sigmoid" else s
+    value = s if act == "sigmoid" else s * g.double()
+    # (2^5 and beyond: 1 - sigmoid, erf's tail and the like are below 2^-45, far under a rounding of 1)
+    close(dwg.T.contiguous(), one * slope, 4 * U32 * one.abs() + 2.0 ** -40, dtype, "dg")
+    close(dwu.T.contiguous(), dh.double() * value, 4 * U32 * (dh.double() * value).abs() + 2.0 ** -35, dtype, "du")
+
+
+@pytest.mark.parametrize("act", ACTS)
+def test_ffn_forward_of_far_activations(dense, act):
+    """The same gates forward, by the few-rows kernel and by tiles, f32."""
+    far = [s * 2.0 ** e for e in (5, 7, 20, 44, 62, 65, 100) for s in (1, -1)]
+    n = len(far)
+    for m in (3, 40000):
+        x = rand(1, m, 1).abs() + 0.5
+        wg, wu = torch.tensor(far, device="cuda").view(n, 1), torch.ones(n, 1, device="cuda")
+        h = dense.gated_ffn(x, wg, wu, act)
+        g = x.double() @ wg.double().T
+        a = (g > 0).double() if act == "sigmoid" else g.clamp(min=0)
+        close(h, a * x.double(), 16 * U32 * (a * x.double()).abs() + 2.0 ** -16, torch.float32, "h")
