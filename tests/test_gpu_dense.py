@@ -901,3 +901,43 @@ def test_ffn_forward_of_far_activations(dense, act):
         g = x.double() @ wg.double().T
         a = (g > 0).double() if act == "sigmoid" else g.clamp(min=0)
         close(h, a * x.double(), 16 * U32 * (a * x.double()).abs() + 2.0 ** -16, torch.float32, "h")
+
+
+def f32_products(dense, m, k, n):
+    """(result, the one product it is, in 64 bits) of the forward pass, dx and both dW: every other term of the sums is zero,
+    every factor has 24 bits, all sizes above the few-rows kernel's."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(m + k + n)
+
+    def full(*shape):  # in 1 .. 2, either sign
+        return (1 + torch.rand(shape, generator=g, device="cuda")) * (1 - 2 * torch.randint(0, 2, shape, generator=g, device="cuda"))
+    x, wg, wu = torch.zeros(m, k, device="cuda"), torch.zeros(n, k, device="cuda"), torch.zeros(n, k, device="cuda")
+    x[:, k // 2], wg[:, k // 2], wu[:, k // 2] = full(m), full(n), full(n)
+    _, gate, up = dense.gated_ffn(x, wg, wu, "relu", save=True)
+    for got, w in ((gate, wg), (up, wu)):
+        yield "forward", got, x[:, k // 2].double()[:, None] * w[:, k // 2].double()
+    x, wg, wu = full(m, k), full(n, k), full(n, k)
+    one, none = torch.ones(m, n, device="cuda"), torch.zeros(m, n, device="cuda")
+    for gate, up, w, i in ((one, none, wu, 2), (none + 2.0 ** -30, one, wg, 1)):  # du = dh, dg = 0; dg = dh, du as good as 0
+        dh = torch.zeros(m, n, device="cuda")
+        dh[:, n // 3] = full(m)
+        dx, *_ = dense.gated_ffn_backward(dh, x, wg if i == 1 else torch.zeros_like(wg), wu if i == 2 else torch.zeros_like(wu), gate, up, "relu")
+        yield "dx", dx, dh[:, n // 3].double()[:, None] * w[n // 3].double()
+        dh.zero_()
+        dh[m // 2] = full(n)
+        got = dense.gated_ffn_backward(dh, x, wg, wu, gate, up, "relu")[i]
+        yield "dW", got, dh[m // 2].double()[:, None] * x[m // 2].double()
+
+
+@pytest.mark.parametrize("m,k,n", [(4096, 256, 1024), (4096, 64, 1024), (9000, 96, 1000), (9000, 160, 1000), (3001, 129, 999)])
+def test_f32_products_of_the_tiled_kernels_are_as_near_as_f32(dense, m, k, n):
+    """One product of two numbers of 24 bits each.  To the nearest, the parts of a number of 1 .. 2 are at most 2, 2^-8 and
+    2^-16, so what is left out is at most 2 x 2^-24 + 2^-32, of a product of 1 at least: 2.1 units of 2^-24.  The six that are
+    taken are added smallest first: one rounding of the result (1 unit, 2 if an addition cuts off) and two of terms below 2^-6
+    of it.  5 in all; and nothing of it leans to one side: the mean over all products within a tenth of a unit.  (Parts cut
+    off instead have one sign and left out 7 units at most, 0.63 on average.)"""
+    for what, got, want in f32_products(dense, m, k, n):
+        assert got.dtype == torch.float32 and want.abs().min() >= 1
+        e = (got.double() - want) / want * 2.0 ** 24
+        assert e.abs().max() <= 5 and abs(float(e.mean())) <= 0.1, (what, float(e.abs().max()), float(e.mean()))
+        assert e.square().mean().sqrt() <= 0.6, (what, float(e.square().mean().sqrt()))
