@@ -508,6 +508,8 @@ int qr_dropout_async(int device, void *hip_stream, int type, size_t rows, size_t
 /* of the weights: QR_ERR_UNSUPPORTED beyond.)                                                */
 /* f32 products: a product of two numbers is off by 0.43 x 2^-24 (root mean square; f32        */
 /* multiplication 0.42), 5 x 2^-24 at most, to neither side; numbers below 2^-110 lose bits.    */
+/* A factor that is infinite, or 3.396e38 (2^128 - 2^119) and more, makes NaN of every sum it     */
+/* enters, except in the forward pass of few rows, whose sums are f32 arithmetic's.               */
 /* h [m][n] = act(x w_gate^T) * (x w_up^T); x [m][k], weights [n][k] of stride ldw.        */
 /* gate / up: NULL (serving), or [m][n] contiguous: the two products, rounded to `type`,    */
 /* for the backward pass.  Outputs must not overlap each other or an input.  The workspace   */

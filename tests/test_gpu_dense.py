@@ -941,3 +941,30 @@ def test_f32_products_of_the_tiled_kernels_are_as_near_as_f32(dense, m, k, n):
         e = (got.double() - want) / want * 2.0 ** 24
         assert e.abs().max() <= 5 and abs(float(e.mean())) <= 0.1, (what, float(e.abs().max()), float(e.mean()))
         assert e.square().mean().sqrt() <= 0.6, (what, float(e.square().mean().sqrt()))
+
+
+@pytest.mark.parametrize("m,n", [(3, 50), (100, 512), (4000, 512), (4001, 200)])
+def test_ffn_f32_of_infinite_factors(dense, m, n):
+    """An infinite feature or weight: its row or column is not finite, whichever kernel makes it, and no other element changes.
+    Few rows: what f32 arithmetic gives."""
+    k = 72
+    x, wg, wu = ffn_inputs(m, m, k, n, torch.float32)
+    x2, wg2 = x.clone(), wg.clone()
+    x2[m // 2, 7], wg2[n // 3, 70] = float("inf"), float("-inf")
+    ref, got = dense.gated_ffn(x, wg, wu, "sigmoid", save=True), dense.gated_ffn(x2, wg2, wu, "sigmoid", save=True)
+    rows, cols = torch.ones(m, dtype=torch.bool), torch.ones(n, dtype=torch.bool)
+    rows[m // 2], cols[n // 3] = False, False
+    for i, (p, q) in enumerate(zip(got, ref)):
+        assert torch.equal(p[rows][:, cols], q[rows][:, cols])
+        if i:  # gate and up; up does not see w_gate
+            assert not torch.isfinite(p[~rows]).any() and (i == 2 or not torch.isfinite(p[:, ~cols]).any())
+    if m <= 100:
+        g = x2.double() @ wg2.double().T
+        assert torch.equal(got[1].isnan(), g.isnan()) and torch.equal(got[1].isinf(), g.isinf())
+        assert torch.equal(got[1][g.isinf()].double(), g[g.isinf()])
+    dh = rand(9, m, n)
+    a, b = dense.gated_ffn_backward(dh, x, wg, wu, *ref[1:], "sigmoid"), dense.gated_ffn_backward(dh, x2, wg, wu, *ref[1:], "sigmoid")
+    keep = torch.arange(k) != 7
+    for i in (1, 2):  # the sums over rows: only the feature's own column
+        assert torch.equal(a[i][:, keep], b[i][:, keep]) and not torch.isfinite(b[i][:, 7]).any()
+    assert torch.equal(a[0], b[0])
