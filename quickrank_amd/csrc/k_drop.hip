@@ -107,17 +107,17 @@ extern "C" int qr_dropout_async(int device, void *stream, int type, size_t rows,
   const size_t n = rows * cols;
   const bool flat = rows == 1 || (ldx == cols && ldy == cols && (!residual || ldr == cols));
   const auto grid = [](size_t threads) { return (unsigned)((threads + 255) / 256 < 8192 ? (threads + 255) / 256 : 8192); };
+  QrDenseStream s(stream);
   qr_dense_dispatch(type, [&](auto tt) {
     using T = decltype(tt);
-    const hipStream_t s = (hipStream_t)stream;
     const unsigned pieces = grid((n + 16 / sizeof(T) - 1) / (16 / sizeof(T)));
     if (flat && residual)
-      k_drop_flat<T, true, 2><<<pieces, 256, 0, s>>>(n, (const T *)x, (const T *)residual, (T *)y, t, scale, mix64(seed), offset, counter);
+      s.launch(k_drop_flat<T, true, 2>, pieces, 256, 0, n, (const T *)x, (const T *)residual, (T *)y, t, scale, mix64(seed), offset, counter);
     else if (flat)
-      k_drop_flat<T, false, 4><<<pieces, 256, 0, s>>>(n, (const T *)x, nullptr, (T *)y, t, scale, mix64(seed), offset, counter);
+      s.launch(k_drop_flat<T, false, 4>, pieces, 256, 0, n, (const T *)x, nullptr, (T *)y, t, scale, mix64(seed), offset, counter);
     else
-      k_drop_rows<T><<<grid((n + 3) / 4), 256, 0, s>>>(rows, cols, (const T *)x, ldx, (const T *)residual, ldr, (T *)y, ldy, t, scale,
-                                                      mix64(seed), offset, counter);
+      s.launch(k_drop_rows<T>, grid((n + 3) / 4), 256, 0, rows, cols, (const T *)x, ldx, (const T *)residual, ldr, (T *)y, ldy, t, scale,
+               mix64(seed), offset, counter);
   });
-  return qr_dense_launched("dropout");
+  return qr_dense_launched(s, "dropout");
 }

@@ -746,11 +746,11 @@ __global__ __launch_bounds__(256) void k_join(const float *__restrict__ part, co
 }
 // 16 shares where there are at least as many splits and one thread an output would not fill the chip's waves
 template <class T>
-void join(hipStream_t s, const float *part, size_t rows, size_t cols, unsigned outs, unsigned splits, T *o0, T *o1, size_t ldo) {
+void join(QrDenseStream &s, const float *part, size_t rows, size_t cols, unsigned outs, unsigned splits, T *o0, T *o1, size_t ldo) {
   const auto go = [&](auto v, auto p) {
     constexpr int V = decltype(v)::value, P = decltype(p)::value;
     const size_t groups = (outs * rows * cols / V + 256 / P - 1) / (256 / P);
-    k_join<T, V, P><<<(unsigned)std::min<size_t>(groups, 65536), 256, 0, s>>>(part, rows, cols, outs, splits, o0, o1, ldo);
+    s.launch(k_join<T, V, P>, (unsigned)std::min<size_t>(groups, 65536), 256, 0, part, rows, cols, outs, splits, o0, o1, ldo);
   };
   using one = std::integral_constant<int, 1>;
   using four = std::integral_constant<int, 4>;
@@ -890,16 +890,16 @@ __global__ __launch_bounds__(256) void k_gate_grad(const size_t m, const size_t 
 }
 // maxima, back: f16 only, MAXIMA floats and one
 template <class T>
-void gate_grad(hipStream_t s, size_t m, size_t n, int act, const void *dh, size_t lddh, const void *g, const void *u, T *dg, T *du,
+void gate_grad(QrDenseStream &s, size_t m, size_t n, int act, const void *dh, size_t lddh, const void *g, const void *u, T *dg, T *du,
                size_t ld, const Packs<T> &packs, float *maxima, float *back) {
   const auto groups = [](size_t threads, size_t most) { return (unsigned)std::min((threads + 255) / 256, most); };
   constexpr bool scaled = __is_same(T, _Float16);
   const unsigned grid = groups(m * (ld / 8), scaled ? 4096 : 65536), parts = scaled ? groups(m * ((n + 7) / 8), MAXIMA) : 0;
   const auto go = [&](auto a) {
     constexpr int ACT = decltype(a)::value;
-    if constexpr (scaled) k_gate_max<T, ACT><<<parts, 256, 0, s>>>(m, n, (const T *)dh, lddh, (const T *)g, (const T *)u, maxima);
-    k_gate_grad<T, ACT><<<packs.groups + grid, 256, 0, s>>>(m, n, (const T *)dh, lddh, (const T *)g, (const T *)u, dg, du, ld, packs, maxima,
-                                                            parts, back);
+    if constexpr (scaled) s.launch(k_gate_max<T, ACT>, parts, 256, 0, m, n, (const T *)dh, lddh, (const T *)g, (const T *)u, maxima);
+    s.launch(k_gate_grad<T, ACT>, packs.groups + grid, 256, 0, m, n, (const T *)dh, lddh, (const T *)g, (const T *)u, dg, du, ld, packs, maxima,
+             parts, back);
   };
   by_act(act, go);
 }
@@ -951,12 +951,12 @@ bool streams(const GemmArgs<T> &P, const size_t outs) {
 }
 
 template <class T, Kind KIND, int TM, int TN, int WN = 2, bool RAG = false>
-void launch_gemm(hipStream_t s, GemmArgs<T> P) {
+void launch_gemm(QrDenseStream &s, GemmArgs<T> P) {
   P.row_tiles = tiles_of(P.rows, TM);
   P.stream = streams(P, KIND == FWD ? (P.o[1] ? 3 : 1) : KIND == DW ? 2 : 1);
   P.col_tiles = tiles_of(P.cols, KIND == FWD ? TN / 2 : TN);
   const unsigned tiles = P.row_tiles * P.col_tiles * (KIND == FWD ? 1 : (KIND == DW ? 2 : 1) * P.splits);
-  k_gemm<T, KIND, TM, TN, WN, RAG><<<(tiles + 7) / 8 * 8, 128 * WN, 0, s>>>(P);
+  s.launch(k_gemm<T, KIND, TM, TN, WN, RAG>, (tiles + 7) / 8 * 8, 128 * WN, 0, P);
 }
 
 
@@ -971,13 +971,13 @@ bool few(size_t e, size_t m, size_t n) {
 }
 
 template <class T>
-void launch_few(hipStream_t s, const GemmArgs<T> &P) {
+void launch_few(QrDenseStream &s, const GemmArgs<T> &P) {
   const unsigned cols = tiles_of(P.cols, 16);
   // the most rows a workgroup that still leave every compute unit one (16-bit types: 64 rows never do)
   if constexpr (sizeof(T) == 4)
-    if (P.rows > 32 && (size_t)cols * tiles_of(P.rows, 64) >= CUS) return k_few<T, 4><<<dim3(cols, tiles_of(P.rows, 64)), 512, 0, s>>>(P);
-  if (P.rows > 16 && (size_t)cols * tiles_of(P.rows, 32) >= CUS) k_few<T, 2><<<dim3(cols, tiles_of(P.rows, 32)), 512, 0, s>>>(P);
-  else k_few<T, 1><<<dim3(cols, tiles_of(P.rows, 16)), 512, 0, s>>>(P);
+    if (P.rows > 32 && (size_t)cols * tiles_of(P.rows, 64) >= CUS) return s.launch(k_few<T, 4>, dim3(cols, tiles_of(P.rows, 64)), 512, 0, P);
+  if (P.rows > 16 && (size_t)cols * tiles_of(P.rows, 32) >= CUS) s.launch(k_few<T, 2>, dim3(cols, tiles_of(P.rows, 32)), 512, 0, P);
+  else s.launch(k_few<T, 1>, dim3(cols, tiles_of(P.rows, 16)), 512, 0, P);
 }
 
 struct Tile {
@@ -1003,7 +1003,7 @@ Tile tile_of(size_t e, size_t rows, size_t cols, size_t times, bool narrow) {
 }
 
 template <class T, Kind KIND>
-void gemm(hipStream_t s, const Tile t, const GemmArgs<T> &P) {
+void gemm(QrDenseStream &s, const Tile t, const GemmArgs<T> &P) {
   if constexpr (sizeof(T) == 2)
     if (t.rows == 256) return t.cols == 256 ? launch_gemm<T, KIND, 256, 256, 4>(s, P) : launch_gemm<T, KIND, 256, 128>(s, P);
   if (t.rows == 128 && t.cols == 128) return launch_gemm<T, KIND, 128, 128>(s, P);
@@ -1118,9 +1118,9 @@ extern "C" int qr_gated_ffn_async(int device, void *stream, int type, int act, s
     for (int j = 0; j < i; ++j) QR_DENSE_ARG(!qr_dense_overlap(out[i], bytes[i], out[j], bytes[j]), "gated ffn: outputs overlap");
   }
   QR_DENSE_DEVICE(device);
+  QrDenseStream s(stream);
   qr_dense_dispatch(type, [&](auto t) {
     using T = decltype(t);
-    const hipStream_t s = (hipStream_t)stream;
     char *ws = (char *)(((uintptr_t)workspace + 255) & ~(uintptr_t)255);
     GemmArgs<T> P{};
     P.a[0] = (const T *)x, P.b[0] = (const T *)w_gate, P.b[1] = (const T *)w_up;
@@ -1136,11 +1136,11 @@ extern "C" int qr_gated_ffn_async(int device, void *stream, int type, int act, s
       size_t ld = ldw;
       pack(packs, n, k, P.b[0], ld, ws, n), pack(packs, n, k, P.b[1], P.ldb, ws, n);
     }
-    if (packs.groups) k_pack<T><<<packs.groups, 256, 0, s>>>(packs);
+    if (packs.groups) s.launch(k_pack<T>, packs.groups, 256, 0, packs);
     if (few(e, m, n)) launch_few(s, P);
     else gemm<T, FWD>(s, tile_forward(e, m, k, n, gate != nullptr), P);
   });
-  return qr_dense_launched("gated ffn");
+  return qr_dense_launched(s, "gated ffn");
 }
 
 extern "C" int qr_gated_ffn_backward_workspace(int type, size_t m, size_t k, size_t n, size_t *bytes) {
@@ -1184,7 +1184,7 @@ extern "C" int qr_gated_ffn_backward_async(int device, void *stream, int type, i
     for (int j = 0; j < i; ++j) QR_DENSE_ARG(!qr_dense_overlap(out[i], ob[i], out[j], ob[j]), "gated ffn backward: outputs overlap");
   }
   QR_DENSE_DEVICE(device);
-  const hipStream_t s = (hipStream_t)stream;
+  QrDenseStream s(stream);
   qr_dense_dispatch(type, [&](auto t) {
     using T = decltype(t);
     char *ws = (char *)(((uintptr_t)workspace + 255) & ~(uintptr_t)255);
@@ -1220,5 +1220,5 @@ extern "C" int qr_gated_ffn_backward_async(int device, void *stream, int type, i
       if (W.part) join(s, part, n, k, 2, pw.splits, (T *)dw_gate, (T *)dw_up, k);
     }
   });
-  return qr_dense_launched("gated ffn backward");
+  return qr_dense_launched(s, "gated ffn backward");
 }

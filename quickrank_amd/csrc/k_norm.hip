@@ -319,9 +319,9 @@ __global__ __launch_bounds__(1024) void k_norm_join(const int cols, const int pa
 }
 // 64 shares, or four where there are few parts (the whole gradient of 5 x 12089 bf16 18.2 us, by 64 shares 20.8)
 template <class P>
-void norm_join(hipStream_t s, size_t cols, size_t parts, const float *part, void *dw, void *db) {
-  if (parts >= 64) k_norm_join<P, 64><<<(unsigned)((2 * cols + 15) / 16), 1024, 0, s>>>((int)cols, (int)parts, part, (P *)dw, (P *)db);
-  else k_norm_join<P, 4><<<(unsigned)((2 * cols + 255) / 256), 1024, 0, s>>>((int)cols, (int)parts, part, (P *)dw, (P *)db);
+void norm_join(QrDenseStream &s, size_t cols, size_t parts, const float *part, void *dw, void *db) {
+  if (parts >= 64) s.launch(k_norm_join<P, 64>, (unsigned)((2 * cols + 15) / 16), 1024, 0, (int)cols, (int)parts, part, (P *)dw, (P *)db);
+  else s.launch(k_norm_join<P, 4>, (unsigned)((2 * cols + 255) / 256), 1024, 0, (int)cols, (int)parts, part, (P *)dw, (P *)db);
 }
 
 // ---- rows that no workgroup's registers hold (and rows of less than 16 bytes): read again for every step ----------
@@ -458,7 +458,7 @@ extern "C" int qr_layer_norm_async(int device, void *stream, int type, int param
   if (!rows) return QR_OK;
   QR_DENSE_ARG(x && y, "layer norm: x or y is NULL");
   QR_DENSE_DEVICE(device);
-  const hipStream_t s = (hipStream_t)stream;
+  QrDenseStream s(stream);
   qr_dense_dispatch(type, [&](auto t) {
     using T = decltype(t);
     auto go = [&](auto p) {
@@ -467,19 +467,19 @@ extern "C" int qr_layer_norm_async(int device, void *stream, int type, int param
         constexpr size_t RPB = 256 / G(), MOST = RPB << 23;  // (a launch has fewer than 2^32 threads)
         for (size_t r = 0; r < rows; r += MOST) {
           const size_t n = std::min(rows - r, MOST);
-          k_norm<T, P, G(), N()><<<(unsigned)((n + RPB - 1) / RPB), 256, 0, s>>>(
-              n, (int)cols, (const T *)x + r * ldx, ldx, (const P *)weight, (const P *)bias, eps, (T *)y + r * ldy, ldy,
-              mean ? mean + r : nullptr, rstd ? rstd + r : nullptr);
+          s.launch(k_norm<T, P, G(), N()>, (unsigned)((n + RPB - 1) / RPB), 256, 0,
+                   n, (int)cols, (const T *)x + r * ldx, ldx, (const P *)weight, (const P *)bias, eps, (T *)y + r * ldy, ldy,
+                   mean ? mean + r : nullptr, rstd ? rstd + r : nullptr);
         }
       });
       if (!fits)
-        k_norm_any<T, P><<<(unsigned)(rows < 65536 ? rows : 65536), 1024, 0, s>>>(rows, (int)cols, (const T *)x, ldx, (const P *)weight,
-                                                                                (const P *)bias, eps, (T *)y, ldy, mean, rstd);
+        s.launch(k_norm_any<T, P>, (unsigned)(rows < 65536 ? rows : 65536), 1024, 0, rows, (int)cols, (const T *)x, ldx, (const P *)weight,
+                 (const P *)bias, eps, (T *)y, ldy, mean, rstd);
     };
     if (param_type == QR_F32) go(float{});
     else go(T{});
   });
-  return qr_dense_launched("layer norm");
+  return qr_dense_launched(s, "layer norm");
 }
 
 extern "C" int qr_layer_norm_backward_workspace(size_t rows, size_t cols, size_t *bytes) {
@@ -506,7 +506,7 @@ extern "C" int qr_layer_norm_backward_async(int device, void *stream, int type, 
   QR_DENSE_ARG(!sums || !rows || (workspace && workspace_bytes >= need), "layer norm backward: the workspace is too small");
   if (!rows && !sums) return QR_OK;
   QR_DENSE_DEVICE(device);
-  const hipStream_t s = (hipStream_t)stream;
+  QrDenseStream s(stream);
   const unsigned any = (unsigned)parts_any(rows, cols);
   qr_dense_dispatch(type, [&](auto t) {
     using T = decltype(t);
@@ -517,23 +517,23 @@ extern "C" int qr_layer_norm_backward_async(int device, void *stream, int type, 
         constexpr size_t RPB = G() > 256 ? 1 : 256 / G();
         const size_t want = (rows + RPB - 1) / RPB, parts = parts_of(rows, G(), N());
         const unsigned grid = want <= ALONE ? 1 : (unsigned)(want < parts ? want : parts);
-        k_norm_grad<T, P, G(), N()><<<grid, G() > 256 ? G() : 256, RPB > 1 && sums ? 8 * cols * 4 : 0, s>>>(
-            rows, (int)cols, (const T *)dy, lddy, (const T *)x, ldx, (const P *)weight, mean, rstd, (T *)dx, lddx, part, (P *)dweight, (P *)dbias);
+        s.launch(k_norm_grad<T, P, G(), N()>, grid, G() > 256 ? G() : 256, RPB > 1 && sums ? 8 * cols * 4 : 0,
+                 rows, (int)cols, (const T *)dy, lddy, (const T *)x, ldx, (const P *)weight, mean, rstd, (T *)dx, lddx, part, (P *)dweight, (P *)dbias);
         if (sums && grid > 1) norm_join<P>(s, cols, grid, part, dweight, dbias);
       });
       if (fits && rows) return;
       // (the column sums first: dx may be written over dy or x)
       if (rows && sums)
-        k_norm_cols<T><<<dim3((unsigned)((cols + 255) / 256), any), 256, 0, s>>>(rows, (int)cols, (const T *)dy, lddy, (const T *)x,
-                                                                                  ldx, mean, rstd, part);
+        s.launch(k_norm_cols<T>, dim3((unsigned)((cols + 255) / 256), any), 256, 0, rows, (int)cols, (const T *)dy, lddy, (const T *)x,
+                 ldx, mean, rstd, part);
       if (sums)
         norm_join<P>(s, cols, any, part, dweight, dbias);
       if (rows && dx)
-        k_norm_grad_any<T, P><<<(unsigned)(rows < 65536 ? rows : 65536), 1024, 0, s>>>(
-            rows, (int)cols, (const T *)dy, lddy, (const T *)x, ldx, (const P *)weight, mean, rstd, (T *)dx, lddx);
+        s.launch(k_norm_grad_any<T, P>, (unsigned)(rows < 65536 ? rows : 65536), 1024, 0,
+                 rows, (int)cols, (const T *)dy, lddy, (const T *)x, ldx, (const P *)weight, mean, rstd, (T *)dx, lddx);
     };
     if (param_type == QR_F32) go(float{});
     else go(T{});
   });
-  return qr_dense_launched("layer norm backward");
+  return qr_dense_launched(s, "layer norm backward");
 }

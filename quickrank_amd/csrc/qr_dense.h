@@ -9,6 +9,7 @@
 #include <stdint.h>
 
 #include <string>
+#include <tuple>
 
 #include "../../include/qr_hip.h"
 
@@ -45,10 +46,29 @@ struct QrDeviceGuard {
                          "the device cannot be made current (this library has no CPU fallback)"); \
   }
 
-inline int qr_dense_launched(const char *what) noexcept {
-  const hipError_t e = hipGetLastError();
-  if (e == hipSuccess) return QR_OK;
-  return qr_dense_fail(QR_ERR_HIP, hipGetErrorString(e) ? hipGetErrorString(e) : what);
+// The call's stream.  A launch's outcome is what it returns, not the thread's last error, which an earlier call of somebody
+// else's may have left; behind one that failed nothing more is launched.
+struct QrDenseStream {
+  hipStream_t stream;
+  hipError_t err = hipSuccess;
+  explicit QrDenseStream(void *s) : stream((hipStream_t)s) {}
+  template <class... P, class... A>
+  void launch(void (*kernel)(P...), dim3 grid, unsigned block, size_t lds, const A &...a) {
+    if (err != hipSuccess) return;
+    std::tuple<P...> v(static_cast<P>(a)...);
+    std::apply(
+        [&](P &...p) {
+          void *args[] = {(void *)&p...};
+          err = hipLaunchKernel((const void *)kernel, grid, dim3(block), args, lds, stream);
+        },
+        v);
+  }
+};
+
+inline int qr_dense_launched(const QrDenseStream &s, const char *what) noexcept {
+  if (s.err == hipSuccess) return QR_OK;
+  (void)hipGetLastError();  // (reported here)
+  return qr_dense_fail(QR_ERR_HIP, hipGetErrorString(s.err) ? hipGetErrorString(s.err) : what);
 }
 
 inline bool qr_dense_type_ok(int t) { return t == QR_F32 || t == QR_BF16 || t == QR_F16; }

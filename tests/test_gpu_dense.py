@@ -968,3 +968,24 @@ def test_ffn_f32_of_infinite_factors(dense, m, n):
     for i in (1, 2):  # the sums over rows: only the feature's own column
         assert torch.equal(a[i][:, keep], b[i][:, keep]) and not torch.isfinite(b[i][:, 7]).any()
     assert torch.equal(a[0], b[0])
+
+
+def test_an_earlier_failed_call_of_the_runtime_is_not_ours(dense):
+    """A HIP call that failed before on this thread does not make an enqueued operator fail, and its error is still there for
+    whom it concerns."""
+    L = raw(dense)
+    L.hipSetDevice.argtypes, L.hipSetDevice.restype, L.hipGetLastError.restype = [C.c_int], C.c_int, C.c_int
+    x, w = rand(1, 30, 8), rand(2, 6, 8)
+    h, g, u = dense.gated_ffn(x, w, w, save=True)
+    _, mean, rstd = dense.layer_norm(x)
+    for call in (lambda: dense.layer_norm(x), lambda: dense.layer_norm_backward(x, x, None, mean, rstd), lambda: dense.dropout(x, 0.5, 1),
+                 lambda: dense.gated_ffn(x, w, w), lambda: dense.gated_ffn_backward(h, x, w, w, g, u)):
+        want = call()
+        e = L.hipSetDevice(4096)
+        try:
+            got = call()
+        finally:
+            left = L.hipGetLastError()
+        assert e != 0 and left == e
+        pairs = [(want, got)] if isinstance(want, torch.Tensor) else zip(want, got)
+        assert all(torch.equal(p, q) for p, q in pairs)
