@@ -5,7 +5,7 @@ Every call runs the HIP kernels of libqr_hip.so on the tensors' own device, on t
 stream of that device, and only enqueues; tensors used on another stream than the one they were
 made on need `Tensor.record_stream`, as with any torch operator.  Gradients are explicit calls, as
 the lambda pass is one: nothing is recorded by autograd, so a tensor that requires a gradient is
-refused while autograd records.
+refused while autograd records, and one with a forward-mode tangent always.
 
 A tensor of rows is f32, bf16 or f16 and is read as a matrix of its last dimension: 2-D with any
 row stride (0 included), or contiguous with any leading dimensions.
@@ -14,6 +14,7 @@ import ctypes as C
 from operator import index
 
 import torch
+from torch.autograd import forward_ad
 
 from ._capi import QrError, lib
 
@@ -36,12 +37,14 @@ def _check(t, what, device=None):
     """The tensor's device number, of `device` where that is given."""
     if not isinstance(t, torch.Tensor) or t.dtype not in TYPES:
         _refuse(f"{what} is a torch tensor of f32, bf16 or f16")
-    at = t.get_device()
-    if at < 0 or not t.is_cuda:
-        _refuse(f"{what} is not on a GPU: there is no CPU fallback")
     if t.requires_grad and torch.is_grad_enabled():
         _refuse(f"{what} requires a gradient, which this call would not record: use torch.no_grad() and the "
                 "backward call")
+    if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
+        _refuse(f"{what} has a forward-mode tangent, which this call would lose")
+    at = t.get_device()
+    if at < 0 or not t.is_cuda:
+        _refuse(f"{what} is not on a GPU: there is no CPU fallback")
     if device is not None and at != device:
         _refuse(f"{what} is on {t.device}, not on cuda:{device}")
     return at

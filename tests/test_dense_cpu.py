@@ -179,3 +179,21 @@ def test_weights_of_one_layout(monkeypatch, n, k, gate, up, ldw):
     from quickrank_amd import dense
     monkeypatch.setattr(dense, "_check", lambda t, what, device=None: 0)
     assert dense._weights(torch.zeros(3, k), k, _laid_out(n, k, *gate), _laid_out(n, k, *up), 0) == (n, ldw)
+
+
+def test_forward_mode_tangents_are_refused():
+    """A dual tensor requires no gradient; its tangent would be lost without a word."""
+    from torch.autograd import forward_ad
+    from quickrank_amd import QrError, dense
+    x, w = torch.rand(4, 6), torch.rand(6, 6)
+    with forward_ad.dual_level():
+        d = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: dense.layer_norm(d), lambda: dense.dropout(d, 0.1, 1), lambda: dense.dropout_backward(d, 0.1, 1),
+                     lambda: dense.gated_ffn(d, w, w), lambda: dense.layer_norm_backward(x, d, None, x[:, 0], x[:, 0]),
+                     lambda: dense.gated_ffn_backward(x, d, w, w, x, x), lambda: dense._check(d, "w_gate")):
+            with pytest.raises(QrError) as e:
+                call()
+            assert e.value.code == ARG and "tangent" in str(e.value)
+        with pytest.raises(QrError) as e:
+            dense.layer_norm(x)  # one without a tangent
+        assert "GPU" in str(e.value)

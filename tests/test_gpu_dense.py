@@ -989,3 +989,23 @@ def test_an_earlier_failed_call_of_the_runtime_is_not_ours(dense):
         assert e != 0 and left == e
         pairs = [(want, got)] if isinstance(want, torch.Tensor) else zip(want, got)
         assert all(torch.equal(p, q) for p, q in pairs)
+
+
+def test_tangents_of_any_argument_are_refused(dense):
+    from torch.autograd import forward_ad
+    from quickrank_amd import QrError
+    x, wg, wu = ffn_inputs(1, 4, 8, 6, torch.float32)
+    w = rand(1, 8)
+    want, mean, rstd = dense.layer_norm(x, w)
+    h, g, u = dense.gated_ffn(x, wg, wu, save=True)
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))
+        for call in (lambda: dense.layer_norm(x, dual(w)), lambda: dense.layer_norm(x, None, dual(w)),
+                     lambda: dense.layer_norm_backward(dual(x), x, w, mean, rstd), lambda: dense.layer_norm_backward(x, x, w, dual(mean), rstd),
+                     lambda: dense.dropout(x, 0.1, 1, residual=dual(x)), lambda: dense.gated_ffn(x, dual(wg), wu),
+                     lambda: dense.gated_ffn(x, wg, dual(wu)), lambda: dense.gated_ffn_backward(dual(h), x, wg, wu, g, u),
+                     lambda: dense.gated_ffn_backward(h, x, wg, wu, g, dual(u))):
+            with pytest.raises(QrError) as e:
+                call()
+            assert "tangent" in str(e.value)
+        assert torch.equal(dense.layer_norm(x, w)[0], want)
