@@ -42,6 +42,8 @@ def _check(t, what, device=None):
                 "backward call")
     if forward_ad._current_level >= 0 and forward_ad.unpack_dual(t).tangent is not None:
         _refuse(f"{what} has a forward-mode tangent, which this call would lose")
+    if t.is_neg():
+        _refuse(f"{what} is a view whose numbers are negated when read: use resolve_neg()")
     at = t.get_device()
     if at < 0 or not t.is_cuda:
         _refuse(f"{what} is not on a GPU: there is no CPU fallback")

@@ -197,3 +197,16 @@ def test_forward_mode_tangents_are_refused():
         with pytest.raises(QrError) as e:
             dense.layer_norm(x)  # one without a tangent
         assert "GPU" in str(e.value)
+
+
+def test_views_that_are_negated_when_read_are_refused():
+    """The imaginary part of a conjugate shares its memory with the number's own: what lies there has the other sign."""
+    from quickrank_amd import QrError, dense
+    z = torch.complex(torch.rand(5, 1), torch.rand(5, 1))
+    x = z.conj().imag
+    assert x.is_neg() and x.dtype == torch.float32
+    for call in (lambda: dense.layer_norm(x), lambda: dense.dropout(x, 0.1, 1), lambda: dense.gated_ffn(x, x, x)):
+        with pytest.raises(QrError) as e:
+            call()
+        assert e.value.code == ARG and "negated" in str(e.value)
+    assert not x.resolve_neg().is_neg()
