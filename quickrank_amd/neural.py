@@ -3,9 +3,10 @@
 A document's score is a function of its feature row alone, as an ensemble's is: normalised features, residual
 blocks  z + dropout(gated_ffn(layer_norm(z)) w_down^T),  a last layer norm and one weight vector.  The gradient
 that reaches the scores is the one the trees are fitted to (LambdaMart::compute_pseudoresponses,
-lambdamart.cc:62-152): the context ranks the scorer's scores and its pseudo-responses are walked up.  Same
-surface as trainer.Mart: learn() on rows, labels and query offsets, score_dataset() on rows; the scores can
-also be what boosting starts from (Context.set_scores)."""
+lambdamart.cc:62-152): the context ranks the scorer's scores and its pseudo-responses are walked up.  As of
+trainer.Mart there are learn() on rows, labels and query offsets and score_dataset() on rows (a scorer is
+`params`, plain tensors: there is no file format of its own); the scores can also be what boosting starts
+from (Context.set_scores)."""
 import numpy as np
 import torch
 
@@ -44,9 +45,12 @@ class NeuralScorer:
 
     @torch.no_grad()
     def forward(self, x, train=False):
-        """(scores f32, what backward needs) of rows on the device; without train nothing is dropped or kept."""
-        x = x.to(self.dtype)
+        """(scores f32, what backward needs) of rows on the device; without train nothing is dropped and
+        the blocks keep nothing."""
+        # (features are standardised from f32: in 16 bits large ones would be infinite, small differences gone)
+        x = x.to(torch.float32)
         z, mean, rstd = self._norm(x, "in")
+        z = z.to(self.dtype)
         kept = [(x, mean, rstd)]
         for b in range(self.blocks):
             y, mean, rstd = self._norm(z, b)
@@ -82,7 +86,7 @@ class NeuralScorer:
             dy, out[f"gate_{b}"], out[f"up_{b}"] = dense.gated_ffn_backward(
                 branch @ p[f"down_{b}"], y, p[f"gate_{b}"], p[f"up_{b}"], g, u, self.act)
             dz = dz + norm(dy, b, z, mean, rstd)
-        norm(dz, "in", *kept[0])
+        norm(dz.to(torch.float32), "in", *kept[0])
         return out
 
     def step(self, x, optimizer):

@@ -88,3 +88,29 @@ def test_learns_from_the_lambda_pass(dtype):
     unit = 2.0 ** -24 if dtype == torch.float32 else 2.0 ** -8
     assert abs(one[0] - a[7]) <= unit * 200 * max(1.0, np.abs(a).max())
     other.close()
+
+
+@pytest.mark.parametrize("dtype,shift,scale", [(torch.bfloat16, 1e4, 1.0), (torch.bfloat16, -300.0, 0.5), (torch.float16, 2e5, 3e4),
+                                               (torch.float16, 1000.0, 0.25), (torch.float32, 1e4, 1.0)])
+def test_raw_features_keep_their_digits(dtype, shift, scale):
+    """Features are standardised from the 32 bits they come in, whatever type the scorer computes in.  No blocks: the score is
+    norm(norm(x)) w with two roundings of half a step on the way.  A rounding of the first result moves the second by at most
+    as much (a projection, times a scale of 1), so the score is off by |w| 136^1/2 (1.05 + 1) half steps, and f32's own."""
+    s = scorer(blocks=0, drop=0.0, dtype=dtype)
+    s.init(136)
+    x = (torch.randn(300, 136, generator=torch.Generator().manual_seed(4)) * scale + shift).cuda()
+    half = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}[dtype]
+    # (f32: the mean and the difference from it are off by some steps of the shift)
+    own = 2.0 ** -24 * (8 * abs(shift) / scale + 300)
+    want, p = reference(s, x, None)
+    scores, kept = s.forward(x, train=True)
+    assert (scores.double() - want).abs().max() <= (2.1 * half + own) * 136 ** 0.5 * float(p["score"].detach().norm())
+    # the first norm's gradients: the sums of |terms|, each off by the roundings of eight factors
+    ds = torch.randn(300, generator=torch.Generator().manual_seed(2)).cuda()
+    grads = s.backward(kept, ds)
+    (want * ds.double()).sum().backward()
+    hat = (x.double() - x.double().mean(1, keepdim=True)) / (x.double().var(1, keepdim=True, unbiased=False) + 1e-5).sqrt()
+    g = (ds.double()[:, None] * p["score"]).abs()
+    dz = g + g.mean(1, keepdim=True) + hat.abs() * (g * hat.abs()).mean(1, keepdim=True)
+    for name, terms in (("norm_in.weight", dz * hat.abs()), ("norm_in.bias", dz)):
+        assert ((grads[name].double() - p[name].grad).abs() <= (8 * half + 4 * own) * 1.1 * terms.sum(0)).all(), name
