@@ -505,7 +505,8 @@ int qr_dropout_async(int device, void *hip_stream, int type, size_t rows, size_t
                      uint64_t offset, const uint64_t *counter);
 
 /* (Rows of x and the weights, and backward of h, up to 4 MB, up to 2^30 rows of x and 2^28   */
-/* of the weights: QR_ERR_UNSUPPORTED beyond.)                                                */
+/* of the weights, less than 2^24 tiles of 128 x 64 elements of h or dx: QR_ERR_UNSUPPORTED    */
+/* beyond.)                                                                                    */
 /* f32 products: a product of two numbers is off by 0.43 x 2^-24 (root mean square; f32        */
 /* multiplication 0.42), 5 x 2^-24 at most, to neither side; numbers below 2^-110 lose bits.    */
 /* A factor that is infinite, or 3.396e38 (2^128 - 2^119) and more, makes NaN of every sum it     */

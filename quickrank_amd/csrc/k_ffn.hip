@@ -920,6 +920,8 @@ unsigned blocks(size_t n) { return (unsigned)((n + 255) / 256 < 65536 ? (n + 255
 constexpr size_t ROW_BYTES = (size_t)1 << 22;
 // most rows and most outputs of a row: a launch has fewer than 2^32 threads
 constexpr size_t ROWS_MOST = (size_t)1 << 30, OUTS_MOST = (size_t)1 << 28;
+// ... and most tiles of 128 x 128 sums (dx: 128 x 64, its narrowest), of 256 threads
+constexpr size_t TILES_MOST = ((size_t)1 << 24) - 1;
 
 // whether the product kernel can read a matrix where it lies: rows of whole pieces of 16 bytes at 16-byte boundaries
 bool in_place(const void *p, size_t ld, size_t cols, size_t e) {
@@ -1107,6 +1109,8 @@ extern "C" int qr_gated_ffn_async(int device, void *stream, int type, int act, s
   QR_DENSE_ARG(!need || (workspace && workspace_bytes >= need),
                "gated ffn: rows that start or end off 16-byte boundaries or lie more than 4 MB apart need the workspace");
   if (m > ROWS_MOST || n > OUTS_MOST) return qr_dense_fail(QR_ERR_UNSUPPORTED, "gated ffn: more than 2^30 rows or 2^28 outputs");
+  if (!few(e, m, n) && (size_t)tiles_of(m, 128) * tiles_of(2 * n, 128) > TILES_MOST)
+    return qr_dense_fail(QR_ERR_UNSUPPORTED, "gated ffn: 2^24 tiles of 128 x 64 outputs or more");
   if (!few(e, m, n) && k * e > ROW_BYTES) return qr_dense_fail(QR_ERR_UNSUPPORTED, "gated ffn: rows longer than 4 MB");
   const void *out[4] = {h, gate, up, workspace};
   const size_t bytes[4] = {qr_dense_span(m, n, ldh, e), m * n * e, m * n * e, need};
@@ -1175,6 +1179,8 @@ extern "C" int qr_gated_ffn_backward_async(int device, void *stream, int type, i
   if (m > ROWS_MOST) return qr_dense_fail(QR_ERR_UNSUPPORTED, "gated ffn backward: more than 2^30 rows");
   if (k * e > ROW_BYTES || stages_of(n, e) * e > ROW_BYTES)
     return qr_dense_fail(QR_ERR_UNSUPPORTED, "gated ffn backward: rows longer than 4 MB");
+  if (dx && (size_t)tiles_of(m, 128) * tiles_of(k, 64) > TILES_MOST)
+    return qr_dense_fail(QR_ERR_UNSUPPORTED, "gated ffn backward: 2^24 tiles of 128 x 64 elements of dx or more");
   const void *out[4] = {dx, dw_gate, dw_up, workspace}, *in[6] = {dh, x, w_gate, w_up, gate, up};
   const size_t ob[4] = {qr_dense_span(m, k, lddx, e), n * k * e, n * k * e, need};
   const size_t ib[6] = {qr_dense_span(m, n, lddh, e), qr_dense_span(m, k, ldx, e), qr_dense_span(n, k, ldw, e),

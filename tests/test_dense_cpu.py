@@ -210,3 +210,15 @@ def test_views_that_are_negated_when_read_are_refused():
             call()
         assert e.value.code == ARG and "negated" in str(e.value)
     assert not x.resolve_neg().is_neg()
+
+
+def test_ffn_of_more_tiles_than_a_launch_has_threads_for_is_unsupported(L):
+    """2^24 tiles of 256 threads: rows and outputs within their own limits, in the forward pass and in dx."""
+    big, ws = 1 << 56, 1 << 57
+    for m, n, type in ((1 << 30, 65, 1), (1 << 30, 128, 0), (1 << 26, 2048, 2), ((1 << 30) - 127, 100, 0)):
+        assert ffn(L, type=type, m=m, k=16, n=n, ldx=16, ldw=16, ldh=n, wg=1 << 50, wu=1 << 51, h=big, ws=ws, nbytes=ws) == 5
+        assert "tiles" in message(L)
+    for m, k, type in ((1 << 30, 128, 1), (1 << 30, 65, 0), (1 << 26, 2048, 2)):
+        assert ffn_back(L, type=type, m=m, k=k, dh=big >> 1, x=big >> 2, wg=R + Q, wu=8 * R, g=big >> 3, u=big >> 4, dx=big, lddx=k,
+                        dwg=16 * R, dwu=32 * R, ws=ws, nbytes=ws) == 5
+        assert "tiles" in message(L)
