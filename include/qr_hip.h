@@ -464,9 +464,15 @@ int qr_oblivious_score(qr_ctx *ctx, const float *rowmajor, size_t N, size_t F,
 /*     outputs: at least a row).  Sums, statistics and products are held in 32 bits,    */
 /*     every output is rounded once.  No alignment beyond the element's own is needed;  */
 /*     16 bytes (base and stride) is faster                                             */
-/*   - rows == 0 is no work (sums over rows are then written as zeros); no columns,     */
-/*     unknown codes, missing pointers, a short workspace: QR_ERR_ARG before any launch  */
+/*   - rows == 0 is no work (sums over rows are then written as zeros); no columns       */
+/*     (dropout: no work), unknown codes, missing pointers, a short workspace: QR_ERR_ARG */
+/*     before any launch                                                                   */
 /*   - the message of a failed call: qr_last_error(NULL) on the calling thread           */
+/*   - an output shares no element with an input or another output but where a call says   */
+/*     "may be": that is the same matrix, row for row, of one stride.  Rows of one stride    */
+/*     may lie side by side (x in the first columns of a buffer, h in the next).  Matrices of */
+/*     two strides whose memory overlaps from end to end: QR_ERR_ARG                           */
+/*   - workspaces lie at 4-byte boundaries, counters at 8-byte ones                             */
 /*   - results do not depend on timing: no atomics, joins in a fixed order               */
 #define QR_F32 0
 #define QR_BF16 1
@@ -513,10 +519,9 @@ int qr_dropout_async(int device, void *hip_stream, int type, size_t rows, size_t
 /* enters, except in the forward pass of few rows, whose sums are f32 arithmetic's.               */
 /* h [m][n] = act(x w_gate^T) * (x w_up^T); x [m][k], weights [n][k] of stride ldw.        */
 /* gate / up: NULL (serving), or [m][n] contiguous: the two products, rounded to `type`,    */
-/* for the backward pass.  Outputs must not overlap each other or an input.  The workspace   */
-/* is used (NULL, 0 will do otherwise) where a row of x or of a weight does not start and end  */
-/* at 16-byte boundaries or lies more than 4 MB behind the one before: such matrices may be    */
-/* copied.                                                                                    */
+/* for the backward pass.  The workspace is used (NULL, 0 will do otherwise) where a row of x */
+/* or of a weight does not start and end at 16-byte boundaries or lies more than 4 MB behind  */
+/* the one before: such matrices may be copied.                                               */
 int qr_gated_ffn_workspace(int type, size_t m, size_t k, size_t n, size_t *bytes);
 int qr_gated_ffn_async(int device, void *hip_stream, int type, int act, size_t m, size_t k, size_t n,
                        const void *x, size_t ldx, const void *w_gate, const void *w_up, size_t ldw, void *h,

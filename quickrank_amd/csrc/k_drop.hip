@@ -101,6 +101,10 @@ extern "C" int qr_dropout_async(int device, void *stream, int type, size_t rows,
   QR_DENSE_ARG(rows < 2 || ldy >= cols, "dropout: the stride of y is shorter than a row");
   if (!rows || !cols) return QR_OK;
   QR_DENSE_ARG(x && y, "dropout: x or y is NULL");
+  const QrDenseMatrix my{y, rows, cols, ldy}, in[2] = {{x, rows, cols, ldx}, {residual, rows, cols, ldr}};
+  for (int i = 0; i < 2; ++i)
+    QR_DENSE_ARG(qr_dense_in_place(my, in[i]) || !qr_dense_share(my, in[i], qr_dense_size(type)),
+                 "dropout: y lies over x or the residual, but not row for row");
   QR_DENSE_DEVICE(device);
   const uint32_t t = (uint32_t)(p * 65536.0 + 0.5);
   const float scale = t < 65536 ? 65536.f / (float)(65536 - t) : 0.f;

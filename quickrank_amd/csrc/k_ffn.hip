@@ -1112,14 +1112,12 @@ extern "C" int qr_gated_ffn_async(int device, void *stream, int type, int act, s
   if (!few(e, m, n) && (size_t)tiles_of(m, 128) * tiles_of(2 * n, 128) > TILES_MOST)
     return qr_dense_fail(QR_ERR_UNSUPPORTED, "gated ffn: 2^24 tiles of 128 x 64 outputs or more");
   if (!few(e, m, n) && k * e > ROW_BYTES) return qr_dense_fail(QR_ERR_UNSUPPORTED, "gated ffn: rows longer than 4 MB");
-  const void *out[4] = {h, gate, up, workspace};
-  const size_t bytes[4] = {qr_dense_span(m, n, ldh, e), m * n * e, m * n * e, need};
+  // (the workspace as one row)
+  const QrDenseMatrix out[4] = {{h, m, n, ldh}, {gate, m, n, n}, {up, m, n, n}, {workspace, 1, need / e, need / e}},
+                      in[3] = {{x, m, k, ldx}, {w_gate, n, k, ldw}, {w_up, n, k, ldw}};
   for (int i = 0; i < 4; ++i) {
-    QR_DENSE_ARG(!qr_dense_overlap(out[i], bytes[i], x, qr_dense_span(m, k, ldx, e)) &&
-                     !qr_dense_overlap(out[i], bytes[i], w_gate, qr_dense_span(n, k, ldw, e)) &&
-                     !qr_dense_overlap(out[i], bytes[i], w_up, qr_dense_span(n, k, ldw, e)),
-                 "gated ffn: an output lies over an input");
-    for (int j = 0; j < i; ++j) QR_DENSE_ARG(!qr_dense_overlap(out[i], bytes[i], out[j], bytes[j]), "gated ffn: outputs overlap");
+    for (int j = 0; j < 3; ++j) QR_DENSE_ARG(!qr_dense_share(out[i], in[j], e), "gated ffn: an output lies over an input");
+    for (int j = 0; j < i; ++j) QR_DENSE_ARG(!qr_dense_share(out[i], out[j], e), "gated ffn: outputs overlap");
   }
   QR_DENSE_DEVICE(device);
   QrDenseStream s(stream);
@@ -1181,13 +1179,11 @@ extern "C" int qr_gated_ffn_backward_async(int device, void *stream, int type, i
     return qr_dense_fail(QR_ERR_UNSUPPORTED, "gated ffn backward: rows longer than 4 MB");
   if (dx && (size_t)tiles_of(m, 128) * tiles_of(k, 64) > TILES_MOST)
     return qr_dense_fail(QR_ERR_UNSUPPORTED, "gated ffn backward: 2^24 tiles of 128 x 64 elements of dx or more");
-  const void *out[4] = {dx, dw_gate, dw_up, workspace}, *in[6] = {dh, x, w_gate, w_up, gate, up};
-  const size_t ob[4] = {qr_dense_span(m, k, lddx, e), n * k * e, n * k * e, need};
-  const size_t ib[6] = {qr_dense_span(m, n, lddh, e), qr_dense_span(m, k, ldx, e), qr_dense_span(n, k, ldw, e),
-                        qr_dense_span(n, k, ldw, e), m * n * e, m * n * e};
+  const QrDenseMatrix out[4] = {{dx, m, k, lddx}, {dw_gate, n, k, k}, {dw_up, n, k, k}, {workspace, 1, need / e, need / e}},
+                      in[6] = {{dh, m, n, lddh}, {x, m, k, ldx}, {w_gate, n, k, ldw}, {w_up, n, k, ldw}, {gate, m, n, n}, {up, m, n, n}};
   for (int i = 0; i < 4; ++i) {
-    for (int j = 0; j < 6; ++j) QR_DENSE_ARG(!qr_dense_overlap(out[i], ob[i], in[j], ib[j]), "gated ffn backward: an output lies over an input");
-    for (int j = 0; j < i; ++j) QR_DENSE_ARG(!qr_dense_overlap(out[i], ob[i], out[j], ob[j]), "gated ffn backward: outputs overlap");
+    for (int j = 0; j < 6; ++j) QR_DENSE_ARG(!qr_dense_share(out[i], in[j], e), "gated ffn backward: an output lies over an input");
+    for (int j = 0; j < i; ++j) QR_DENSE_ARG(!qr_dense_share(out[i], out[j], e), "gated ffn backward: outputs overlap");
   }
   QR_DENSE_DEVICE(device);
   QrDenseStream s(stream);

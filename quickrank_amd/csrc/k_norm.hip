@@ -457,6 +457,8 @@ extern "C" int qr_layer_norm_async(int device, void *stream, int type, int param
   QR_DENSE_ARG(rows < 2 || ldy >= cols, "layer norm: the stride of y is shorter than a row");
   if (!rows) return QR_OK;
   QR_DENSE_ARG(x && y, "layer norm: x or y is NULL");
+  const QrDenseMatrix mx{x, rows, cols, ldx}, my{y, rows, cols, ldy};
+  QR_DENSE_ARG(qr_dense_in_place(my, mx) || !qr_dense_share(my, mx, qr_dense_size(type)), "layer norm: y lies over x, but not row for row");
   QR_DENSE_DEVICE(device);
   QrDenseStream s(stream);
   qr_dense_dispatch(type, [&](auto t) {
@@ -504,6 +506,10 @@ extern "C" int qr_layer_norm_backward_async(int device, void *stream, int type, 
   size_t need = 0;
   (void)qr_layer_norm_backward_workspace(rows, cols, &need);
   QR_DENSE_ARG(!sums || !rows || (workspace && workspace_bytes >= need), "layer norm backward: the workspace is too small");
+  const QrDenseMatrix mdx{dx, rows, cols, lddx}, in[2] = {{dy, rows, cols, lddy}, {x, rows, cols, ldx}};
+  for (int i = 0; i < 2; ++i)
+    QR_DENSE_ARG(qr_dense_in_place(mdx, in[i]) || !qr_dense_share(mdx, in[i], qr_dense_size(type)),
+                 "layer norm backward: dx lies over dy or x, but not row for row");
   if (!rows && !sums) return QR_OK;
   QR_DENSE_DEVICE(device);
   QrDenseStream s(stream);

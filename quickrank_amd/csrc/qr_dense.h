@@ -81,6 +81,24 @@ inline bool qr_dense_overlap(const void *p, size_t np, const void *q, size_t nq)
   const uintptr_t a = (uintptr_t)p, b = (uintptr_t)q;
   return p && q && np && nq && a < b + nq && b < a + np;
 }
+// A matrix of a call.
+struct QrDenseMatrix {
+  const void *p;
+  size_t rows, cols, ld;
+};
+// Whether two matrices of elements of e bytes may share any.  Exact for rows of one stride, of which one matrix may have the
+// first columns and the other the rest; those of two strides do if their memory from end to end overlaps.
+inline bool qr_dense_share(const QrDenseMatrix &a, const QrDenseMatrix &b, size_t e) {
+  if (!qr_dense_overlap(a.p, qr_dense_span(a.rows, a.cols, a.ld, e), b.p, qr_dense_span(b.rows, b.cols, b.ld, e))) return false;
+  const uintptr_t p = (uintptr_t)a.p, q = (uintptr_t)b.p;
+  if (a.ld != b.ld || a.cols > a.ld || b.cols > a.ld || (p > q ? p - q : q - p) % e) return true;
+  const size_t away = (p > q ? p - q : q - p) / e % a.ld, d = p > q && away ? a.ld - away : away;  // b's first column among a's
+  return d < a.cols || d + b.cols > a.ld;
+}
+// ... of an output that may also be the input itself, row for row
+inline bool qr_dense_in_place(const QrDenseMatrix &out, const QrDenseMatrix &in) {
+  return out.p == in.p && (out.rows < 2 || out.ld == in.ld);
+}
 // rows * cols elements of stride ld stay far below 2^63 bytes
 inline bool qr_dense_spans(size_t rows, size_t cols, size_t ld) {
   const size_t most = (size_t)1 << 58;

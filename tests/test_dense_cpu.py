@@ -222,3 +222,43 @@ def test_ffn_of_more_tiles_than_a_launch_has_threads_for_is_unsupported(L):
         assert ffn_back(L, type=type, m=m, k=k, dh=big >> 1, x=big >> 2, wg=R + Q, wu=8 * R, g=big >> 3, u=big >> 4, dx=big, lddx=k,
                         dwg=16 * R, dwu=32 * R, ws=ws, nbytes=ws) == 5
         assert "tiles" in message(L)
+
+
+# matrices of 4 rows of 8 f32: a row is 32 bytes
+@pytest.mark.parametrize("bad", [dict(y=P, ldy=9), dict(y=P, ldx=0), dict(y=P + 4, ldx=16, ldy=16), dict(y=P + 28, ldx=16, ldy=16),
+                                 dict(y=P + 16, ldx=16, ldy=16), dict(y=P + 64 - 16, ldx=16, ldy=16), dict(y=P + 64 + 4, ldx=16, ldy=16),
+                                 dict(y=P + 8), dict(y=P - 8), dict(y=P + 2, ldx=16, ldy=16)])
+def test_outputs_that_lie_over_an_input_elsewhere_are_refused(L, bad):
+    """Layer norm's and dropout's result may be an input, of one stride, and lie over none otherwise."""
+    assert norm(L, **bad) == ARG and "lies over" in message(L)
+    assert drop(L, **bad) == ARG and "lies over" in message(L)
+    over_residual = {{"x": "r", "ldx": "ldr"}.get(k, k): v for k, v in bad.items()}
+    assert drop(L, **{**dict(x=R, r=P, ldr=8), **over_residual}) == ARG and "lies over" in message(L)
+    back = {{"y": "dx", "ldy": "lddx", "ldx": "lddy"}.get(k, k): v for k, v in bad.items()}
+    assert norm_back(L, **back) == ARG and "lies over" in message(L)
+    back = {{"y": "dx", "ldy": "lddx"}.get(k, k): v for k, v in bad.items()}
+    assert norm_back(L, **{**back, "dy": R, "x": P}) == ARG and "lies over" in message(L)
+
+
+@pytest.mark.parametrize("fine", [dict(y=P), dict(y=P, ldx=16, ldy=16), dict(y=P + 32, ldx=16, ldy=16), dict(y=P - 32, ldx=16, ldy=16),
+                                  dict(y=P + 36, ldx=17, ldy=17), dict(y=P + 64 * 2 + 32, ldx=16, ldy=16), dict(y=P + 128),
+                                  dict(y=P, ldy=9, rows=1)])
+def test_outputs_in_place_and_beside_an_input(L, fine):
+    """Nothing but the device is missing."""
+    if torch.cuda.is_available():
+        pytest.skip("a GPU is visible")
+    assert norm(L, **fine) in (1, ARG) and "device" in message(L)
+    assert drop(L, **fine) in (1, ARG) and "device" in message(L)
+
+
+def test_ffn_outputs_beside_the_inputs(L):
+    """x, h of 4 rows of 8 and 16 in one buffer of rows of 24; dx beside dh: no element is shared.  One element is refused."""
+    if torch.cuda.is_available():
+        pytest.skip("a GPU is visible")
+    W = dict(wg=8 * R, wu=16 * R)
+    assert ffn(L, x=P, ldx=24, h=P + 32, ldh=24, **W) in (1, ARG) and "device" in message(L)
+    assert ffn(L, x=P, ldx=24, h=P + 28, ldh=24, **W) == ARG and "lies over" in message(L)
+    assert ffn(L, x=P, ldx=23, h=P + 32, ldh=23, **W) == ARG and "lies over" in message(L)
+    assert ffn_back(L, dh=P, lddh=24, dx=P + 64, lddx=24, x=64 * R) in (1, ARG) and "device" in message(L)
+    assert ffn_back(L, dh=P, lddh=24, dx=P + 60, lddx=24, x=64 * R) == ARG and "lies over" in message(L)
+    assert ffn_back(L, dh=P, lddh=24, dx=P + 64, lddx=23, x=64 * R) == ARG and "lies over" in message(L)

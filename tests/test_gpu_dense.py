@@ -1009,3 +1009,46 @@ def test_tangents_of_any_argument_are_refused(dense):
                 call()
             assert "tangent" in str(e.value)
         assert torch.equal(dense.layer_norm(x, w)[0], want)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k,n", [(37, 45, 21), (3000, 64, 200), (5000, 136, 264)])
+def test_outputs_beside_the_inputs_in_one_buffer(dense, dtype, m, k, n):
+    """x in the first columns of a buffer and h in the next, dx beside dh, y beside x: the C calls write their columns only."""
+    L, code, s = raw(dense), dense.TYPES[dtype], torch.cuda.current_stream().cuda_stream
+    x, wg, wu = ffn_inputs(1, m, k, n, dtype)
+    e, need = x.element_size(), C.c_size_t()
+
+    def space():
+        return torch.empty(need.value, dtype=torch.uint8, device="cuda")
+    buf = torch.full((m, k + n + 3), 7.0, dtype=dtype, device="cuda")
+    buf[:, :k] = x
+    ld = k + n + 3
+    g, u = torch.empty(2, m, n, dtype=dtype, device="cuda")
+    assert L.qr_gated_ffn_workspace(code, m, k, n, C.byref(need)) == 0
+    ws = space()
+    assert L.qr_gated_ffn_async(0, s, code, 0, m, k, n, buf.data_ptr(), ld, wg.data_ptr(), wu.data_ptr(), k, buf.data_ptr() + k * e, ld,
+                                g.data_ptr(), u.data_ptr(), ws.data_ptr(), need.value) == 0
+    want = dense.gated_ffn(buf[:, :k], wg, wu, save=True)
+    assert torch.equal(buf[:, k:k + n], want[0]) and torch.equal(g, want[1]) and torch.equal(u, want[2])
+    assert torch.equal(buf[:, :k], x) and (buf[:, k + n:] == 7).all()
+    # dh in the first n columns, dx in the next k
+    buf[:, :n] = rand(2, m, n, dtype=dtype)
+    dh = buf[:, :n].clone()
+    dw = torch.empty(2, n, k, dtype=dtype, device="cuda")
+    assert L.qr_gated_ffn_backward_workspace(code, m, k, n, C.byref(need)) == 0
+    ws = space()
+    assert L.qr_gated_ffn_backward_async(0, s, code, 0, m, k, n, buf.data_ptr(), ld, x.data_ptr(), k, wg.data_ptr(), wu.data_ptr(), k,
+                                         g.data_ptr(), u.data_ptr(), buf.data_ptr() + n * e, ld, dw.data_ptr(), dw[1].data_ptr(),
+                                         ws.data_ptr(), need.value) == 0
+    want = dense.gated_ffn_backward(dh, x, wg, wu, g, u)
+    assert torch.equal(buf[:, n:n + k], want[0]) and torch.equal(dw[0], want[1]) and torch.equal(dw[1], want[2])
+    assert torch.equal(buf[:, :n], dh) and (buf[:, k + n:] == 7).all()
+    # y, dropout's y beside x
+    two = torch.full((m, 2 * k + 1), 7.0, dtype=dtype, device="cuda")
+    two[:, :k] = x
+    assert L.qr_layer_norm_async(0, s, code, code, m, k, two.data_ptr(), 2 * k + 1, None, None, 1e-5, two.data_ptr() + k * e, 2 * k + 1,
+                                 None, None) == 0
+    assert torch.equal(two[:, k:2 * k], dense.layer_norm(two[:, :k])[0]) and torch.equal(two[:, :k], x)
+    assert L.qr_dropout_async(0, s, code, m, k, two.data_ptr(), 2 * k + 1, None, 0, two.data_ptr() + k * e, 2 * k + 1, 0.3, 1, 2, None) == 0
+    assert torch.equal(two[:, k:2 * k], dense.dropout(x, 0.3, 1, 2)) and torch.equal(two[:, :k], x) and (two[:, 2 * k:] == 7).all()
