@@ -63,3 +63,23 @@ def test_no_kernel_of_ours_spills_vector_registers_but_the_known_ones(rows):
     spilling = {n: (k.get(".vgpr_spill_count", 0), k.get(".private_segment_fixed_size", 0)) for n, k in ours.items()
                 if k.get(".vgpr_spill_count", 0) or k.get(".private_segment_fixed_size", 0)}
     assert set(spilling) <= {"k_hist_root", "k_obl_plan"}, spilling
+
+
+# the gated unit's product kernel, by (bytes of an element, tile): waves a SIMD that the registers have to leave room for
+DENSE_WAVES = {(2, 64, 64): 5, (2, 128, 64): 4, (2, 128, 128): 2, (2, 256, 128): 2, (2, 256, 256): 2,
+               (4, 64, 64): 4, (4, 128, 64): 4, (4, 128, 96): 3, (4, 128, 128): 2, (4, 128, 160): 2}
+
+
+def test_product_kernels_keep_their_occupancy(rows):
+    """Two workgroups a compute unit (of 256 threads; one of 512) need two waves a SIMD; the narrow tiles more."""
+    import re
+    import kernel_resources as K
+    seen = set()
+    for k in rows.values():
+        m = re.search(r"k_gemmI(f|DF16b|DF16_)LNS_4KindE(\d)ELi(\d+)ELi(\d+)ELi(\d)ELb(\d)E", k[".name"])
+        if m:
+            key = (4 if m[1] == "f" else 2, int(m[3]), int(m[4]))
+            waves = K.waves_per_simd(k.get(".vgpr_count", 0), k.get(".agpr_count", 0))
+            assert waves >= DENSE_WAVES[key] and not k.get(".private_segment_fixed_size", 0), (k[".name"], waves)
+            seen.add(key)
+    assert seen == set(DENSE_WAVES)
