@@ -21,7 +21,7 @@ class NeuralScorer:
         self.rate, self.steps, self.metric, self.cutoff = rate, steps, metric, cutoff
         self.dtype, self.seed, self.device = dtype, seed, torch.device("cuda", device)
         self.ctx = ctx if ctx is not None else Context(device)
-        self.params, self.drawn, self.train_metric = {}, 0, []
+        self.params, self.leaves, self.drawn, self.train_metric = {}, {}, 0, []
 
     def init(self, features):
         """Parameters for rows of `features` values: norms and the last vector in f32, products in self.dtype."""
@@ -38,7 +38,13 @@ class NeuralScorer:
             p[f"gate_{b}"], p[f"up_{b}"] = normal(self.units, features), normal(self.units, features)
             p[f"down_{b}"] = normal(features, self.units)
         p["score"] = torch.randn(features, generator=g, device=self.device) * features ** -0.5
-        self.params = p
+        self.params, self.leaves = p, {}
+
+    def optimizer(self):
+        """Adam over the parameters, in 32 bits: where the operators read 16-bit ones, those are rounded after each step from
+        leaves in f32 (in bf16 a step below 2^-9 of a parameter would be lost, in f16 the square of a gradient)."""
+        self.leaves = {name: v if v.dtype == torch.float32 else v.float() for name, v in self.params.items()}
+        return torch.optim.Adam(list(self.leaves.values()), lr=self.rate)
 
     def _norm(self, z, name):
         return dense.layer_norm(z, self.params[f"norm_{name}.weight"], self.params[f"norm_{name}.bias"])
@@ -90,16 +96,21 @@ class NeuralScorer:
         return out
 
     def step(self, x, optimizer):
-        """One pass over the uploaded training set's rows: scores, their lambdas, the parameters' update."""
+        """One pass over the uploaded training set's rows: scores, their lambdas, the update of the parameters by what
+        optimizer() has given (or, without a call of it, by an optimizer of the parameters themselves)."""
         scores, kept = self.forward(x, train=True)
         self.ctx.set_scores(scores.double().cpu().numpy())
         self.ctx.compute_lambdas(self.metric, self.cutoff)
         lam, _ = self.ctx.get_pseudo()
         # (the pseudo-responses point where the scores should go; an optimizer steps against a gradient)
         grads = self.backward(kept, torch.from_numpy(-lam).to(self.device, torch.float32))
-        for name, param in self.params.items():
-            param.grad = grads[name]
+        leaves = self.leaves or self.params
+        for name, leaf in leaves.items():
+            leaf.grad = grads[name].to(leaf.dtype)
         optimizer.step()
+        for name, param in self.params.items():
+            if param is not leaves[name]:
+                param.copy_(leaves[name])
         self.train_metric.append(self.ctx.metric_last())
 
     def learn(self, x, labels, qoff):
@@ -108,7 +119,7 @@ class NeuralScorer:
         if not self.params:
             self.init(x.shape[1])
         rows = torch.from_numpy(x).to(self.device)
-        optimizer = torch.optim.Adam(list(self.params.values()), lr=self.rate)
+        optimizer = self.optimizer()
         for _ in range(self.steps):
             self.step(rows, optimizer)
         return self

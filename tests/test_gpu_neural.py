@@ -114,3 +114,34 @@ def test_raw_features_keep_their_digits(dtype, shift, scale):
     dz = g + g.mean(1, keepdim=True) + hat.abs() * (g * hat.abs()).mean(1, keepdim=True)
     for name, terms in (("norm_in.weight", dz * hat.abs()), ("norm_in.bias", dz)):
         assert ((grads[name].double() - p[name].grad).abs() <= (8 * half + 4 * own) * 1.1 * terms.sum(0)).all(), name
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16, torch.float16])
+def test_optimizer_holds_32_bits(dtype):
+    """Parameters in 16 bits are rounded from ones in 32 that the optimizer steps, whose moments have 32 bits too: steps below a
+    rounding of a parameter add up, squares of small gradients do not vanish."""
+    x, labels, qoff = make_dataset(nq=12, docs_per_query=25, F=40, seed=3)
+    s = scorer(dtype=dtype, units=24, drop=0.0, steps=60, rate=1e-5)
+    s.init(40)
+    before = {k: v.clone() for k, v in s.params.items()}
+    seen = []
+    plain = torch.optim.Adam
+
+    def adam(*a, **kw):
+        seen.append(plain(*a, **kw))
+        return seen[-1]
+    torch.optim.Adam = adam
+    try:
+        s.learn(x, labels, qoff)
+    finally:
+        torch.optim.Adam = plain
+    state = [v for st in seen[0].state.values() for v in st.values() if v.dim()]
+    assert len(state) == 2 * len(s.params) and all(v.dtype == torch.float32 and torch.isfinite(v).all() for v in state)
+    for name, v in s.params.items():
+        assert v.dtype == before[name].dtype and torch.isfinite(v).all(), name
+    for name in ("gate_0", "up_1", "down_0"):
+        # at least 2^-6: one step of 1e-5 is below half a step of bf16 there (2^-14) and 1.4 half steps of f16 (2^-17)
+        old = before[name].float().abs() >= 2.0 ** -6
+        moved = (s.params[name] != before[name])[old].double().mean()
+        # sixty steps of one direction are 6e-4, ten half steps of bf16's smallest of these and one of its largest (0.3)
+        assert moved > 0.1, (name, float(moved))
