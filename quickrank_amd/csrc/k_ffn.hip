@@ -268,11 +268,12 @@ __device__ __forceinline__ uint32_t lds_offset(const char *p) { return (uint32_t
 // zero-filled.  RAG (FWD, WN = 2): rows at any alignment, both operands through registers.
 //
 // What bounds it, 16-bit types: at 256 x 128 the way from L2 to the compute units (48 bytes a cycle and unit at the full
-// matrix rate, of 64), at 256 x 256 (32 bytes) the matrix cores at the clock that the card holds under them, 1.9 GHz.  1530
-// TF at 8192 x 8192 x (2 x 4096) bf16, where a large library product reaches 1320; 1270 TF at 32768 x 1024 x (2 x 4096),
-// whose 16 stages leave a fifth of a tile's time to its first loads and its results (1020 TF with g and u stored too: 805
-// MB whose writing overlaps little).
-// f32: the six products and the splits before them, whose times add up (matrix cores 59 % busy): 190 to 200 TF.
+// matrix rate, of 64), at 256 x 256 (32 bytes) the matrix cores at the clock that the card holds under them, 1.9 GHz (76 %
+// of the cycles).  1490 TF at 8192 x 8192 x (2 x 4096) bf16, where a large library product reaches 1300; 1240 TF at 32768 x
+// 1024 x (2 x 4096), whose 16 stages leave a fifth of a tile's time to its first loads and its results (1040 TF with g and u
+// stored too: 805 MB whose writing overlaps little).
+// f32: the six products and the splits before them, whose times add up: 190 TF at 4096 x 1024 x (2 x 4096), the matrix cores
+// busy for 50 % of the cycles (37 and 46 % in the gradients of 136 columns, padded to 160).
 template <class T, Kind KIND, int TM, int TN, int WN, bool RAG>
 __global__ __launch_bounds__(128 * WN, 2) void k_gemm(const GemmArgs<T> P) {
   constexpr bool AKS = KIND == DW, BKS = KIND != FWD, BD = WN > 2;
@@ -296,7 +297,6 @@ __global__ __launch_bounds__(128 * WN, 2) void k_gemm(const GemmArgs<T> P) {
 
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave / WN, wn = wave % WN;
-  const T *const a0 = P.a[z];
 
   // a row of the second operand's tile: the output column it makes, and (FWD) of which product
   auto b_row = [&](int r, size_t &row, bool &up) {
