@@ -74,7 +74,7 @@ def build(force=False, verbose=False):
     if verbose:
         print(" ".join(cmd), file=sys.stderr)
     subprocess.check_call(cmd)
-    build_ubench(verbose=verbose)
+    build_ubench(force=force, verbose=verbose)
     return LIB
 
 
